@@ -52,7 +52,7 @@ def listed():
         _adamw("adamw_bert", 32, "float32", _bert(30522, 1024, 24, 4096), clip=True),
         # The same with a quarter of the memory for moments.
         _adamw("adamw8_bert", 8, "float32", _bert(30522, 1024, 24, 4096)),
-        # Parameters and gradients in bf16 with float32 masters, odd sizes, clipped.
+        # Parameters and gradients in bf16, odd sizes, clipped. (The masters are put together as for a checkpoint.)
         _adamw("adamw8_ragged_bf16", 8, "bfloat16", _ragged(301, 400_000, 7), clip=True),
         # The gradients of one 25 MB bucket of BERT-large: many small tensors and a few large ones.
         {"name": "grad_norm_bucket", "kind": "grad_norm", "dtype": "float32", **_ragged(28, 1 << 22, 6)},
@@ -179,9 +179,10 @@ def prepare(case, seed):
     m = 0.3 * normal(total) * scale
     v = scale.square_().mul_(torch.rand(total, device="cuda", generator=gen) + 0.5)
     state = {"kind": "adamw", "bits": case["bits"], "clip": 1.0 if case["clip"] else None, "seed": seed & 0x7FFFFFFF, "step": _STEP,
-             "param": master.to(dtype), "grad": grad}
+             "param": master, "grad": grad}
     if dtype == torch.bfloat16:
-        state["master"] = master
+        state["master"], state["param"] = master, _to_bf16(master)
+        state["remainder"] = master.view(torch.int32).to(torch.int16)  # the low half
     if case["bits"] == 32:
         state["exp_avg"], state["exp_avg_sq"] = m, v
     else:
@@ -201,7 +202,7 @@ def prepare(case, seed):
         for i, (n, at) in enumerate(zip(sizes, places)):
             kept["state"][i] = {"step": torch.tensor(_STEP), **{
                 k: state[k][at:at + n] if not k.endswith("_scale") else state[k][at // 32:at // 32 + -(-n // 32)]
-                for k in ("master", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale") if k in state}}
+                for k in ("remainder", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale") if k in state}}
         optimizer.load_state_dict(kept)
         return {"kind": "adamw", "optimizer": optimizer, "param": state["param"]}
     return state
@@ -225,6 +226,8 @@ def _run_own(state):
         optimizer = state["optimizer"]
         optimizer.step()
         out = {"param": state["param"], **optimizer.state_buffers()[0]}
+        if out.pop("remainder", None) is not None:
+            out["master"] = optimizer.master_buffers()[0]
         if optimizer.grad_norm is not None:
             out["norm"] = optimizer.grad_norm
         return out
@@ -304,6 +307,10 @@ def _to_8_bits(x, bits16, never_zero):
     return code.to(torch.uint8).view(-1).view(torch.float8_e4m3fn), (exponent - 7).to(torch.uint8).view(-1).view(torch.float8_e8m0fnu)
 
 
+def _to_bf16(x):
+    return ((x.view(torch.int32) + 0x8000) >> 16).to(torch.int16).view(torch.bfloat16)
+
+
 def _from_8_bits(x, scale):
     return (x.float().view(-1, 32) * scale.float().unsqueeze(1)).view(-1)
 
@@ -326,7 +333,7 @@ def _adamw_step(state):
     master = state.get("master", state["param"])
     master.copy_(master * (1 - _LR * _DECAY) - _LR / (1 - _BETA1 ** step) * (m / denominator))
     if master is not state["param"]:
-        state["param"].copy_(master)
+        state["param"] = _to_bf16(master)
         out["master"] = master
     if eight:
         bits = _random_bits(m.numel(), state["seed"], step, m.device)
@@ -351,8 +358,7 @@ def work(case):
     n, size = sum(_sizes(case)), _BYTES[case["dtype"]]
     if case["kind"] == "grad_norm":
         return {"bytes": n * size + 4, "flops": 2 * n}
-    values = 8 + size  # the parameter (or its master) there and back, the gradient
-    values += 0 if size == 4 else 2
+    values = 8 + size  # the parameter (with its remainder) there and back, the gradient
     values += 16 if case["bits"] == 32 else 4 * (1 + 1 / 32)
     return {"bytes": n * values, "flops": n * (14 if case["bits"] == 32 else 40)}
 
