@@ -103,6 +103,36 @@ def lib():
     return _LIB
 
 
+_EXTENSIONS = {}
+
+
+def native_extension(name):
+    """lib/<name>.so, an extension module of PyTorch; built first if it does not exist yet. There is nothing in Python to
+    take its place: where it can be neither built nor loaded this raises."""
+    module = _EXTENSIONS.get(name)
+    if module is None:
+        with _LOCK:
+            if name not in _EXTENSIONS:
+                import importlib.util
+                import torch  # noqa: F401  (the extension needs its libraries)
+                path = library_path(name + ".so")
+                try:
+                    if not os.path.exists(path):
+                        spec = importlib.util.spec_from_file_location("_switchml_build", os.path.join(_HERE, "build.py"))
+                        mod = importlib.util.module_from_spec(spec)
+                        spec.loader.exec_module(mod)
+                        mod.build(programs=False)
+                        mod.build_torch_extension()
+                    spec = importlib.util.spec_from_file_location(name, path)
+                    module = importlib.util.module_from_spec(spec)
+                    spec.loader.exec_module(module)
+                except (ImportError, OSError, RuntimeError) as e:
+                    raise NativeError("cannot load %s: %s" % (path, e))
+                _EXTENSIONS[name] = module
+            module = _EXTENSIONS[name]
+    return module
+
+
 def last_error():
     return lib().sml_last_error().decode(errors="replace")
 

@@ -8,8 +8,10 @@ Products (all inside this directory, never installed elsewhere):
     lib/libswitchml_b200.so        core + CPU backends + CUDA backend + C interface
     lib/libswitchml_b200.a         the same as a static archive
     lib/libswitchml_gemm.so        tcgen05 weight-gradient GEMM (loaded on demand)
+    lib/libswitchml_train.so       layer norm, gradient norm, AdamW (loaded on demand)
     lib/torch_switchml.so          native c10d backend for PyTorch (python build.py --torch)
     lib/torch_switchml_linear.so   autograd node of FusedWgradLinear (python build.py --torch)
+    lib/torch_switchml_train.so    layer norm, gradient norm and AdamW for PyTorch (python build.py --torch)
     lib/torch_switchml_jobs.so     submission of torch tensors without Python (python build.py --torch)
     build-checked/libswitchml_b200.so   the library with the kernels' bounds checks (--checked)
     lib/libnccl-net-switchml.so    NCCL collective-network plugin (bin/collnet_harness drives it)
@@ -59,6 +61,7 @@ LIB_SOURCES = [
     "csrc/capi/switchml_c.cc",
 ]
 GEMM_SOURCES = ["csrc/kernels/wgrad_gemm.cu", "csrc/kernels/linear_ops.cu"]
+TRAIN_SOURCES = ["csrc/kernels/layer_norm.cu", "csrc/kernels/adamw.cu"]
 NCCL_PLUGIN_SOURCES = ["csrc/nccl/collnet_plugin.cc"]
 PROGRAMS = {
     "switchml_switchd": ["controller/switchd.cc"],
@@ -124,7 +127,8 @@ def build(jobs=None, verbose=False, programs=True):
     progs = {k: v for k, v in PROGRAMS.items()
              if programs and all(os.path.exists(os.path.join(ROOT, s)) for s in v)}
     plugin = [s for s in NCCL_PLUGIN_SOURCES if os.path.exists(os.path.join(ROOT, s))]
-    every = sources + gemm + plugin + [s for v in progs.values() for s in v]
+    train = [s for s in TRAIN_SOURCES if os.path.exists(os.path.join(ROOT, s))]
+    every = sources + gemm + train + plugin + [s for v in progs.values() for s in v]
     errors = []
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
         for obj, err in ex.map(lambda s: _compile(s, hdr, verbose), every):
@@ -148,11 +152,10 @@ def build(jobs=None, verbose=False, programs=True):
         if os.path.exists(static_lib):
             os.remove(static_lib)
         _link(["ar", "rcs", static_lib] + objs, verbose)
-    if gemm:
-        gemm_lib = os.path.join(LIB, "libswitchml_gemm.so")
-        gobjs = [_obj_path(s) for s in gemm]
-        if newer(gemm_lib, gobjs):
-            _link([NVCC] + ARCH + ["-shared", "-o", gemm_lib] + gobjs + ["-lpthread", "-ldl", "-lrt"], verbose)
+    for name, srcs in (("libswitchml_gemm.so", gemm), ("libswitchml_train.so", train)):
+        target, tobjs = os.path.join(LIB, name), [_obj_path(s) for s in srcs]
+        if srcs and newer(target, tobjs):
+            _link([NVCC] + ARCH + ["-shared", "-o", target] + tobjs + ["-lpthread", "-ldl", "-lrt"], verbose)
     if plugin:
         # NCCL looks for libnccl-net-<NCCL_NET_PLUGIN>.so on the library path.
         plugin_lib = os.path.join(LIB, "libnccl-net-switchml.so")
@@ -242,12 +245,14 @@ def build_checked(verbose=False, jobs=None):
 # Extensions of PyTorch: product, source, libraries of this package that it links.
 TORCH_EXTENSIONS = [("torch_switchml", "csrc/torch/process_group_sml.cc", ["switchml_b200"]),
                     ("torch_switchml_linear", "csrc/torch/fused_linear.cc", ["switchml_gemm"]),
+                    ("torch_switchml_train", "csrc/torch/train_ops.cc", ["switchml_train"]),
                     ("torch_switchml_jobs", "csrc/torch/jobs.cc", [])]
 
 
 def build_torch_extension(verbose=False):
     """lib/torch_switchml.so, the native c10d backend, lib/torch_switchml_linear.so, the autograd node of
-    FusedWgradLinear, and lib/torch_switchml_jobs.so, submission without Python. Needs the headers and libraries of the installed PyTorch; returns None (with a note) when
+    FusedWgradLinear, lib/torch_switchml_train.so, layer norm and the optimizer's step, and
+    lib/torch_switchml_jobs.so, submission without Python. Needs the headers and libraries of the installed PyTorch; returns None (with a note) when
     they are not usable, else the path of the former."""
     try:
         import torch
@@ -281,7 +286,7 @@ def build_torch_extension(verbose=False):
         os.replace(part, out)
         return out
 
-    with cf.ThreadPoolExecutor(max_workers=3) as ex:
+    with cf.ThreadPoolExecutor(max_workers=len(TORCH_EXTENSIONS)) as ex:
         return list(ex.map(lambda e: one(*e), TORCH_EXTENSIONS))[0]
 
 

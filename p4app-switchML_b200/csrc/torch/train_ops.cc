@@ -1,0 +1,304 @@
+// lib/torch_switchml_train.so: the operators of a training step around its gradients, for ops/layer_norm.py and
+// ops/adamw.py. Arguments are checked and kernels launched without Python: a step of BERT-large's optimizer has 298
+// parameters to ask for their gradients, and layer norm's backward pass runs on the engine's thread.
+#include <ATen/autocast_mode.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include <algorithm>
+#include <array>
+#include <vector>
+
+#include "kernels/adamw.h"
+#include "kernels/layer_norm.h"
+
+namespace {
+
+using torch::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using OptTensor = std::optional<Tensor>;
+
+void* CurrentStream() { return at::cuda::getCurrentCUDAStream().stream(); }
+
+void Check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed: ", rc == -4 ? "kernel launch" : "bad argument"); }
+
+bool Known(const Tensor& t) { return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16; }
+
+int NormType(const Tensor& t) { return t.scalar_type() == at::kFloat ? SML_NORM_F32 : SML_NORM_BF16; }
+
+void* Data(const Tensor& t) { return t.defined() ? const_cast<void*>(t.const_data_ptr()) : nullptr; }
+
+// ---- layer norm ----
+
+constexpr int64_t kMaxFeatures = 1 << 30;
+
+void CheckParameter(const Tensor& p, const char* name, const Tensor& x, const Tensor& other) {
+  if (!p.defined()) return;
+  TORCH_CHECK_VALUE(p.device() == x.device(), "layer_norm: ", name, " is on ", p.device(), ", x on ", x.device());
+  TORCH_CHECK_VALUE(p.dim() == 1 && p.size(0) == x.size(-1), "layer_norm: ", name, " has the shape ", p.sizes(), ", the last dimension of x is ",
+              x.size(-1));
+  TORCH_CHECK_TYPE(p.scalar_type() == at::kFloat || p.scalar_type() == x.scalar_type(), "layer_norm: ", name, " is ", p.scalar_type(),
+              ": float32 or the type of x (", x.scalar_type(), ") is wanted");
+  TORCH_CHECK_TYPE(!other.defined() || other.scalar_type() == p.scalar_type(), "layer_norm: weight and bias are of different types");
+}
+
+class LayerNorm : public torch::autograd::Function<LayerNorm> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Tensor& x_in, const OptTensor& residual_in, const OptTensor& weight_in,
+                               const OptTensor& bias_in, double eps, bool backward_comes) {
+    const c10::cuda::OptionalCUDAGuard device(x_in.device());
+    const bool add = residual_in.has_value();
+    const Tensor x = x_in.contiguous(), residual = add ? residual_in->contiguous() : Tensor();
+    const Tensor weight = weight_in ? weight_in->contiguous() : Tensor(), bias = bias_in ? bias_in->contiguous() : Tensor();
+    const int64_t n = x.size(-1), rows = x.numel() / n;
+    Tensor y = at::empty_like(x), sum = add ? at::empty_like(x) : Tensor(), stats;
+    if (backward_comes) stats = at::empty({2, rows}, x.options().dtype(at::kFloat));
+    float* mean = backward_comes ? stats.data_ptr<float>() : nullptr;
+    if (rows > 0) {
+      const Tensor& p = weight.defined() ? weight : bias;
+      Check(switchml_layer_norm_forward(Data(x), Data(residual), Data(weight), Data(bias), y.data_ptr(), Data(sum), mean,
+                                        mean ? mean + rows : nullptr, rows, static_cast<int>(n), static_cast<float>(eps), NormType(x),
+                                        p.defined() ? NormType(p) : SML_NORM_F32, CurrentStream()),
+            "layer_norm");
+    }
+    if (backward_comes) {
+      ctx->save_for_backward({add ? sum : x, weight, stats});
+      ctx->saved_data["residual"] = add;
+      ctx->saved_data["bias"] = bias.defined();
+      ctx->saved_data["bias_bf16"] = bias.defined() && bias.scalar_type() == at::kBFloat16;
+      ctx->set_materialize_grads(false);
+    }
+    if (add) return {y, sum};
+    return {y};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "layer_norm has no gradient of its gradient (create_graph)");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &s = saved[0], &weight = saved[1], &stats = saved[2];
+    const bool bias = ctx->saved_data["bias"].toBool();
+    // needs_input_grad() counts the tensors that were given.
+    const size_t residual_edge = 1, weight_edge = 1 + ctx->saved_data["residual"].toBool(), bias_edge = weight_edge + weight.defined();
+    const bool want_weight = weight.defined() && ctx->needs_input_grad(weight_edge), want_bias = bias && ctx->needs_input_grad(bias_edge);
+    const c10::cuda::OptionalCUDAGuard device(s.device());
+    const Tensor dsum = grads.size() > 1 && grads[1].defined() ? grads[1].contiguous() : Tensor();
+    Tensor dx, dweight, dbias;
+    if (!grads[0].defined()) {  // only the sum was used
+      dx = dsum;
+    } else {
+      const Tensor dy = grads[0].contiguous();
+      const int64_t n = s.size(-1), rows = s.numel() / n;
+      const auto ptype = weight.defined() ? weight.scalar_type() : ctx->saved_data["bias_bf16"].toBool() ? at::kBFloat16 : at::kFloat;
+      dx = at::empty_like(s);
+      if (want_weight) dweight = at::empty({n}, s.options().dtype(ptype));
+      if (want_bias) dbias = at::empty({n}, s.options().dtype(ptype));
+      if (rows > 0) {
+        Tensor workspace;
+        if (want_weight || want_bias)
+          workspace = at::empty({switchml_layer_norm_workspace(rows, static_cast<int>(n), NormType(s))}, s.options().dtype(at::kFloat));
+        const float* mean = stats.const_data_ptr<float>();
+        Check(switchml_layer_norm_backward(Data(dy), Data(dsum), Data(s), Data(weight), mean, mean + rows, dx.data_ptr(), Data(dweight),
+                                           Data(dbias), static_cast<float*>(Data(workspace)), rows, static_cast<int>(n), NormType(s),
+                                           ptype == at::kFloat ? SML_NORM_F32 : SML_NORM_BF16, CurrentStream()),
+              "layer_norm");
+      } else {
+        if (dweight.defined()) dweight.zero_();
+        if (dbias.defined()) dbias.zero_();
+      }
+    }
+    const bool want_residual = weight_edge == 2 && ctx->needs_input_grad(residual_edge);
+    return {ctx->needs_input_grad(0) ? dx : Tensor(), want_residual ? dx : Tensor(), dweight, dbias, Tensor(), Tensor()};
+  }
+};
+
+variable_list LayerNormForward(Tensor x, OptTensor residual, const OptTensor& weight, const OptTensor& bias, double eps) {
+  const bool autocast = x.is_cuda() && at::autocast::is_autocast_enabled(at::kCUDA);
+  c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::DispatchKey::AutocastCUDA);
+  if (autocast) {
+    const auto type = at::autocast::get_autocast_dtype(at::kCUDA);
+    if (x.is_floating_point()) x = x.to(type);
+    if (residual && residual->is_floating_point()) residual = residual->to(type);
+  }
+  TORCH_CHECK_TYPE(Known(x), "layer_norm: x is ", x.scalar_type(), ": float32 or bfloat16 is wanted");
+  TORCH_CHECK_VALUE(x.is_cuda(), "layer_norm: x is on ", x.device(), ": a CUDA device is wanted");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= kMaxFeatures, "layer_norm: x has the shape ", x.sizes(),
+                    ": a last dimension of 1 to 2^30 is wanted");
+  TORCH_CHECK_VALUE(eps >= 0, "layer_norm: eps is ", eps);
+  if (residual) {
+    TORCH_CHECK_VALUE(residual->device() == x.device() && residual->scalar_type() == x.scalar_type() && residual->sizes() == x.sizes(),
+                      "layer_norm: the residual is ", residual->scalar_type(), " ", residual->sizes(), " on ", residual->device(), ", x is ",
+                      x.scalar_type(), " ", x.sizes(), " on ", x.device());
+  }
+  CheckParameter(weight.value_or(Tensor()), "weight", x, Tensor());
+  CheckParameter(bias.value_or(Tensor()), "bias", x, weight.value_or(Tensor()));
+  const auto wants = [](const OptTensor& t) { return t && t->requires_grad(); };
+  const bool backward_comes = at::GradMode::is_enabled() && (x.requires_grad() || wants(residual) || wants(weight) || wants(bias));
+  return LayerNorm::apply(x, residual, weight, bias, eps, backward_comes);
+}
+
+// ---- gradient norm ----
+
+int AdamwType(const Tensor& t) { return t.scalar_type() == at::kFloat ? SML_ADAMW_F32 : SML_ADAMW_BF16; }
+
+// Same values in the same places of memory, without gaps: what an elementwise pass over memory may take.
+bool Dense(const Tensor& t) { return t.is_non_overlapping_and_dense(); }
+
+void NormOf(const std::vector<SmlNormTensor>& list, Tensor* workspace, const Tensor& out) {
+  const int64_t doubles = std::max<int64_t>(1, switchml_grad_norm_workspace(static_cast<int>(list.size())));
+  if (!workspace->defined() || workspace->numel() < doubles) *workspace = at::empty({doubles}, out.options().dtype(at::kDouble));
+  Check(switchml_grad_norm(list.data(), static_cast<int>(list.size()), workspace->data_ptr<double>(), out.data_ptr<float>(), CurrentStream()),
+        "grad_norm");
+}
+
+Tensor GradNorm(const std::vector<Tensor>& tensors) {
+  TORCH_CHECK_VALUE(!tensors.empty(), "grad_norm: no tensors");
+  std::vector<SmlNormTensor> list;
+  std::vector<Tensor> keep;
+  list.reserve(tensors.size());
+  for (const Tensor& t : tensors) {
+    TORCH_CHECK_TYPE(t.layout() == at::kStrided && Known(t), "grad_norm: a tensor is ", t.layout(), " ", t.scalar_type(),
+                     ": strided float32 or bfloat16 is wanted");
+    TORCH_CHECK_VALUE(t.is_cuda() && t.device() == tensors[0].device(), "grad_norm: tensors on ", tensors[0].device(), " and ", t.device(),
+                      ": one CUDA device is wanted");
+  }
+  const c10::cuda::OptionalCUDAGuard device(tensors[0].device());
+  at::NoGradGuard no_grad;
+  for (const Tensor& t : tensors) {
+    if (!Dense(t)) keep.push_back(t.contiguous());
+    const Tensor& use = Dense(t) ? t : keep.back();
+    list.push_back({Data(use), use.numel(), AdamwType(use)});
+  }
+  Tensor out = at::empty({}, tensors[0].options().dtype(at::kFloat).requires_grad(false)), workspace;
+  NormOf(list, &workspace, out);
+  return out;
+}
+
+// ---- AdamW ----
+
+struct Group {
+  std::vector<Tensor> params;
+  std::vector<int64_t> numel, place;  // place: in units of SML_ADAMW_ALIGN values
+  Tensor exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, remainder, steps;
+  int64_t first = 0;
+};
+
+class Adamw {
+ public:
+  Adamw(int bits, int64_t seed) : bits_(bits), seed_(static_cast<unsigned>(seed)) {}
+
+  void AddGroup(std::vector<Tensor> params, std::vector<int64_t> place, Tensor exp_avg, Tensor exp_avg_sq, OptTensor exp_avg_scale,
+                OptTensor exp_avg_sq_scale, OptTensor remainder, Tensor steps, int64_t first) {
+    Group g;
+    for (const Tensor& p : params) g.numel.push_back(p.numel());
+    g.params = std::move(params), g.place = std::move(place);
+    g.exp_avg = std::move(exp_avg), g.exp_avg_sq = std::move(exp_avg_sq), g.steps = std::move(steps), g.first = first;
+    g.exp_avg_scale = exp_avg_scale.value_or(Tensor()), g.exp_avg_sq_scale = exp_avg_sq_scale.value_or(Tensor());
+    g.remainder = remainder.value_or(Tensor());
+    if (!ticket_.defined()) {
+      ticket_ = at::zeros({1}, g.exp_avg.options().dtype(at::kInt));
+      norm_ = at::zeros({}, g.exp_avg.options().dtype(at::kFloat));
+    }
+    groups_.push_back(std::move(g));
+  }
+
+  // settings: (lr, beta1, beta2, eps, weight decay) of every group; lr_tensors: lr in device memory, or None.
+  void Step(const std::vector<std::array<double, 5>>& settings, const std::vector<OptTensor>& lr_tensors, std::optional<double> max_norm) {
+    TORCH_CHECK(settings.size() == groups_.size() && lr_tensors.size() == groups_.size(), "FusedAdamW: groups have come or gone");
+    const c10::cuda::OptionalCUDAGuard device(ticket_.device());
+    at::NoGradGuard no_grad;
+    tensors_.clear(), norms_.clear();
+    std::vector<Tensor> keep, grads;
+    struct Run { size_t begin, end; int type; };
+    std::vector<std::pair<size_t, Run>> runs;  // of tensors whose gradients are of one type, by group
+    for (size_t k = 0; k < groups_.size(); k++) {
+      Group& g = groups_[k];
+      for (const int type : {SML_ADAMW_F32, SML_ADAMW_BF16}) {
+        const size_t begin = tensors_.size();
+        for (size_t i = 0; i < g.params.size(); i++) {
+          const Tensor& p = g.params[i];
+          if (AdamwType(p) != type) continue;
+          Tensor grad = p.grad();
+          if (!grad.defined()) continue;
+          CheckGrad(p, grad, g.numel[i]);
+          if (!(p.is_contiguous() && grad.is_contiguous()) && p.strides() != grad.strides()) {
+            grad = at::empty_strided(p.sizes(), p.strides(), grad.options()).copy_(grad);
+            keep.push_back(grad);
+          }
+          tensors_.push_back({Data(p), Data(grad), g.numel[i], static_cast<unsigned>(g.place[i]), static_cast<int>(i)});
+          if (max_norm) norms_.push_back({Data(grad), g.numel[i], type});
+          p.unsafeGetTensorImpl()->bump_version();
+        }
+        if (tensors_.size() > begin) runs.push_back({k, {begin, tensors_.size(), type}});
+      }
+    }
+    if (max_norm) NormOf(norms_, &workspace_, norm_);
+    for (const auto& [k, run] : runs) {
+      const Group& g = groups_[k];
+      const auto bytes = [](const Tensor& t) { return static_cast<unsigned char*>(Data(t)); };
+      const SmlAdamwState state{Data(g.exp_avg), Data(g.exp_avg_sq), bytes(g.exp_avg_scale), bytes(g.exp_avg_sq_scale),
+                                static_cast<short*>(Data(g.remainder)), g.steps.data_ptr<int>(), ticket_.data_ptr<int>(), bits_, seed_, static_cast<unsigned long long>(g.first)};
+      const auto& s = settings[k];
+      const SmlAdamwStep step{s[0], s[1], s[2], s[3], s[4], lr_tensors[k] ? lr_tensors[k]->const_data_ptr<float>() : nullptr,
+                              max_norm ? norm_.data_ptr<float>() : nullptr, static_cast<float>(max_norm.value_or(0.0))};
+      Check(switchml_adamw_step(&tensors_[run.begin], static_cast<int>(run.end - run.begin), &state, &step, run.type, CurrentStream()),
+            "FusedAdamW");
+    }
+  }
+
+  // The fp32 values of a group's parameters, in the layout of its state.
+  Tensor Masters(size_t k) {
+    const c10::cuda::OptionalCUDAGuard device(ticket_.device());
+    const Group& g = groups_.at(k);
+    Tensor out = at::zeros({g.exp_avg.numel()}, g.exp_avg.options().dtype(at::kFloat));
+    for (const int type : {SML_ADAMW_F32, SML_ADAMW_BF16}) {
+      tensors_.clear();
+      for (size_t i = 0; i < g.params.size(); i++) {
+        CheckParam(g.params[i], g.numel[i]);
+        if (AdamwType(g.params[i]) == type)
+          tensors_.push_back({Data(g.params[i]), nullptr, g.numel[i], static_cast<unsigned>(g.place[i]), static_cast<int>(i)});
+      }
+      if (tensors_.empty()) continue;
+      Check(switchml_adamw_masters(tensors_.data(), static_cast<int>(tensors_.size()), static_cast<short*>(Data(g.remainder)),
+                                   out.data_ptr<float>(), type, CurrentStream()),
+            "FusedAdamW");
+    }
+    return out;
+  }
+
+  Tensor norm() const { return norm_; }
+
+ private:
+  static void CheckParam(const Tensor& p, int64_t numel) {
+    TORCH_CHECK(p.numel() == numel && Dense(p), "FusedAdamW: a parameter has another size or other strides than when its state was made");
+  }
+  static void CheckGrad(const Tensor& p, const Tensor& grad, int64_t numel) {
+    TORCH_CHECK(grad.layout() == at::kStrided, "FusedAdamW: a gradient is ", grad.layout(), ": strided is wanted");
+    TORCH_CHECK(grad.scalar_type() == p.scalar_type() && grad.device() == p.device() && grad.sizes() == p.sizes(),
+                "FusedAdamW: a parameter is ", p.scalar_type(), " ", p.sizes(), " on ", p.device(), ", its gradient ", grad.scalar_type(), " ",
+                grad.sizes(), " on ", grad.device());
+    CheckParam(p, numel);
+  }
+
+  const int bits_;
+  const unsigned seed_;
+  std::vector<Group> groups_;
+  Tensor ticket_, norm_, workspace_;
+  std::vector<SmlAdamwTensor> tensors_;
+  std::vector<SmlNormTensor> norms_;
+};
+
+}  // namespace
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.def("layer_norm", &LayerNormForward);
+  m.def("grad_norm", &GradNorm);
+  m.attr("ALIGN") = static_cast<int>(SML_ADAMW_ALIGN);
+  py::class_<Adamw>(m, "Adamw")
+      .def(py::init<int, int64_t>())
+      .def("add_group", &Adamw::AddGroup)
+      .def("step", &Adamw::Step)
+      .def("masters", &Adamw::Masters)
+      .def_property_readonly("norm", &Adamw::norm);
+}

@@ -2,7 +2,8 @@
 FFN 4096, vocabulary 30522, ~335 M parameters. Attention uses
 ``scaled_dot_product_attention``; with ``fused_ffn=True`` the two FFN projections of
 every layer compute their weight gradients with the tcgen05 GEMM fused with the cross-GPU
-reduction (ops/wgrad.py)."""
+reduction (ops/wgrad.py); with ``fused_norm=True`` every layer norm takes the residual sum in front of it
+into its kernel, forward and backward (ops/layer_norm.py; under autocast the residual stream is then of its type)."""
 import math
 from dataclasses import dataclass
 
@@ -10,6 +11,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from ..ops.layer_norm import FusedLayerNorm
 from ..ops.wgrad import FusedWgradLinear
 
 
@@ -24,6 +26,15 @@ class BertConfig:
     type_vocab: int = 2
     dropout: float = 0.1
     fused_ffn: bool = False
+    fused_norm: bool = False
+
+
+def _norm(c):
+    return (FusedLayerNorm if c.fused_norm else nn.LayerNorm)(c.hidden, eps=1e-12)
+
+
+def _add_and_norm(norm, x, h):
+    return norm(h, x) if isinstance(norm, FusedLayerNorm) else norm(x + h)
 
 
 class Layer(nn.Module):
@@ -33,10 +44,10 @@ class Layer(nn.Module):
         self.heads = c.heads
         self.qkv = nn.Linear(c.hidden, 3 * c.hidden)
         self.proj = nn.Linear(c.hidden, c.hidden)
-        self.ln1 = nn.LayerNorm(c.hidden, eps=1e-12)
+        self.ln1 = _norm(c)
         self.ffn1 = lin(c.hidden, c.ffn)
         self.ffn2 = lin(c.ffn, c.hidden)
-        self.ln2 = nn.LayerNorm(c.hidden, eps=1e-12)
+        self.ln2 = _norm(c)
         self.drop = nn.Dropout(c.dropout)
 
     def forward(self, x):
@@ -44,8 +55,8 @@ class Layer(nn.Module):
         q, k, v = self.qkv(x).view(b, s, 3, self.heads, h // self.heads).permute(2, 0, 3, 1, 4)
         a = F.scaled_dot_product_attention(q, k, v, dropout_p=self.drop.p if self.training else 0.0)
         a = a.transpose(1, 2).reshape(b, s, h)
-        x = self.ln1(x + self.drop(self.proj(a)))
-        return self.ln2(x + self.drop(self.ffn2(F.gelu(self.ffn1(x)))))
+        x = _add_and_norm(self.ln1, x, self.drop(self.proj(a)))
+        return _add_and_norm(self.ln2, x, self.drop(self.ffn2(F.gelu(self.ffn1(x)))))
 
 
 class BertForMaskedLM(nn.Module):
@@ -55,11 +66,11 @@ class BertForMaskedLM(nn.Module):
         self.tok = nn.Embedding(c.vocab_size, c.hidden)
         self.pos = nn.Embedding(c.max_pos, c.hidden)
         self.typ = nn.Embedding(c.type_vocab, c.hidden)
-        self.ln = nn.LayerNorm(c.hidden, eps=1e-12)
+        self.ln = _norm(c)
         self.drop = nn.Dropout(c.dropout)
         self.layers = nn.ModuleList([Layer(c) for _ in range(c.layers)])
         self.head_dense = nn.Linear(c.hidden, c.hidden)
-        self.head_ln = nn.LayerNorm(c.hidden, eps=1e-12)
+        self.head_ln = _norm(c)
         self.head_bias = nn.Parameter(torch.zeros(c.vocab_size))
         self.apply(self._init)
 
@@ -86,5 +97,5 @@ class BertForMaskedLM(nn.Module):
         return F.cross_entropy(logits.view(-1, logits.shape[-1]).float(), labels.view(-1), ignore_index=-100)
 
 
-def bert_large(fused_ffn=False, **overrides):
-    return BertForMaskedLM(BertConfig(fused_ffn=fused_ffn, **overrides))
+def bert_large(fused_ffn=False, fused_norm=False, **overrides):
+    return BertForMaskedLM(BertConfig(fused_ffn=fused_ffn, fused_norm=fused_norm, **overrides))

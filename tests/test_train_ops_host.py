@@ -1,0 +1,98 @@
+"""Host side of ops/layer_norm.py and ops/adamw.py: what is refused before a kernel is launched, and the arithmetic of
+moments in 8 bits, in its plain form."""
+import math
+
+import pytest
+import torch
+
+from _train_reference import decode, encode, random_bits
+from switchml_b200.ops.adamw import FusedAdamW, dequantized, grad_norm
+from switchml_b200.ops.layer_norm import FusedLayerNorm, layer_norm
+
+
+def test_layer_norm_refuses():
+    x = torch.zeros(2, 8)
+    with pytest.raises(ValueError, match="CUDA"):
+        layer_norm(x)
+    with pytest.raises(TypeError, match="float32 or bfloat16"):
+        layer_norm(x.half())
+    with pytest.raises(ValueError):
+        FusedLayerNorm((2, 8))
+
+
+def test_grad_norm_refuses():
+    with pytest.raises(ValueError):
+        grad_norm([])
+    with pytest.raises(ValueError, match="CUDA"):
+        grad_norm([torch.zeros(3)])
+    with pytest.raises(TypeError):
+        grad_norm([torch.zeros(3, dtype=torch.int32)])
+    with pytest.raises(TypeError):
+        grad_norm([torch.eye(3).to_sparse()])
+
+
+@pytest.mark.parametrize("options", [{"state_bits": 16}, {"max_norm": 0.0}, {"max_norm": float("nan")}, {"seed": -1}, {"seed": 1 << 32},
+                                     {}, {"lr": -1.0}])
+def test_adamw_refuses(options):
+    with pytest.raises(ValueError):
+        FusedAdamW([torch.nn.Parameter(torch.zeros(4))], **options)
+
+
+def test_adamw_refuses_types():
+    with pytest.raises(TypeError):
+        FusedAdamW([torch.nn.Parameter(torch.zeros(4, dtype=torch.float16))])
+
+
+def test_random_bits_are_uniform_and_independent():
+    """Means and correlations of 2^18 values lie within 5 standard deviations."""
+    n = 1 << 18
+    halves = []
+    for step in (1, 2, 1000):
+        h = random_bits(0, n, 7, step)
+        for half in (h & 0xFFFF, h >> 16):
+            u = (half.double() + 0.5) / 65536 - 0.5
+            assert abs(u.mean()) < 5 / math.sqrt(12 * n)
+            for lag in (1, 2, 32, 256):
+                assert abs((u[lag:] * u[:-lag]).mean()) < 5 / 12 / math.sqrt(n)
+            halves.append(u)
+    for i in range(len(halves)):
+        for j in range(i):
+            assert abs((halves[i] * halves[j]).mean()) < 5 / 12 / math.sqrt(n)
+
+
+def test_rounding_to_8_bits():
+    """Every value becomes one of its two neighbours among the codes, and their mean is the value."""
+    torch.manual_seed(0)
+    x = torch.randn(64, 32).abs() * torch.exp(3 * torch.randn(64, 1))
+    x[0, 0], x[1] = 0.0, 0.0
+    flat = x.reshape(-1)
+    total, n = torch.zeros(flat.numel(), dtype=torch.float64), 2000
+    for step in range(n):
+        codes, scales = encode(flat, random_bits(0, flat.numel(), 3, step) & 0xFFFF, False)
+        got = decode(codes, scales)
+        total += got.double()
+        biggest = torch.exp2(torch.floor(torch.log2(x.amax(1, keepdim=True).clamp(min=2.0 ** -100)))) / 128
+        step_size = torch.maximum(torch.exp2(torch.floor(torch.log2(x.clamp(min=2.0 ** -120))) - 3), biggest * 2.0 ** -9).reshape(-1)
+        assert ((got - flat).abs() <= step_size).all()
+    assert (got[flat == 0] == 0).all()
+    # The mean of n values that are at most a step apart: 6 standard deviations of at most half a step each.
+    assert ((total / n - flat).abs() <= 6 * 0.5 / math.sqrt(n) * step_size + 1e-30).all()
+    # A block that is on codes already comes back unchanged, whatever the random bits.
+    again, scales2 = encode(got, random_bits(5, flat.numel(), 9, 1) & 0xFFFF, False)
+    assert torch.equal(decode(again, scales2), got)
+
+
+def test_second_moments_stay_above_zero():
+    v = torch.full((32,), 1e-30)
+    v[0] = 1.0
+    v[5] = 0.0
+    codes, scales = encode(v, torch.zeros(32, dtype=torch.int64), True)
+    got = decode(codes, scales)
+    assert got[5] == 0 and (got[torch.arange(32) != 5] > 0).all()
+
+
+def test_dequantized_on_the_cpu():
+    codes = torch.arange(0, 120, dtype=torch.uint8).view(4, 30)
+    scales = torch.tensor([127, 128, 126, 127], dtype=torch.uint8)
+    got = dequantized(codes.view(torch.float8_e4m3fn), scales.view(torch.float8_e8m0fnu))
+    assert torch.equal(got.reshape(-1), decode(codes.view(-1), scales))
