@@ -9,6 +9,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "kernels/adamw.h"
 #include "kernels/dependent_launch.cuh"
 
@@ -72,15 +74,21 @@ struct Factors {
   unsigned key;
 };
 
-__device__ __forceinline__ Factors FactorsOf(const StepArgs& a, int t, float lr, unsigned long long value) {
+__device__ __forceinline__ Factors FactorsOf(const StepArgs& a, int t, float lr) {
   Factors f;
   // 1 - beta^t = -expm1(t log beta): the logarithm comes from the host in more than fp32, and expm1 keeps what a
   // difference from 1 would lose.
   f.size = lr / -expm1f(t * a.log_beta1);
   f.rsqrt2 = 1.f / sqrtf(-expm1f(t * a.log_beta2));
   f.keep = 1.f - lr * a.decay;
-  f.key = Mix(Mix(Mix(a.state.seed) + static_cast<unsigned>(t)) + static_cast<unsigned>(value >> 32));
+  f.key = Mix(Mix(a.state.seed) + static_cast<unsigned>(t));
   return f;
+}
+
+// What is hashed for the value at `place` of the flat buffers; for the next 255 behind a multiple of 256 it counts on.
+__device__ __forceinline__ unsigned HashedAt(const StepArgs& a, const Factors& f, long long place) {
+  const unsigned long long value = a.state.first + place;
+  return static_cast<unsigned>(value) + Mix(f.key + static_cast<unsigned>(value >> 32));
 }
 
 // The code (without sign) of a magnitude over its scale.
@@ -91,11 +99,221 @@ __device__ __forceinline__ unsigned ToCode(float y, unsigned bits16) {
 }
 
 // The fp32 value of a parameter, and back.
-__device__ __forceinline__ float WithRemainder(__nv_bfloat16 p, short remainder) {
-  return __uint_as_float((static_cast<unsigned>(__bfloat16_as_ushort(p)) << 16) + static_cast<unsigned>(static_cast<int>(remainder)));
+__device__ __forceinline__ float WithRemainder(unsigned param, unsigned remainder) {  // 16 bits each
+  return __uint_as_float((param << 16) + static_cast<unsigned>(static_cast<int>(static_cast<short>(remainder))));
 }
-__device__ __forceinline__ unsigned PlusHalf(float p) {  // the parameter is the high half
+__device__ __forceinline__ unsigned PlusHalf(float p) {  // the parameter is the high half, the remainder the low half ^ 0x8000
   return (isnan(p) ? 0x7fc00000u : __float_as_uint(p)) + 0x8000u;
+}
+
+// sqrt and the quotient of an update come from the SM's approximations (2^-23 and 2 units in the last place, by the PTX
+// manual): they touch p alone, in which the update is a small term.
+__device__ __forceinline__ float Sqrt(float x) {
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float Quotient(float x, float y) {
+  float r;
+  asm("div.approx.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+
+__device__ __forceinline__ void Update(const StepArgs& a, const Factors& f, float clip, float g, float* p, float* m, float* v) {
+  g = __fmul_rn(g, clip);
+  *m = __fadd_rn(__fmul_rn(*m, a.beta1), __fmul_rn(g, a.one_minus_beta1));
+  *v = __fadd_rn(__fmul_rn(*v, a.beta2), __fmul_rn(__fmul_rn(g, a.one_minus_beta2), g));
+  *p = *p * f.keep - f.size * Quotient(*m, fmaf(Sqrt(*v), f.rsqrt2, a.eps));
+}
+
+// Scales of a block whose largest magnitude has the bits `largest`: its exponent e (see adamw.h), and the codes.
+__device__ __forceinline__ unsigned ExponentOf(unsigned largest) { return max(largest >> 23, 8u); }
+__device__ __forceinline__ unsigned char ScaleByte(unsigned e) { return static_cast<unsigned char>(e < 255 ? e - 7 : 255); }
+__device__ __forceinline__ float ScaleOf(unsigned char byte) { return __uint_as_float(static_cast<unsigned>(byte) << 23); }
+__device__ __forceinline__ unsigned Codes(float m, unsigned e, unsigned bits16) {
+  return ToCode(fabsf(m) * __uint_as_float((261 - e) << 23), bits16) | (__float_as_uint(m) >> 24 & 0x80);
+}
+__device__ __forceinline__ unsigned CodesAboveZero(float v, unsigned e, unsigned bits16) {
+  const unsigned code = ToCode(v * __uint_as_float((261 - e) << 23), bits16);
+  return code == 0 && v > 0.f ? 1 : code;
+}
+constexpr unsigned kNanCode = 0x7f;
+
+// 8 values of a lane that are neighbours in memory, as they lie there.
+template <class T> struct Packed;
+template <> struct Packed<float> {
+  unsigned w[8];
+  __device__ __forceinline__ float At(int i) const { return __uint_as_float(w[i]); }
+};
+template <> struct Packed<__nv_bfloat16> {
+  unsigned w[4];
+  __device__ __forceinline__ float At(int i) const { return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16); }
+};
+template <> struct Packed<unsigned char> {
+  unsigned w[2];
+  __device__ __forceinline__ float2 Pair(int i) const {  // values 2i and 2i + 1 of e4m3
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i / 2] >> (i & 1) * 16), __NV_E4M3);
+    return __half22float2(h);
+  }
+};
+
+template <int kWords> __device__ __forceinline__ void LoadWords(const void* from, unsigned (&w)[kWords]) {
+  if constexpr (kWords == 8) {
+    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(from));
+  } else if constexpr (kWords == 4) {
+    asm volatile("ld.global.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(from));
+  } else {
+    asm volatile("ld.global.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(from));
+  }
+}
+template <int kWords> __device__ __forceinline__ void StoreWords(void* to, const unsigned (&w)[kWords]) {
+  if constexpr (kWords == 8) {
+    asm volatile("st.global.v8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};"
+                 :: "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "l"(to) : "memory");
+  } else if constexpr (kWords == 4) {
+    asm volatile("st.global.v4.b32 [%4], {%0,%1,%2,%3};" :: "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "l"(to) : "memory");
+  } else {
+    asm volatile("st.global.v2.b32 [%2], {%0,%1};" :: "r"(w[0]), "r"(w[1]), "l"(to) : "memory");
+  }
+}
+
+// kBlock values of a tensor whose parameter and gradient lie at whole vectors: 8 neighbours per lane, a scale for 4 lanes.
+template <class T, int kBits>
+__device__ __forceinline__ void VectorBlock(const StepArgs& a, const SmlAdamwTensor& x, long long k, long long state, const Factors& f,
+                                            float clip, int lane) {
+  using M = std::conditional_t<kBits == 32, float, unsigned char>;
+  constexpr int kMoment = kBits / 8;
+  k += lane * 8;
+  state += k;
+  T* const param = static_cast<T*>(x.param) + k;
+  char* const m_at = static_cast<char*>(a.state.exp_avg) + state * kMoment;
+  char* const v_at = static_cast<char*>(a.state.exp_avg_sq) + state * kMoment;
+  Packed<T> p, g;
+  Packed<__nv_bfloat16> r;
+  Packed<M> m, v;
+  unsigned char sm = 0, sv = 0;
+  LoadWords(static_cast<const T*>(x.grad) + k, g.w);
+  LoadWords(param, p.w);
+  LoadWords(m_at, m.w);
+  LoadWords(v_at, v.w);
+  if constexpr (sizeof(T) == 2) LoadWords(a.state.remainder + state, r.w);
+  if constexpr (kBits == 8) sm = a.state.exp_avg_scale[state / kScaled], sv = a.state.exp_avg_sq_scale[state / kScaled];
+  float mf[8], vf[8];
+  unsigned largest_m = 0, largest_v = 0, even = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    if constexpr (kBits == 32) {
+      mf[i] = m.At(i), vf[i] = v.At(i);
+    } else if (i % 2 == 0) {
+      const float2 pm = m.Pair(i / 2), pv = v.Pair(i / 2);
+      const float m_scale = ScaleOf(sm), v_scale = ScaleOf(sv);
+      mf[i] = pm.x * m_scale, mf[i + 1] = pm.y * m_scale, vf[i] = pv.x * v_scale, vf[i + 1] = pv.y * v_scale;
+    }
+    float pf = p.At(i);
+    if constexpr (sizeof(T) == 2) pf = WithRemainder(p.w[i / 2] >> (i & 1) * 16 & 0xffff, r.w[i / 2] >> (i & 1) * 16);
+    Update(a, f, clip, g.At(i), &pf, &mf[i], &vf[i]);
+    if constexpr (sizeof(T) == 2) {
+      const unsigned w = PlusHalf(pf);
+      if (i & 1) {
+        p.w[i / 2] = __byte_perm(even, w, 0x7632);
+        r.w[i / 2] = __byte_perm(even, w, 0x5410) ^ 0x80008000u;
+      } else {
+        even = w;
+      }
+    } else {
+      p.w[i] = __float_as_uint(pf);
+    }
+    if constexpr (kBits == 32) {
+      m.w[i] = __float_as_uint(mf[i]), v.w[i] = __float_as_uint(vf[i]);
+    } else {
+      largest_m = max(largest_m, __float_as_uint(mf[i]) & 0x7fffffffu);
+      largest_v = max(largest_v, __float_as_uint(vf[i]) & 0x7fffffffu);
+    }
+  }
+  StoreWords(param, p.w);
+  if constexpr (sizeof(T) == 2) StoreWords(a.state.remainder + state, r.w);
+  if constexpr (kBits == 8) {
+#pragma unroll
+    for (int o = 1; o < kScaled / 8; o *= 2) {
+      largest_m = max(largest_m, __shfl_xor_sync(0xffffffffu, largest_m, o));
+      largest_v = max(largest_v, __shfl_xor_sync(0xffffffffu, largest_v, o));
+    }
+    const unsigned em = ExponentOf(largest_m), ev = ExponentOf(largest_v);
+    const unsigned first = HashedAt(a, f, state);
+    m.w[0] = m.w[1] = v.w[0] = v.w[1] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const unsigned h = Mix(first + i);
+      m.w[i / 4] |= Codes(mf[i], em, h & 0xffff) << i % 4 * 8;
+      v.w[i / 4] |= CodesAboveZero(vf[i], ev, h >> 16) << i % 4 * 8;
+    }
+    if (em == 255) m.w[0] = m.w[1] = kNanCode * 0x01010101u;
+    if (ev == 255) v.w[0] = v.w[1] = kNanCode * 0x01010101u;
+    if (lane % (kScaled / 8) == 0) {
+      a.state.exp_avg_scale[state / kScaled] = ScaleByte(em);
+      a.state.exp_avg_sq_scale[state / kScaled] = ScaleByte(ev);
+    }
+  }
+  StoreWords(m_at, m.w);
+  StoreWords(v_at, v.w);
+}
+
+// Up to kBlock values from k on at any address: the lanes take neighbouring values, 32 of which share a scale.
+template <class T, int kBits>
+__device__ __noinline__ void AnyBlock(const StepArgs& a, const SmlAdamwTensor& x, long long k, long long state, Factors f, float clip,
+                                      int lane) {
+  const unsigned first = HashedAt(a, f, state + k);
+#pragma unroll 1
+  for (int j = lane; j < kBlock; j += 32) {
+    const long long at = k + j;
+    const bool in = at < x.numel;
+    T* const param = static_cast<T*>(x.param) + at;
+    float m = 0.f, v = 0.f, g = 0.f, p = 0.f;
+    if (in) {
+      if constexpr (sizeof(T) == 2) p = WithRemainder(__bfloat16_as_ushort(*param), static_cast<unsigned short>(a.state.remainder[state + at]));
+      else p = *param;
+      g = static_cast<float>(static_cast<const T*>(x.grad)[at]);
+      if constexpr (kBits == 32) {
+        m = static_cast<const float*>(a.state.exp_avg)[state + at];
+        v = static_cast<const float*>(a.state.exp_avg_sq)[state + at];
+      } else {
+        m = FromCode(static_cast<const unsigned char*>(a.state.exp_avg)[state + at]) * ScaleOf(a.state.exp_avg_scale[(state + at) / kScaled]);
+        v = FromCode(static_cast<const unsigned char*>(a.state.exp_avg_sq)[state + at]) * ScaleOf(a.state.exp_avg_sq_scale[(state + at) / kScaled]);
+      }
+    }
+    Update(a, f, clip, g, &p, &m, &v);
+    if (in) {
+      if constexpr (sizeof(T) == 2) {
+        const unsigned w = PlusHalf(p);
+        *param = __ushort_as_bfloat16(static_cast<unsigned short>(w >> 16));
+        a.state.remainder[state + at] = static_cast<short>(w ^ 0x8000u);
+      } else {
+        *param = p;
+      }
+    } else {
+      m = v = 0.f;
+    }
+    if constexpr (kBits == 32) {
+      if (in) {
+        static_cast<float*>(a.state.exp_avg)[state + at] = m;
+        static_cast<float*>(a.state.exp_avg_sq)[state + at] = v;
+      }
+    } else {
+      const unsigned em = ExponentOf(__reduce_max_sync(0xffffffffu, __float_as_uint(m) & 0x7fffffffu));
+      const unsigned ev = ExponentOf(__reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu));
+      const unsigned h = Mix(first + j);
+      if (in) {
+        static_cast<unsigned char*>(a.state.exp_avg)[state + at] = static_cast<unsigned char>(em < 255 ? Codes(m, em, h & 0xffff) : kNanCode);
+        static_cast<unsigned char*>(a.state.exp_avg_sq)[state + at] =
+            static_cast<unsigned char>(ev < 255 ? CodesAboveZero(v, ev, h >> 16) : kNanCode);
+        if (lane == 0) {
+          a.state.exp_avg_scale[(state + at) / kScaled] = ScaleByte(em);
+          a.state.exp_avg_sq_scale[(state + at) / kScaled] = ScaleByte(ev);
+        }
+      }
+    }
+  }
 }
 
 template <class T, int kBits>
@@ -115,68 +333,12 @@ __global__ void __launch_bounds__(kThreads) AdamwKernel(const __grid_constant__ 
     const SmlAdamwTensor& x = a.tensor[i];
     const long long start = static_cast<long long>(tile - a.first_tile[i]) * a.tile_blocks * kBlock;
     const long long end = min(x.numel, start + static_cast<long long>(a.tile_blocks) * kBlock);
-    const int t = a.state.steps[x.step] + 1;
     const long long state = static_cast<long long>(x.place) * kBlock;
-    for (long long at = start; at < end; at += kBlock) {
-      const unsigned long long first = a.state.first + state + at;
-      const Factors f = FactorsOf(a, t, lr, first);
-#pragma unroll 1
-      for (int j = 0; j < kBlock / 32; j++) {
-        const long long k = at + j * 32 + lane;  // 32 values that share a scale: one per lane
-        const bool in = k < end;
-        float m = 0.f, v = 0.f, g = 0.f, p = 0.f;
-        if (in) {
-          p = static_cast<float>(static_cast<const T*>(x.param)[k]);
-          if constexpr (sizeof(T) == 2) p = WithRemainder(static_cast<const T*>(x.param)[k], a.state.remainder[state + k]);
-          g = static_cast<float>(static_cast<const T*>(x.grad)[k]);
-          if constexpr (kBits == 32) {
-            m = static_cast<const float*>(a.state.exp_avg)[state + k];
-            v = static_cast<const float*>(a.state.exp_avg_sq)[state + k];
-          } else {
-            m = FromCode(static_cast<const unsigned char*>(a.state.exp_avg)[state + k]) *
-                __uint_as_float(static_cast<unsigned>(a.state.exp_avg_scale[(state + k) / kScaled]) << 23);
-            v = FromCode(static_cast<const unsigned char*>(a.state.exp_avg_sq)[state + k]) *
-                __uint_as_float(static_cast<unsigned>(a.state.exp_avg_sq_scale[(state + k) / kScaled]) << 23);
-          }
-        }
-        g = __fmul_rn(g, clip);
-        m = __fadd_rn(__fmul_rn(m, a.beta1), __fmul_rn(g, a.one_minus_beta1));
-        v = __fadd_rn(__fmul_rn(v, a.beta2), __fmul_rn(__fmul_rn(g, a.one_minus_beta2), g));
-        p = p * f.keep - f.size * (m / (sqrtf(v) * f.rsqrt2 + a.eps));
-        if (in) {
-          if constexpr (sizeof(T) == 2) {
-            const unsigned w = PlusHalf(p);
-            static_cast<T*>(x.param)[k] = __ushort_as_bfloat16(static_cast<unsigned short>(w >> 16));
-            a.state.remainder[state + k] = static_cast<short>(w ^ 0x8000u);  // (w - 0x8000) of its low half
-          } else {
-            static_cast<T*>(x.param)[k] = p;
-          }
-        }
-        if constexpr (kBits == 32) {
-          if (in) {
-            static_cast<float*>(a.state.exp_avg)[state + k] = m;
-            static_cast<float*>(a.state.exp_avg_sq)[state + k] = v;
-          }
-        } else {
-          const unsigned em = max(__reduce_max_sync(0xffffffffu, __float_as_uint(m) & 0x7fffffffu) >> 23, 8u);
-          const unsigned ev = max(__reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu) >> 23, 8u);
-          const unsigned h = Mix(static_cast<unsigned>(first) + j * 32 + lane + f.key);
-          unsigned cm = 0x7f, cv = 0x7f;  // NaN
-          if (em < 255) cm = ToCode(fabsf(m) * __uint_as_float((261 - em) << 23), h & 0xffff) | (__float_as_uint(m) >> 24 & 0x80);
-          if (ev < 255) {
-            cv = ToCode(v * __uint_as_float((261 - ev) << 23), h >> 16);
-            if (cv == 0 && v > 0.f) cv = 1;
-          }
-          if (in) {
-            static_cast<unsigned char*>(a.state.exp_avg)[state + k] = static_cast<unsigned char>(cm);
-            static_cast<unsigned char*>(a.state.exp_avg_sq)[state + k] = static_cast<unsigned char>(cv);
-            if (lane == 0) {
-              a.state.exp_avg_scale[(state + k) / kScaled] = static_cast<unsigned char>(em < 255 ? em - 7 : 255);
-              a.state.exp_avg_sq_scale[(state + k) / kScaled] = static_cast<unsigned char>(ev < 255 ? ev - 7 : 255);
-            }
-          }
-        }
-      }
+    const Factors f = FactorsOf(a, a.state.steps[x.step] + 1, lr);
+    const bool vectors = ((reinterpret_cast<uintptr_t>(x.param) | reinterpret_cast<uintptr_t>(x.grad)) & (8 * sizeof(T) - 1)) == 0;
+    for (long long k = start; k < end; k += kBlock) {
+      if (vectors && k + kBlock <= end) VectorBlock<T, kBits>(a, x, k, state, f, clip, lane);
+      else AnyBlock<T, kBits>(a, x, k, state, f, clip, lane);
     }
   }
   // The block that ends last counts the step: every block has read the counts by then.
@@ -214,7 +376,7 @@ __global__ void __launch_bounds__(kThreads) MastersKernel(const __grid_constant_
     const long long k = start + j * 32 + (threadIdx.x & 31);
     if (k >= x.numel) break;
     const T p = static_cast<const T*>(x.param)[k];
-    if constexpr (sizeof(T) == 2) a.out[state + k] = WithRemainder(p, a.remainder[state + k]);
+    if constexpr (sizeof(T) == 2) a.out[state + k] = WithRemainder(__bfloat16_as_ushort(p), static_cast<unsigned short>(a.remainder[state + k]));
     else a.out[state + k] = p;
   }
 }
@@ -241,6 +403,33 @@ __device__ __forceinline__ double BlockSum(double v) {
   return sum;
 }
 
+// Over this thread's share of the values from start to end, at most kNormTile.
+template <class T>
+__device__ __forceinline__ double SquaresOf(const T* x, long long start, long long end) {
+  double sum = 0.0;
+  if (end - start == kNormTile && (reinterpret_cast<uintptr_t>(x) & (8 * sizeof(T) - 1)) == 0) {
+    constexpr int kVectors = kNormTile / (kThreads * 8);
+    Packed<T> v[kVectors];
+#pragma unroll
+    for (int u = 0; u < kVectors; u++) LoadWords(x + start + (u * kThreads + threadIdx.x) * 8, v[u].w);
+#pragma unroll
+    for (int u = 0; u < kVectors; u++) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const double g = v[u].At(i);
+        sum += g * g;
+      }
+    }
+  } else {
+#pragma unroll 4
+    for (long long k = start + threadIdx.x; k < end; k += kThreads) {
+      const double g = static_cast<float>(x[k]);
+      sum += g * g;
+    }
+  }
+  return sum;
+}
+
 // Squares are summed in fp64: 2^-53 of a sum over 10^9 values still leaves the result right to its last fp32 bit, and no
 // gradient's square overflows or vanishes.
 __global__ void __launch_bounds__(kThreads) NormKernel(const __grid_constant__ NormArgs a) {
@@ -251,17 +440,8 @@ __global__ void __launch_bounds__(kThreads) NormKernel(const __grid_constant__ N
     const SmlNormTensor& x = a.tensor[i];
     const long long start = static_cast<long long>(tile - a.first_tile[i]) * kNormTile;
     const long long end = min(x.numel, start + kNormTile);
-    if (x.type == SML_ADAMW_F32) {
-      for (long long k = start + threadIdx.x; k < end; k += kThreads) {
-        const double g = static_cast<const float*>(x.data)[k];
-        sum += g * g;
-      }
-    } else {
-      for (long long k = start + threadIdx.x; k < end; k += kThreads) {
-        const double g = __bfloat162float(static_cast<const __nv_bfloat16*>(x.data)[k]);
-        sum += g * g;
-      }
-    }
+    sum += x.type == SML_ADAMW_F32 ? SquaresOf(static_cast<const float*>(x.data), start, end)
+                                   : SquaresOf(static_cast<const __nv_bfloat16*>(x.data), start, end);
   }
   sum = BlockSum(sum);
   if (threadIdx.x == 0) a.partial[blockIdx.x] = sum;
