@@ -91,13 +91,6 @@ __device__ __forceinline__ unsigned HashedAt(const StepArgs& a, const Factors& f
   return static_cast<unsigned>(value) + Mix(f.key + static_cast<unsigned>(value >> 32));
 }
 
-// The code (without sign) of a magnitude over its scale.
-__device__ __forceinline__ unsigned ToCode(float y, unsigned bits16) {
-  const bool small = y < 0.015625f;
-  const float t = small ? __fadd_rn(y, 0.015625f) : y;
-  return ((__float_as_uint(t) + (bits16 << 4 | 8)) >> 20) - (small ? 968 : 960);
-}
-
 // The fp32 value of a parameter, and back.
 __device__ __forceinline__ float WithRemainder(unsigned param, unsigned remainder) {  // 16 bits each
   return __uint_as_float((param << 16) + static_cast<unsigned>(static_cast<int>(static_cast<short>(remainder))));
@@ -106,16 +99,23 @@ __device__ __forceinline__ unsigned PlusHalf(float p) {  // the parameter is the
   return (isnan(p) ? 0x7fc00000u : __float_as_uint(p)) + 0x8000u;
 }
 
-// sqrt and the quotient of an update come from the SM's approximations (2^-23 and 2 units in the last place, by the PTX
-// manual): they touch p alone, in which the update is a small term.
-__device__ __forceinline__ float Sqrt(float x) {
+// The root and the reciprocal of an update come from the SM's approximations (2^-23 and 2^-23 of the result, by the PTX
+// manual; correctly rounded ones are sequences of a dozen instructions): they touch p alone, in which the update is a
+// small term. Both flush subnormal numbers, so second moments below 2^-126 count as 2^-126.
+__device__ __forceinline__ float Root(float x) {
   float r;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-__device__ __forceinline__ float Quotient(float x, float y) {
+__device__ __forceinline__ float Reciprocal(float x) {
   float r;
-  asm("div.approx.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// The largest of three; NaN where one of them is.
+__device__ __forceinline__ float Largest(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -123,19 +123,28 @@ __device__ __forceinline__ void Update(const StepArgs& a, const Factors& f, floa
   g = __fmul_rn(g, clip);
   *m = __fadd_rn(__fmul_rn(*m, a.beta1), __fmul_rn(g, a.one_minus_beta1));
   *v = __fadd_rn(__fmul_rn(*v, a.beta2), __fmul_rn(__fmul_rn(g, a.one_minus_beta2), g));
-  *p = *p * f.keep - f.size * Quotient(*m, fmaf(Sqrt(*v), f.rsqrt2, a.eps));
+  const float root = isnan(*v) ? *v : Root(fmaxf(*v, 1.17549435e-38f));
+  *p = fmaf(*p, f.keep, -f.size * (*m * Reciprocal(fmaf(root, f.rsqrt2, a.eps))));
 }
 
-// Scales of a block whose largest magnitude has the bits `largest`: its exponent e (see adamw.h), and the codes.
-__device__ __forceinline__ unsigned ExponentOf(unsigned largest) { return max(largest >> 23, 8u); }
+// Scales of a block whose largest magnitude is `largest`: its exponent e (see adamw.h), the byte and the number.
+__device__ __forceinline__ unsigned ExponentOf(float largest) { return max(__float_as_uint(largest) >> 23, 8u); }
 __device__ __forceinline__ unsigned char ScaleByte(unsigned e) { return static_cast<unsigned char>(e < 255 ? e - 7 : 255); }
 __device__ __forceinline__ float ScaleOf(unsigned char byte) { return __uint_as_float(static_cast<unsigned>(byte) << 23); }
-__device__ __forceinline__ unsigned Codes(float m, unsigned e, unsigned bits16) {
-  return ToCode(fabsf(m) * __uint_as_float((261 - e) << 23), bits16) | (__float_as_uint(m) >> 24 & 0x80);
+
+// A magnitude, rounded to its code: in the top 8 bits of the result. A number over its scale times 2^-120 has the bits of
+// its e4m3 form in front of 20 more, subnormal numbers too, since both formats then begin at the same exponent; the
+// product rounds as the addition of 2^-6 in adamw.h does. `random` is what those 20 bits get added, 4 places up.
+__device__ __forceinline__ unsigned ToCode(float x, unsigned e, unsigned random) {
+  const float y = __fmul_rn(__fmul_rn(fabsf(x), __uint_as_float((261 - e) << 23)), 7.52316385e-37f);
+  return (__float_as_uint(y) << 4) + random;
 }
-__device__ __forceinline__ unsigned CodesAboveZero(float v, unsigned e, unsigned bits16) {
-  const unsigned code = ToCode(v * __uint_as_float((261 - e) << 23), bits16);
-  return code == 0 && v > 0.f ? 1 : code;
+__device__ __forceinline__ unsigned MCode(float m, unsigned e, unsigned hash) {
+  return ToCode(m, e, __byte_perm(hash, 0x80, 0x5104)) | (__float_as_uint(m) & 0x80000000u);
+}
+__device__ __forceinline__ unsigned VCode(float v, unsigned e, unsigned hash) {
+  const unsigned code = ToCode(v, e, __byte_perm(hash, 0x80, 0x5324));
+  return v > 0.f ? max(code, 1u << 24) : code;
 }
 constexpr unsigned kNanCode = 0x7f;
 
@@ -200,7 +209,7 @@ __device__ __forceinline__ void VectorBlock(const StepArgs& a, const SmlAdamwTen
   if constexpr (sizeof(T) == 2) LoadWords(a.state.remainder + state, r.w);
   if constexpr (kBits == 8) sm = a.state.exp_avg_scale[state / kScaled], sv = a.state.exp_avg_sq_scale[state / kScaled];
   float mf[8], vf[8];
-  unsigned largest_m = 0, largest_v = 0, even = 0;
+  unsigned even = 0;
 #pragma unroll
   for (int i = 0; i < 8; i++) {
     if constexpr (kBits == 32) {
@@ -224,29 +233,35 @@ __device__ __forceinline__ void VectorBlock(const StepArgs& a, const SmlAdamwTen
     } else {
       p.w[i] = __float_as_uint(pf);
     }
-    if constexpr (kBits == 32) {
-      m.w[i] = __float_as_uint(mf[i]), v.w[i] = __float_as_uint(vf[i]);
-    } else {
-      largest_m = max(largest_m, __float_as_uint(mf[i]) & 0x7fffffffu);
-      largest_v = max(largest_v, __float_as_uint(vf[i]) & 0x7fffffffu);
-    }
+    if constexpr (kBits == 32) m.w[i] = __float_as_uint(mf[i]), v.w[i] = __float_as_uint(vf[i]);
   }
   StoreWords(param, p.w);
   if constexpr (sizeof(T) == 2) StoreWords(a.state.remainder + state, r.w);
   if constexpr (kBits == 8) {
+    float largest_m = 0.f, largest_v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      largest_m = Largest(largest_m, fabsf(mf[i]), fabsf(mf[i + 1]));
+      largest_v = Largest(largest_v, vf[i], vf[i + 1]);
+    }
 #pragma unroll
     for (int o = 1; o < kScaled / 8; o *= 2) {
-      largest_m = max(largest_m, __shfl_xor_sync(0xffffffffu, largest_m, o));
-      largest_v = max(largest_v, __shfl_xor_sync(0xffffffffu, largest_v, o));
+      largest_m = Largest(largest_m, __shfl_xor_sync(0xffffffffu, largest_m, o), 0.f);
+      largest_v = Largest(largest_v, __shfl_xor_sync(0xffffffffu, largest_v, o), 0.f);
     }
     const unsigned em = ExponentOf(largest_m), ev = ExponentOf(largest_v);
     const unsigned first = HashedAt(a, f, state);
-    m.w[0] = m.w[1] = v.w[0] = v.w[1] = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const unsigned h = Mix(first + i);
-      m.w[i / 4] |= Codes(mf[i], em, h & 0xffff) << i % 4 * 8;
-      v.w[i / 4] |= CodesAboveZero(vf[i], ev, h >> 16) << i % 4 * 8;
+    for (int i = 0; i < 8; i += 4) {
+      unsigned cm[4], cv[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const unsigned h = Mix(first + i + j);
+        cm[j] = MCode(mf[i + j], em, h);
+        cv[j] = VCode(vf[i + j], ev, h);
+      }
+      m.w[i / 4] = __byte_perm(__byte_perm(cm[0], cm[1], 0x73), __byte_perm(cm[2], cm[3], 0x73), 0x5410);
+      v.w[i / 4] = __byte_perm(__byte_perm(cv[0], cv[1], 0x73), __byte_perm(cv[2], cv[3], 0x73), 0x5410);
     }
     if (em == 255) m.w[0] = m.w[1] = kNanCode * 0x01010101u;
     if (ev == 255) v.w[0] = v.w[1] = kNanCode * 0x01010101u;
@@ -300,13 +315,12 @@ __device__ __noinline__ void AnyBlock(const StepArgs& a, const SmlAdamwTensor& x
         static_cast<float*>(a.state.exp_avg_sq)[state + at] = v;
       }
     } else {
-      const unsigned em = ExponentOf(__reduce_max_sync(0xffffffffu, __float_as_uint(m) & 0x7fffffffu));
-      const unsigned ev = ExponentOf(__reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu));
+      const unsigned em = ExponentOf(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(m)))));
+      const unsigned ev = ExponentOf(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(v)))));
       const unsigned h = Mix(first + j);
       if (in) {
-        static_cast<unsigned char*>(a.state.exp_avg)[state + at] = static_cast<unsigned char>(em < 255 ? Codes(m, em, h & 0xffff) : kNanCode);
-        static_cast<unsigned char*>(a.state.exp_avg_sq)[state + at] =
-            static_cast<unsigned char>(ev < 255 ? CodesAboveZero(v, ev, h >> 16) : kNanCode);
+        static_cast<unsigned char*>(a.state.exp_avg)[state + at] = static_cast<unsigned char>(em < 255 ? MCode(m, em, h) >> 24 : kNanCode);
+        static_cast<unsigned char*>(a.state.exp_avg_sq)[state + at] = static_cast<unsigned char>(ev < 255 ? VCode(v, ev, h) >> 24 : kNanCode);
         if (lane == 0) {
           a.state.exp_avg_scale[(state + at) / kScaled] = ScaleByte(em);
           a.state.exp_avg_sq_scale[(state + at) / kScaled] = ScaleByte(ev);
