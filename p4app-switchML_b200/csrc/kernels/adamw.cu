@@ -15,6 +15,7 @@
 #include "kernels/dependent_launch.cuh"
 
 using switchml::kernels::LaunchOverlapped;
+using switchml::kernels::LetNextKernelStart;
 using switchml::kernels::WaitForEarlierKernels;
 
 namespace {
@@ -26,7 +27,7 @@ int Launched(cudaError_t e) {
   return -4;
 }
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr int kBlock = SML_ADAMW_ALIGN;  // values that a warp takes at once: 8 per lane
 constexpr int kScaled = 32;              // values that share a scale
 constexpr long long kMaxNumel = 1ll << 38;  // of a tensor: the number of its tiles fits 31 bits
@@ -38,7 +39,7 @@ struct StepArgs {
   int count;
   int tile_blocks;  // kBlock's of a tile
   SmlAdamwState state;
-  float lr, beta1, one_minus_beta1, beta2, one_minus_beta2, eps, decay, log_beta1, log_beta2, max_norm;
+  float lr, beta1, one_minus_beta1, beta2, one_minus_beta2, eps, decay, log_beta1, log_beta2, max_norm, minus_zero;
   const float *lr_tensor, *norm;
 };
 
@@ -112,19 +113,58 @@ __device__ __forceinline__ float Reciprocal(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// The largest of three; NaN where one of them is.
+// Two fp32 operations in one instruction: the 8-bit kernel's pace is that of issuing instructions.
+struct Pair {
+  unsigned long long w;
+  __device__ __forceinline__ Pair() {}
+  __device__ __forceinline__ Pair(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(w) : "f"(x), "f"(y)); }
+  __device__ __forceinline__ explicit Pair(float x) : Pair(x, x) {}
+  __device__ __forceinline__ float2 Both() const {
+    float2 v;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(w));
+    return v;
+  }
+};
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.w) : "l"(a.w), "l"(b.w));
+  return r;
+}
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.w) : "l"(a.w), "l"(b.w));
+  return r;
+}
+__device__ __forceinline__ Pair Fma(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.w) : "l"(a.w), "l"(b.w), "l"(c.w));
+  return r;
+}
+
+// The larger of two, the largest of three; NaN where one of them is.
+__device__ __forceinline__ float Larger(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ float Largest(float a, float b, float c) {
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
-__device__ __forceinline__ void Update(const StepArgs& a, const Factors& f, float clip, float g, float* p, float* m, float* v) {
-  g = __fmul_rn(g, clip);
-  *m = __fadd_rn(__fmul_rn(*m, a.beta1), __fmul_rn(g, a.one_minus_beta1));
-  *v = __fadd_rn(__fmul_rn(*v, a.beta2), __fmul_rn(__fmul_rn(g, a.one_minus_beta2), g));
-  const float root = isnan(*v) ? *v : Root(fmaxf(*v, 1.17549435e-38f));
-  *p = fmaf(*p, f.keep, -f.size * (*m * Reciprocal(fmaf(root, f.rsqrt2, a.eps))));
+// One step of two values.
+__device__ __forceinline__ void Update(const StepArgs& a, const Factors& f, float clip, Pair g, Pair* p, Pair* m, Pair* v) {
+  g = g * Pair(clip);
+  // Products that are rounded before they are added: ptxas makes one operation with one rounding of mul.rn.f32x2 and
+  // add.rn.f32x2, but not of this, as long as it does not know that what is added is -0.
+  const Pair none(a.minus_zero);
+  *m = Fma(*m, Pair(a.beta1), none) + Fma(g, Pair(a.one_minus_beta1), none);
+  *v = Fma(*v, Pair(a.beta2), none) + Fma(g * Pair(a.one_minus_beta2), g, none);
+  const float2 square = v->Both();
+  const Pair root(Root(Larger(square.x, 1.17549435e-38f)), Root(Larger(square.y, 1.17549435e-38f)));
+  const float2 below = Fma(root, Pair(f.rsqrt2), Pair(a.eps)).Both();
+  *p = Fma(*p, Pair(f.keep), *m * Pair(Reciprocal(below.x), Reciprocal(below.y)) * Pair(-f.size));
 }
 
 // Scales of a block whose largest magnitude is `largest`: its exponent e (see adamw.h), the byte and the number.
@@ -132,18 +172,18 @@ __device__ __forceinline__ unsigned ExponentOf(float largest) { return max(__flo
 __device__ __forceinline__ unsigned char ScaleByte(unsigned e) { return static_cast<unsigned char>(e < 255 ? e - 7 : 255); }
 __device__ __forceinline__ float ScaleOf(unsigned char byte) { return __uint_as_float(static_cast<unsigned>(byte) << 23); }
 
-// A magnitude, rounded to its code: in the top 8 bits of the result. A number over its scale times 2^-120 has the bits of
-// its e4m3 form in front of 20 more, subnormal numbers too, since both formats then begin at the same exponent; the
-// product rounds as the addition of 2^-6 in adamw.h does. `random` is what those 20 bits get added, 4 places up.
-__device__ __forceinline__ unsigned ToCode(float x, unsigned e, unsigned random) {
-  const float y = __fmul_rn(__fmul_rn(fabsf(x), __uint_as_float((261 - e) << 23)), 7.52316385e-37f);
-  return (__float_as_uint(y) << 4) + random;
+// Values, rounded to their codes without the sign: in the top 8 bits of the results. A number over its scale times 2^-120
+// has the bits of its e4m3 form in front of 20 more, subnormal numbers too, since both formats then begin at the same
+// exponent; the product rounds as the addition of 2^-6 in adamw.h does. `random` is what those 20 bits get added, 4 places up.
+__device__ __forceinline__ Pair OverScale(Pair x, unsigned e) {
+  return x * Pair(__uint_as_float((261 - e) << 23)) * Pair(7.52316385e-37f);
 }
-__device__ __forceinline__ unsigned MCode(float m, unsigned e, unsigned hash) {
-  return ToCode(m, e, __byte_perm(hash, 0x80, 0x5104)) | (__float_as_uint(m) & 0x80000000u);
+__device__ __forceinline__ unsigned ToCode(float y, unsigned random) { return (__float_as_uint(y) << 4) + random; }
+__device__ __forceinline__ unsigned MCode(float y, unsigned hash) {
+  return ToCode(y, __byte_perm(hash, 0x80, 0x5104)) | (__float_as_uint(y) & 0x80000000u);
 }
-__device__ __forceinline__ unsigned VCode(float v, unsigned e, unsigned hash) {
-  const unsigned code = ToCode(v, e, __byte_perm(hash, 0x80, 0x5324));
+__device__ __forceinline__ unsigned VCode(float y, float v, unsigned hash) {
+  const unsigned code = ToCode(y, __byte_perm(hash, 0x80, 0x5324));
   return v > 0.f ? max(code, 1u << 24) : code;
 }
 constexpr unsigned kNanCode = 0x7f;
@@ -160,9 +200,10 @@ template <> struct Packed<__nv_bfloat16> {
 };
 template <> struct Packed<unsigned char> {
   unsigned w[2];
-  __device__ __forceinline__ float2 Pair(int i) const {  // values 2i and 2i + 1 of e4m3
+  __device__ __forceinline__ Pair Decoded(int i) const {  // values 2i and 2i + 1 of e4m3
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i / 2] >> (i & 1) * 16), __NV_E4M3);
-    return __half22float2(h);
+    const float2 v = __half22float2(h);
+    return Pair(v.x, v.y);
   }
 };
 
@@ -208,60 +249,61 @@ __device__ __forceinline__ void VectorBlock(const StepArgs& a, const SmlAdamwTen
   LoadWords(v_at, v.w);
   if constexpr (sizeof(T) == 2) LoadWords(a.state.remainder + state, r.w);
   if constexpr (kBits == 8) sm = a.state.exp_avg_scale[state / kScaled], sv = a.state.exp_avg_sq_scale[state / kScaled];
-  float mf[8], vf[8];
-  unsigned even = 0;
+  Pair mf[4], vf[4];
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
+  for (int i = 0; i < 4; i++) {
     if constexpr (kBits == 32) {
-      mf[i] = m.At(i), vf[i] = v.At(i);
-    } else if (i % 2 == 0) {
-      const float2 pm = m.Pair(i / 2), pv = v.Pair(i / 2);
-      const float m_scale = ScaleOf(sm), v_scale = ScaleOf(sv);
-      mf[i] = pm.x * m_scale, mf[i + 1] = pm.y * m_scale, vf[i] = pv.x * v_scale, vf[i + 1] = pv.y * v_scale;
-    }
-    float pf = p.At(i);
-    if constexpr (sizeof(T) == 2) pf = WithRemainder(p.w[i / 2] >> (i & 1) * 16 & 0xffff, r.w[i / 2] >> (i & 1) * 16);
-    Update(a, f, clip, g.At(i), &pf, &mf[i], &vf[i]);
-    if constexpr (sizeof(T) == 2) {
-      const unsigned w = PlusHalf(pf);
-      if (i & 1) {
-        p.w[i / 2] = __byte_perm(even, w, 0x7632);
-        r.w[i / 2] = __byte_perm(even, w, 0x5410) ^ 0x80008000u;
-      } else {
-        even = w;
-      }
+      mf[i] = Pair(m.At(2 * i), m.At(2 * i + 1)), vf[i] = Pair(v.At(2 * i), v.At(2 * i + 1));
     } else {
-      p.w[i] = __float_as_uint(pf);
+      mf[i] = m.Decoded(i) * Pair(ScaleOf(sm)), vf[i] = v.Decoded(i) * Pair(ScaleOf(sv));
     }
-    if constexpr (kBits == 32) m.w[i] = __float_as_uint(mf[i]), v.w[i] = __float_as_uint(vf[i]);
+    Pair pf(p.At(2 * i), p.At(2 * i + 1));
+    if constexpr (sizeof(T) == 2)
+      pf = Pair(WithRemainder(p.w[i] & 0xffff, r.w[i]), WithRemainder(p.w[i] >> 16, r.w[i] >> 16));
+    Update(a, f, clip, Pair(g.At(2 * i), g.At(2 * i + 1)), &pf, &mf[i], &vf[i]);
+    const float2 both = pf.Both();
+    if constexpr (sizeof(T) == 2) {
+      const unsigned x = PlusHalf(both.x), y = PlusHalf(both.y);
+      p.w[i] = __byte_perm(x, y, 0x7632);
+      r.w[i] = __byte_perm(x, y, 0x5410) ^ 0x80008000u;
+    } else {
+      p.w[2 * i] = __float_as_uint(both.x), p.w[2 * i + 1] = __float_as_uint(both.y);
+    }
+    if constexpr (kBits == 32) {
+      const float2 mb = mf[i].Both(), vb = vf[i].Both();
+      m.w[2 * i] = __float_as_uint(mb.x), m.w[2 * i + 1] = __float_as_uint(mb.y);
+      v.w[2 * i] = __float_as_uint(vb.x), v.w[2 * i + 1] = __float_as_uint(vb.y);
+    }
   }
   StoreWords(param, p.w);
   if constexpr (sizeof(T) == 2) StoreWords(a.state.remainder + state, r.w);
   if constexpr (kBits == 8) {
     float largest_m = 0.f, largest_v = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      largest_m = Largest(largest_m, fabsf(mf[i]), fabsf(mf[i + 1]));
-      largest_v = Largest(largest_v, vf[i], vf[i + 1]);
+    for (int i = 0; i < 4; i++) {
+      const float2 mb = mf[i].Both(), vb = vf[i].Both();
+      largest_m = Largest(largest_m, fabsf(mb.x), fabsf(mb.y));
+      largest_v = Largest(largest_v, vb.x, vb.y);
     }
 #pragma unroll
     for (int o = 1; o < kScaled / 8; o *= 2) {
-      largest_m = Largest(largest_m, __shfl_xor_sync(0xffffffffu, largest_m, o), 0.f);
-      largest_v = Largest(largest_v, __shfl_xor_sync(0xffffffffu, largest_v, o), 0.f);
+      largest_m = Larger(largest_m, __shfl_xor_sync(0xffffffffu, largest_m, o));
+      largest_v = Larger(largest_v, __shfl_xor_sync(0xffffffffu, largest_v, o));
     }
     const unsigned em = ExponentOf(largest_m), ev = ExponentOf(largest_v);
     const unsigned first = HashedAt(a, f, state);
 #pragma unroll
-    for (int i = 0; i < 8; i += 4) {
+    for (int i = 0; i < 4; i += 2) {
       unsigned cm[4], cv[4];
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const unsigned h = Mix(first + i + j);
-        cm[j] = MCode(mf[i + j], em, h);
-        cv[j] = VCode(vf[i + j], ev, h);
+      for (int j = 0; j < 4; j += 2) {
+        const float2 vb = vf[i + j / 2].Both(), ym = OverScale(mf[i + j / 2], em).Both(), yv = OverScale(vf[i + j / 2], ev).Both();
+        const unsigned hx = Mix(first + i * 2 + j), hy = Mix(first + i * 2 + j + 1);
+        cm[j] = MCode(ym.x, hx), cm[j + 1] = MCode(ym.y, hy);
+        cv[j] = VCode(yv.x, vb.x, hx), cv[j + 1] = VCode(yv.y, vb.y, hy);
       }
-      m.w[i / 4] = __byte_perm(__byte_perm(cm[0], cm[1], 0x73), __byte_perm(cm[2], cm[3], 0x73), 0x5410);
-      v.w[i / 4] = __byte_perm(__byte_perm(cv[0], cv[1], 0x73), __byte_perm(cv[2], cv[3], 0x73), 0x5410);
+      m.w[i / 2] = __byte_perm(__byte_perm(cm[0], cm[1], 0x73), __byte_perm(cm[2], cm[3], 0x73), 0x5410);
+      v.w[i / 2] = __byte_perm(__byte_perm(cv[0], cv[1], 0x73), __byte_perm(cv[2], cv[3], 0x73), 0x5410);
     }
     if (em == 255) m.w[0] = m.w[1] = kNanCode * 0x01010101u;
     if (ev == 255) v.w[0] = v.w[1] = kNanCode * 0x01010101u;
@@ -297,7 +339,9 @@ __device__ __noinline__ void AnyBlock(const StepArgs& a, const SmlAdamwTensor& x
         v = FromCode(static_cast<const unsigned char*>(a.state.exp_avg_sq)[state + at]) * ScaleOf(a.state.exp_avg_sq_scale[(state + at) / kScaled]);
       }
     }
-    Update(a, f, clip, g, &p, &m, &v);
+    Pair p2(p), m2(m), v2(v);
+    Update(a, f, clip, Pair(g), &p2, &m2, &v2);
+    p = p2.Both().x, m = m2.Both().x, v = v2.Both().x;
     if (in) {
       if constexpr (sizeof(T) == 2) {
         const unsigned w = PlusHalf(p);
@@ -319,8 +363,8 @@ __device__ __noinline__ void AnyBlock(const StepArgs& a, const SmlAdamwTensor& x
       const unsigned ev = ExponentOf(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(v)))));
       const unsigned h = Mix(first + j);
       if (in) {
-        static_cast<unsigned char*>(a.state.exp_avg)[state + at] = static_cast<unsigned char>(em < 255 ? MCode(m, em, h) >> 24 : kNanCode);
-        static_cast<unsigned char*>(a.state.exp_avg_sq)[state + at] = static_cast<unsigned char>(ev < 255 ? VCode(v, ev, h) >> 24 : kNanCode);
+        static_cast<unsigned char*>(a.state.exp_avg)[state + at] = static_cast<unsigned char>(em < 255 ? MCode(OverScale(Pair(m), em).Both().x, h) >> 24 : kNanCode);
+        static_cast<unsigned char*>(a.state.exp_avg_sq)[state + at] = static_cast<unsigned char>(ev < 255 ? VCode(OverScale(Pair(v), ev).Both().x, v, h) >> 24 : kNanCode);
         if (lane == 0) {
           a.state.exp_avg_scale[(state + at) / kScaled] = ScaleByte(em);
           a.state.exp_avg_sq_scale[(state + at) / kScaled] = ScaleByte(ev);
@@ -331,7 +375,7 @@ __device__ __noinline__ void AnyBlock(const StepArgs& a, const SmlAdamwTensor& x
 }
 
 template <class T, int kBits>
-__global__ void __launch_bounds__(kThreads) AdamwKernel(const __grid_constant__ StepArgs a) {
+__global__ void __launch_bounds__(kThreads, kBits == 8 ? 6 : 8) AdamwKernel(const __grid_constant__ StepArgs a) {
   WaitForEarlierKernels();
   const int lane = threadIdx.x & 31;
   float clip = 1.f;
@@ -395,7 +439,8 @@ __global__ void __launch_bounds__(kThreads) MastersKernel(const __grid_constant_
   }
 }
 
-constexpr int kNormBlocks = 148 * 4;  // partial sums of a launch, at most
+constexpr int kNormThreads = 256;
+constexpr int kNormBlocks = 148 * 8;  // partial sums of a launch, at most: the blocks that the GPU holds
 constexpr int kNormTile = 4096;       // values that a block takes at once
 
 struct NormArgs {
@@ -406,14 +451,14 @@ struct NormArgs {
 };
 
 __device__ __forceinline__ double BlockSum(double v) {
-  __shared__ double part[kWarps];
+  __shared__ double part[kNormThreads / 32];
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
   __syncthreads();
   double sum = 0.0;
 #pragma unroll
-  for (int w = 0; w < kWarps; w++) sum += part[w];
+  for (int w = 0; w < kNormThreads / 32; w++) sum += part[w];
   return sum;
 }
 
@@ -422,10 +467,10 @@ template <class T>
 __device__ __forceinline__ double SquaresOf(const T* x, long long start, long long end) {
   double sum = 0.0;
   if (end - start == kNormTile && (reinterpret_cast<uintptr_t>(x) & (8 * sizeof(T) - 1)) == 0) {
-    constexpr int kVectors = kNormTile / (kThreads * 8);
+    constexpr int kVectors = kNormTile / (kNormThreads * 8);
     Packed<T> v[kVectors];
 #pragma unroll
-    for (int u = 0; u < kVectors; u++) LoadWords(x + start + (u * kThreads + threadIdx.x) * 8, v[u].w);
+    for (int u = 0; u < kVectors; u++) LoadWords(x + start + (u * kNormThreads + threadIdx.x) * 8, v[u].w);
 #pragma unroll
     for (int u = 0; u < kVectors; u++) {
 #pragma unroll
@@ -436,7 +481,7 @@ __device__ __forceinline__ double SquaresOf(const T* x, long long start, long lo
     }
   } else {
 #pragma unroll 4
-    for (long long k = start + threadIdx.x; k < end; k += kThreads) {
+    for (long long k = start + threadIdx.x; k < end; k += kNormThreads) {
       const double g = static_cast<float>(x[k]);
       sum += g * g;
     }
@@ -446,8 +491,9 @@ __device__ __forceinline__ double SquaresOf(const T* x, long long start, long lo
 
 // Squares are summed in fp64: 2^-53 of a sum over 10^9 values still leaves the result right to its last fp32 bit, and no
 // gradient's square overflows or vanishes.
-__global__ void __launch_bounds__(kThreads) NormKernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(kNormThreads, 8) NormKernel(const __grid_constant__ NormArgs a) {
   WaitForEarlierKernels();
+  LetNextKernelStart();
   double sum = 0.0;
   for (unsigned tile = blockIdx.x; tile < a.first_tile[a.count]; tile += gridDim.x) {
     const int i = TensorOfTile(a.first_tile, a.count, tile);
@@ -461,10 +507,11 @@ __global__ void __launch_bounds__(kThreads) NormKernel(const __grid_constant__ N
   if (threadIdx.x == 0) a.partial[blockIdx.x] = sum;
 }
 
-__global__ void __launch_bounds__(kThreads) FinishNormKernel(const double* partial, int parts, float* out) {
+__global__ void __launch_bounds__(kNormThreads) FinishNormKernel(const double* partial, int parts, float* out) {
   WaitForEarlierKernels();
   double sum = 0.0;
-  for (int i = threadIdx.x; i < parts; i += kThreads) sum += partial[i];
+#pragma unroll 8
+  for (int i = threadIdx.x; i < parts; i += kNormThreads) sum += partial[i];
   sum = BlockSum(sum);
   if (threadIdx.x == 0) *out = static_cast<float>(sqrt(sum));
 }
@@ -485,6 +532,18 @@ unsigned TakeTensors(const Tensor* tensors, int count, long long tile, int* at, 
   return static_cast<unsigned>(tiles);
 }
 
+// A warp's tile, in kBlock's. What a tile costs by itself (finding its tensor, the factors, a place among the resident
+// warps) is shared by its blocks: 2^28 fp32 parameters with moments in 8 bits took 943, 771, 693 and 726 us with tiles
+// of 4, 8, 16 and 32 blocks, with fp32 moments 1104, 1120, 1125 and 1131 us (there the memory is the limit, which likes short ones).
+// Few values make smaller tiles, so that every warp that the GPU holds gets one.
+int TileBlocks(const SmlAdamwTensor* tensors, int count, int bits) {
+  long long blocks = 0;
+  for (int i = 0; i < count; i++) blocks += (tensors[i].numel + kBlock - 1) / kBlock;
+  int tile = bits == 8 ? 16 : 4;
+  while (tile > 1 && blocks < static_cast<long long>(tile) * 148 * 32) tile /= 2;
+  return tile;
+}
+
 }  // namespace
 
 extern "C" int switchml_adamw_step(const SmlAdamwTensor* tensors, int count, const SmlAdamwState* state, const SmlAdamwStep* step,
@@ -502,8 +561,9 @@ extern "C" int switchml_adamw_step(const SmlAdamwTensor* tensors, int count, con
   a.beta2 = static_cast<float>(step->beta2), a.one_minus_beta2 = static_cast<float>(1.0 - step->beta2);
   a.log_beta1 = static_cast<float>(log(step->beta1)), a.log_beta2 = static_cast<float>(log(step->beta2));
   a.eps = static_cast<float>(step->eps), a.decay = static_cast<float>(step->decay);
+  a.minus_zero = -0.f;
   a.max_norm = step->max_norm, a.lr_tensor = step->lr_tensor, a.norm = step->norm;
-  a.tile_blocks = 4;
+  a.tile_blocks = TileBlocks(tensors, count, state->bits);
   for (int at = 0; at < count;) {
     const unsigned tiles = TakeTensors(tensors, count, static_cast<long long>(a.tile_blocks) * kBlock, &at, &a);
     const unsigned blocks = tiles ? (tiles + kWarps - 1) / kWarps : 1;  // (empty tensors' steps count too)
@@ -548,9 +608,9 @@ extern "C" int switchml_grad_norm(const SmlNormTensor* tensors, int count, doubl
     if (!tiles) continue;
     const unsigned blocks = tiles < kNormBlocks ? tiles : kNormBlocks;
     a.partial = workspace + parts;
-    const cudaError_t e = LaunchOverlapped(NormKernel, blocks, kThreads, 0, 1, static_cast<cudaStream_t>(stream), a);
+    const cudaError_t e = LaunchOverlapped(NormKernel, blocks, kNormThreads, 0, 1, static_cast<cudaStream_t>(stream), a);
     if (e != cudaSuccess) return Launched(e);
     parts += blocks;
   }
-  return Launched(LaunchOverlapped(FinishNormKernel, 1, kThreads, 0, 1, static_cast<cudaStream_t>(stream), workspace, parts, out));
+  return Launched(LaunchOverlapped(FinishNormKernel, 1, kNormThreads, 0, 1, static_cast<cudaStream_t>(stream), workspace, parts, out));
 }

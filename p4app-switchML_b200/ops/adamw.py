@@ -55,6 +55,7 @@ class FusedAdamW(torch.optim.Optimizer):
         self._buffers = []   # of every group: flat tensors
         self._values = 0     # in the flat buffers of all groups
         self._device = None
+        self._checked = []   # settings that have been found in order
         super().__init__(params, {"lr": lr, "betas": betas, "eps": eps, "weight_decay": weight_decay})
 
     @property
@@ -140,7 +141,6 @@ class FusedAdamW(torch.optim.Optimizer):
         ``state_buffers``."""
         return [self._native.masters(i) for i in range(len(self._buffers))]
 
-    @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
@@ -148,11 +148,14 @@ class FusedAdamW(torch.optim.Optimizer):
                 loss = closure()
         settings, tensors = [], []
         for group in self.param_groups:
-            lr, (beta1, beta2) = group["lr"], group["betas"]
-            self._check(group, self._device)
+            lr, (beta1, beta2), eps, decay = group["lr"], group["betas"], group["eps"], group["weight_decay"]
             tensor = isinstance(lr, torch.Tensor)
+            now = (0.0 if tensor else lr, beta1, beta2, eps, decay)
+            if tensor or now not in self._checked:
+                self._check(group, self._device)
+                self._checked = self._checked[-15:] + [now]
             tensors.append(lr if tensor else None)
-            settings.append((0.0 if tensor else lr, beta1, beta2, group["eps"], group["weight_decay"]))
+            settings.append(now)
         self._native.step(settings, tensors, self._max_norm)
         return loss
 
