@@ -64,11 +64,6 @@ __device__ __forceinline__ unsigned Mix(unsigned x) {
   return x ^ (x >> 16);
 }
 
-__device__ __forceinline__ float FromCode(unsigned code) {
-  const __half_raw h = __nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(code), __NV_E4M3);
-  return __half2float(h);
-}
-
 // A tensor's factors in this step.
 struct Factors {
   float size, rsqrt2, keep;  // lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t), 1 - lr * decay
@@ -228,14 +223,45 @@ template <int kWords> __device__ __forceinline__ void StoreWords(void* to, const
   }
 }
 
-// kBlock values of a tensor whose parameter and gradient lie at whole vectors: 8 neighbours per lane, a scale for 4 lanes.
-template <class T, int kBits>
-__device__ __forceinline__ void VectorBlock(const StepArgs& a, const SmlAdamwTensor& x, long long k, long long state, const Factors& f,
-                                            float clip, int lane) {
+// 8 neighbours of a tensor: a whole vector, or only the first `valid` of them (the others count as 0) and at any address.
+template <bool kWhole, class T> __device__ __forceinline__ void LoadTensor(const T* from, int valid, Packed<T>* to) {
+  if constexpr (kWhole) {
+    LoadWords(from, to->w);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      if constexpr (sizeof(T) == 2) {
+        const unsigned v = i < valid ? *reinterpret_cast<const unsigned short*>(from + i) : 0;
+        to->w[i / 2] = i & 1 ? to->w[i / 2] | v << 16 : v;
+      } else {
+        to->w[i] = i < valid ? *reinterpret_cast<const unsigned*>(from + i) : 0;
+      }
+    }
+  }
+}
+template <bool kWhole, class T> __device__ __forceinline__ void StoreTensor(T* to, int valid, const Packed<T>& from) {
+  if constexpr (kWhole) {
+    StoreWords(to, from.w);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      if (i >= valid) continue;
+      if constexpr (sizeof(T) == 2) reinterpret_cast<unsigned short*>(to)[i] = static_cast<unsigned short>(from.w[i / 2] >> (i & 1) * 16);
+      else reinterpret_cast<unsigned*>(to)[i] = from.w[i];
+    }
+  }
+}
+
+// kBlock values of a tensor from k on: 8 neighbours per lane, a scale for 4 lanes. State is there for whole blocks, and what
+// lies behind a tensor's end in it stays 0 (with the smallest scale).
+template <class T, int kBits, bool kWhole>
+__device__ __forceinline__ void StepBlock(const StepArgs& a, const SmlAdamwTensor& x, long long k, long long state, const Factors& f,
+                                          float clip, int lane) {
   using M = std::conditional_t<kBits == 32, float, unsigned char>;
   constexpr int kMoment = kBits / 8;
   k += lane * 8;
   state += k;
+  const int valid = static_cast<int>(max(min(x.numel - k, 8ll), 0ll));
   T* const param = static_cast<T*>(x.param) + k;
   char* const m_at = static_cast<char*>(a.state.exp_avg) + state * kMoment;
   char* const v_at = static_cast<char*>(a.state.exp_avg_sq) + state * kMoment;
@@ -243,8 +269,8 @@ __device__ __forceinline__ void VectorBlock(const StepArgs& a, const SmlAdamwTen
   Packed<__nv_bfloat16> r;
   Packed<M> m, v;
   unsigned char sm = 0, sv = 0;
-  LoadWords(static_cast<const T*>(x.grad) + k, g.w);
-  LoadWords(param, p.w);
+  LoadTensor<kWhole>(static_cast<const T*>(x.grad) + k, valid, &g);
+  LoadTensor<kWhole>(param, valid, &p);
   LoadWords(m_at, m.w);
   LoadWords(v_at, v.w);
   if constexpr (sizeof(T) == 2) LoadWords(a.state.remainder + state, r.w);
@@ -275,7 +301,7 @@ __device__ __forceinline__ void VectorBlock(const StepArgs& a, const SmlAdamwTen
       v.w[2 * i] = __float_as_uint(vb.x), v.w[2 * i + 1] = __float_as_uint(vb.y);
     }
   }
-  StoreWords(param, p.w);
+  StoreTensor<kWhole>(param, valid, p);
   if constexpr (sizeof(T) == 2) StoreWords(a.state.remainder + state, r.w);
   if constexpr (kBits == 8) {
     float largest_m = 0.f, largest_v = 0.f;
@@ -316,66 +342,15 @@ __device__ __forceinline__ void VectorBlock(const StepArgs& a, const SmlAdamwTen
   StoreWords(v_at, v.w);
 }
 
-// Up to kBlock values from k on at any address: the lanes take neighbouring values, 32 of which share a scale.
+// For tensors at other addresses and for ends: out of the way of the other's registers and instructions.
 template <class T, int kBits>
-__device__ __noinline__ void AnyBlock(const StepArgs& a, const SmlAdamwTensor& x, long long k, long long state, Factors f, float clip,
-                                      int lane) {
-  const unsigned first = HashedAt(a, f, state + k);
-#pragma unroll 1
-  for (int j = lane; j < kBlock; j += 32) {
-    const long long at = k + j;
-    const bool in = at < x.numel;
-    T* const param = static_cast<T*>(x.param) + at;
-    float m = 0.f, v = 0.f, g = 0.f, p = 0.f;
-    if (in) {
-      if constexpr (sizeof(T) == 2) p = WithRemainder(__bfloat16_as_ushort(*param), static_cast<unsigned short>(a.state.remainder[state + at]));
-      else p = *param;
-      g = static_cast<float>(static_cast<const T*>(x.grad)[at]);
-      if constexpr (kBits == 32) {
-        m = static_cast<const float*>(a.state.exp_avg)[state + at];
-        v = static_cast<const float*>(a.state.exp_avg_sq)[state + at];
-      } else {
-        m = FromCode(static_cast<const unsigned char*>(a.state.exp_avg)[state + at]) * ScaleOf(a.state.exp_avg_scale[(state + at) / kScaled]);
-        v = FromCode(static_cast<const unsigned char*>(a.state.exp_avg_sq)[state + at]) * ScaleOf(a.state.exp_avg_sq_scale[(state + at) / kScaled]);
-      }
-    }
-    Pair p2(p), m2(m), v2(v);
-    Update(a, f, clip, Pair(g), &p2, &m2, &v2);
-    p = p2.Both().x, m = m2.Both().x, v = v2.Both().x;
-    if (in) {
-      if constexpr (sizeof(T) == 2) {
-        const unsigned w = PlusHalf(p);
-        *param = __ushort_as_bfloat16(static_cast<unsigned short>(w >> 16));
-        a.state.remainder[state + at] = static_cast<short>(w ^ 0x8000u);
-      } else {
-        *param = p;
-      }
-    } else {
-      m = v = 0.f;
-    }
-    if constexpr (kBits == 32) {
-      if (in) {
-        static_cast<float*>(a.state.exp_avg)[state + at] = m;
-        static_cast<float*>(a.state.exp_avg_sq)[state + at] = v;
-      }
-    } else {
-      const unsigned em = ExponentOf(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(m)))));
-      const unsigned ev = ExponentOf(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(v)))));
-      const unsigned h = Mix(first + j);
-      if (in) {
-        static_cast<unsigned char*>(a.state.exp_avg)[state + at] = static_cast<unsigned char>(em < 255 ? MCode(OverScale(Pair(m), em).Both().x, h) >> 24 : kNanCode);
-        static_cast<unsigned char*>(a.state.exp_avg_sq)[state + at] = static_cast<unsigned char>(ev < 255 ? VCode(OverScale(Pair(v), ev).Both().x, v, h) >> 24 : kNanCode);
-        if (lane == 0) {
-          a.state.exp_avg_scale[(state + at) / kScaled] = ScaleByte(em);
-          a.state.exp_avg_sq_scale[(state + at) / kScaled] = ScaleByte(ev);
-        }
-      }
-    }
-  }
+__device__ __noinline__ void StepAnyBlock(const StepArgs& a, const SmlAdamwTensor& x, long long k, long long state, Factors f,
+                                          float clip, int lane) {
+  StepBlock<T, kBits, false>(a, x, k, state, f, clip, lane);
 }
 
 template <class T, int kBits>
-__global__ void __launch_bounds__(kThreads, kBits == 8 ? 6 : 8) AdamwKernel(const __grid_constant__ StepArgs a) {
+__global__ void __launch_bounds__(kThreads, kBits == 8 ? 7 : 8) AdamwKernel(const __grid_constant__ StepArgs a) {
   WaitForEarlierKernels();
   const int lane = threadIdx.x & 31;
   float clip = 1.f;
@@ -395,8 +370,8 @@ __global__ void __launch_bounds__(kThreads, kBits == 8 ? 6 : 8) AdamwKernel(cons
     const Factors f = FactorsOf(a, a.state.steps[x.step] + 1, lr);
     const bool vectors = ((reinterpret_cast<uintptr_t>(x.param) | reinterpret_cast<uintptr_t>(x.grad)) & (8 * sizeof(T) - 1)) == 0;
     for (long long k = start; k < end; k += kBlock) {
-      if (vectors && k + kBlock <= end) VectorBlock<T, kBits>(a, x, k, state, f, clip, lane);
-      else AnyBlock<T, kBits>(a, x, k, state, f, clip, lane);
+      if (vectors && k + kBlock <= end) StepBlock<T, kBits, true>(a, x, k, state, f, clip, lane);
+      else StepAnyBlock<T, kBits>(a, x, k, state, f, clip, lane);
     }
   }
   // The block that ends last counts the step: every block has read the counts by then.
@@ -420,7 +395,7 @@ struct MasterArgs {
   float* out;
 };
 
-// A warp per kBlock values.
+// A warp per kBlock values; `out` is written up to the end of a tensor's last block, with zeros there.
 template <class T>
 __global__ void __launch_bounds__(kThreads) MastersKernel(const __grid_constant__ MasterArgs a) {
   WaitForEarlierKernels();
@@ -429,14 +404,25 @@ __global__ void __launch_bounds__(kThreads) MastersKernel(const __grid_constant_
   const int i = TensorOfTile(a.first_tile, a.count, tile);
   const SmlAdamwTensor& x = a.tensor[i];
   const long long start = static_cast<long long>(tile - a.first_tile[i]) * kBlock, state = static_cast<long long>(x.place) * kBlock;
+  const long long k = start + (threadIdx.x & 31) * 8;
+  Packed<T> p;
+  if (k + 8 <= x.numel && (reinterpret_cast<uintptr_t>(x.param) & (8 * sizeof(T) - 1)) == 0)
+    LoadTensor<true>(static_cast<const T*>(x.param) + k, 8, &p);
+  else
+    LoadTensor<false>(static_cast<const T*>(x.param) + k, static_cast<int>(max(min(x.numel - k, 8ll), 0ll)), &p);
+  Packed<float> out;
+  if constexpr (sizeof(T) == 2) {
+    Packed<__nv_bfloat16> r;
+    LoadWords(a.remainder + state + k, r.w);
 #pragma unroll
-  for (int j = 0; j < kBlock / 32; j++) {
-    const long long k = start + j * 32 + (threadIdx.x & 31);
-    if (k >= x.numel) break;
-    const T p = static_cast<const T*>(x.param)[k];
-    if constexpr (sizeof(T) == 2) a.out[state + k] = WithRemainder(__bfloat16_as_ushort(p), static_cast<unsigned short>(a.remainder[state + k]));
-    else a.out[state + k] = p;
+    for (int i = 0; i < 4; i++) {
+      out.w[2 * i] = __float_as_uint(WithRemainder(p.w[i] & 0xffff, r.w[i]));
+      out.w[2 * i + 1] = __float_as_uint(WithRemainder(p.w[i] >> 16, r.w[i] >> 16));
+    }
+  } else {
+    out = p;
   }
+  StoreWords(a.out + state + k, out.w);
 }
 
 constexpr int kNormThreads = 256;
@@ -447,7 +433,11 @@ struct NormArgs {
   SmlNormTensor tensor[kMaxTensors];
   unsigned first_tile[kMaxTensors + 1];
   int count;
-  double* partial;
+  double* partial;  // one for each block of this launch
+  const double* all;  // of all launches: the last one's last block sums them, if there is a ticket
+  int parts;
+  int* ticket;
+  float* out;
 };
 
 __device__ __forceinline__ double BlockSum(double v) {
@@ -459,6 +449,7 @@ __device__ __forceinline__ double BlockSum(double v) {
   double sum = 0.0;
 #pragma unroll
   for (int w = 0; w < kNormThreads / 32; w++) sum += part[w];
+  __syncthreads();
   return sum;
 }
 
@@ -489,6 +480,15 @@ __device__ __forceinline__ double SquaresOf(const T* x, long long start, long lo
   return sum;
 }
 
+// The root of the sum of all partial sums, in their order.
+__device__ __forceinline__ void Finish(const double* partial, int parts, float* out) {
+  double sum = 0.0;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < parts; i += kNormThreads) sum += __ldcg(partial + i);
+  sum = BlockSum(sum);
+  if (threadIdx.x == 0) *out = static_cast<float>(sqrt(sum));
+}
+
 // Squares are summed in fp64: 2^-53 of a sum over 10^9 values still leaves the result right to its last fp32 bit, and no
 // gradient's square overflows or vanishes.
 __global__ void __launch_bounds__(kNormThreads, 8) NormKernel(const __grid_constant__ NormArgs a) {
@@ -505,15 +505,22 @@ __global__ void __launch_bounds__(kNormThreads, 8) NormKernel(const __grid_const
   }
   sum = BlockSum(sum);
   if (threadIdx.x == 0) a.partial[blockIdx.x] = sum;
+  if (!a.ticket) return;
+  __shared__ bool last;
+  if (threadIdx.x == 0) {
+    __threadfence();
+    last = atomicAdd(a.ticket, 1) == static_cast<int>(gridDim.x) - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  Finish(a.all, a.parts, a.out);
+  if (threadIdx.x == 0) *a.ticket = 0;
 }
 
 __global__ void __launch_bounds__(kNormThreads) FinishNormKernel(const double* partial, int parts, float* out) {
   WaitForEarlierKernels();
-  double sum = 0.0;
-#pragma unroll 8
-  for (int i = threadIdx.x; i < parts; i += kNormThreads) sum += partial[i];
-  sum = BlockSum(sum);
-  if (threadIdx.x == 0) *out = static_cast<float>(sqrt(sum));
+  Finish(partial, parts, out);
 }
 
 // Fills in one launch's share of `tensors` from `*at` on and returns the number of its tiles. Empty tensors take none.
@@ -592,25 +599,29 @@ extern "C" int switchml_adamw_masters(const SmlAdamwTensor* tensors, int count, 
 }
 
 extern "C" long long switchml_grad_norm_workspace(int count) {
-  return count <= 0 ? 0 : static_cast<long long>((count + kMaxTensors - 1) / kMaxTensors) * kNormBlocks;
+  return (count <= 0 ? 1ll : static_cast<long long>((count + kMaxTensors - 1) / kMaxTensors)) * kNormBlocks;
 }
 
-extern "C" int switchml_grad_norm(const SmlNormTensor* tensors, int count, double* workspace, float* out, void* stream) {
-  if (count < 0 || !out || (count && (!tensors || !workspace))) return -1;
+extern "C" int switchml_grad_norm(const SmlNormTensor* tensors, int count, double* workspace, int* ticket, float* out, void* stream) {
+  if (count < 0 || !out || !workspace || (count && !tensors)) return -1;
   for (int i = 0; i < count; i++)
     if (tensors[i].numel < 0 || tensors[i].numel > kMaxNumel || (tensors[i].numel && !tensors[i].data) ||
         (tensors[i].type != SML_ADAMW_F32 && tensors[i].type != SML_ADAMW_BF16))
       return -1;
   NormArgs a;
-  int parts = 0;
-  for (int at = 0; at < count;) {
+  a.all = workspace, a.out = out, a.parts = 0;
+  int at = 0;
+  do {
     const unsigned tiles = TakeTensors(tensors, count, kNormTile, &at, &a);
-    if (!tiles) continue;
-    const unsigned blocks = tiles < kNormBlocks ? tiles : kNormBlocks;
-    a.partial = workspace + parts;
+    if (!tiles && !(ticket && at == count)) continue;
+    const unsigned each = (tiles + kNormBlocks - 1) / kNormBlocks;  // tiles of a block: the same number for all but the last
+    const unsigned blocks = tiles ? (tiles + each - 1) / each : 1;
+    a.partial = workspace + a.parts;
+    a.parts += blocks;
+    a.ticket = at == count ? ticket : nullptr;
     const cudaError_t e = LaunchOverlapped(NormKernel, blocks, kNormThreads, 0, 1, static_cast<cudaStream_t>(stream), a);
     if (e != cudaSuccess) return Launched(e);
-    parts += blocks;
-  }
-  return Launched(LaunchOverlapped(FinishNormKernel, 1, kNormThreads, 0, 1, static_cast<cudaStream_t>(stream), workspace, parts, out));
+  } while (at < count);
+  if (ticket) return 0;
+  return Launched(LaunchOverlapped(FinishNormKernel, 1, kNormThreads, 0, 1, static_cast<cudaStream_t>(stream), a.all, a.parts, out));
 }

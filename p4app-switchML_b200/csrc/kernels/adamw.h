@@ -66,7 +66,8 @@ typedef struct SmlAdamwStep {
 /* One step of `count` tensors of one type (any number: cut into launches). */
 int switchml_adamw_step(const SmlAdamwTensor* tensors, int count, const SmlAdamwState* state, const SmlAdamwStep* step, int type,
                         void* stream);
-/* The fp32 values of `count` tensors of one type, each at its place of the flat buffer `out`. */
+/* The fp32 values of `count` tensors of one type, each at its place of the flat buffer `out`, zeros up to the next
+ * multiple of SML_ADAMW_ALIGN. */
 int switchml_adamw_masters(const SmlAdamwTensor* tensors, int count, const short* remainder, float* out, int type, void* stream);
 
 typedef struct SmlNormTensor {
@@ -77,8 +78,9 @@ typedef struct SmlNormTensor {
 
 /* Doubles of workspace for `count` tensors. */
 long long switchml_grad_norm_workspace(int count);
-/* out = sqrt of the sum of squares of all tensors, summed in fp64; the same bits in every run. `workspace` need not be initialised. */
-int switchml_grad_norm(const SmlNormTensor* tensors, int count, double* workspace, float* out, void* stream);
+/* out = sqrt of the sum of squares of all tensors, summed in fp64; the same bits in every run. `workspace` need not be
+ * initialised. `ticket`: one int, zero between launches, saves a launch; or NULL. */
+int switchml_grad_norm(const SmlNormTensor* tensors, int count, double* workspace, int* ticket, float* out, void* stream);
 
 #ifdef __cplusplus
 }

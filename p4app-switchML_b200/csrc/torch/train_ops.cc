@@ -145,33 +145,40 @@ int AdamwType(const Tensor& t) { return t.scalar_type() == at::kFloat ? SML_ADAM
 // Same values in the same places of memory, without gaps: what an elementwise pass over memory may take.
 bool Dense(const Tensor& t) { return t.is_non_overlapping_and_dense(); }
 
-void NormOf(const std::vector<SmlNormTensor>& list, Tensor* workspace, const Tensor& out) {
-  const int64_t doubles = std::max<int64_t>(1, switchml_grad_norm_workspace(static_cast<int>(list.size())));
+void NormOf(const std::vector<SmlNormTensor>& list, Tensor* workspace, int* ticket, const Tensor& out) {
+  const int64_t doubles = switchml_grad_norm_workspace(static_cast<int>(list.size()));
   if (!workspace->defined() || workspace->numel() < doubles) *workspace = at::empty({doubles}, out.options().dtype(at::kDouble));
-  Check(switchml_grad_norm(list.data(), static_cast<int>(list.size()), workspace->data_ptr<double>(), out.data_ptr<float>(), CurrentStream()),
+  Check(switchml_grad_norm(list.data(), static_cast<int>(list.size()), workspace->data_ptr<double>(), ticket, out.data_ptr<float>(), CurrentStream()),
         "grad_norm");
 }
 
-Tensor GradNorm(const std::vector<Tensor>& tensors) {
-  TORCH_CHECK_VALUE(!tensors.empty(), "grad_norm: no tensors");
+// Takes a list as it is: a vector of tensors would count every one of them up and down.
+Tensor GradNorm(const py::list& tensors) {
+  const Py_ssize_t count = PyList_GET_SIZE(tensors.ptr());
+  TORCH_CHECK_VALUE(count > 0, "grad_norm: no tensors");
   std::vector<SmlNormTensor> list;
   std::vector<Tensor> keep;
-  list.reserve(tensors.size());
-  for (const Tensor& t : tensors) {
-    TORCH_CHECK_TYPE(t.layout() == at::kStrided && Known(t), "grad_norm: a tensor is ", t.layout(), " ", t.scalar_type(),
-                     ": strided float32 or bfloat16 is wanted");
-    TORCH_CHECK_VALUE(t.is_cuda() && t.device() == tensors[0].device(), "grad_norm: tensors on ", tensors[0].device(), " and ", t.device(),
-                      ": one CUDA device is wanted");
-  }
-  const c10::cuda::OptionalCUDAGuard device(tensors[0].device());
+  list.reserve(count);
+  at::Device where(at::kCPU);
   at::NoGradGuard no_grad;
-  for (const Tensor& t : tensors) {
-    if (!Dense(t)) keep.push_back(t.contiguous());
-    const Tensor& use = Dense(t) ? t : keep.back();
-    list.push_back({Data(use), use.numel(), AdamwType(use)});
+  std::optional<c10::cuda::CUDAGuard> device;
+  for (Py_ssize_t i = 0; i < count; i++) {
+    PyObject* const item = PyList_GET_ITEM(tensors.ptr(), i);
+    TORCH_CHECK_TYPE(THPVariable_Check(item), "grad_norm: tensors are wanted");
+    const Tensor* t = &THPVariable_Unpack(item);
+    TORCH_CHECK_TYPE(t->layout() == at::kStrided && Known(*t), "grad_norm: a tensor is ", t->layout(), " ", t->scalar_type(),
+                     ": strided float32 or bfloat16 is wanted");
+    if (i == 0) where = t->device();
+    TORCH_CHECK_VALUE(t->is_cuda() && t->device() == where, "grad_norm: tensors on ", where, " and ", t->device(), ": one CUDA device is wanted");
+    if (i == 0) device.emplace(where);
+    if (!Dense(*t)) {
+      keep.push_back(t->contiguous());
+      t = &keep.back();
+    }
+    list.push_back({Data(*t), t->numel(), AdamwType(*t)});
   }
-  Tensor out = at::empty({}, tensors[0].options().dtype(at::kFloat).requires_grad(false)), workspace;
-  NormOf(list, &workspace, out);
+  Tensor out = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(where)), workspace;
+  NormOf(list, &workspace, nullptr, out);
   return out;
 }
 
@@ -233,7 +240,7 @@ class Adamw {
         if (tensors_.size() > begin) runs.push_back({k, {begin, tensors_.size(), type}});
       }
     }
-    if (max_norm) NormOf(norms_, &workspace_, norm_);
+    if (max_norm) NormOf(norms_, &workspace_, ticket_.data_ptr<int>(), norm_);
     for (const auto& [k, run] : runs) {
       const Group& g = groups_[k];
       const auto bytes = [](const Tensor& t) { return static_cast<unsigned char*>(Data(t)); };
@@ -251,7 +258,7 @@ class Adamw {
   Tensor Masters(size_t k) {
     const c10::cuda::OptionalCUDAGuard device(ticket_.device());
     const Group& g = groups_.at(k);
-    Tensor out = at::zeros({g.exp_avg.numel()}, g.exp_avg.options().dtype(at::kFloat));
+    Tensor out = at::empty({g.exp_avg.numel()}, g.exp_avg.options().dtype(at::kFloat));
     for (const int type : {SML_ADAMW_F32, SML_ADAMW_BF16}) {
       tensors_.clear();
       for (size_t i = 0; i < g.params.size(); i++) {
