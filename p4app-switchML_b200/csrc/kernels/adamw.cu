@@ -13,9 +13,15 @@
 
 #include "kernels/adamw.h"
 #include "kernels/dependent_launch.cuh"
+#include "kernels/packed.cuh"
 
+using switchml::kernels::Fma;
 using switchml::kernels::LaunchOverlapped;
 using switchml::kernels::LetNextKernelStart;
+using switchml::kernels::LoadWords;
+using switchml::kernels::Packed;
+using switchml::kernels::Pair;
+using switchml::kernels::StoreWords;
 using switchml::kernels::WaitForEarlierKernels;
 
 namespace {
@@ -108,34 +114,6 @@ __device__ __forceinline__ float Reciprocal(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// Two fp32 operations in one instruction: the 8-bit kernel's pace is that of issuing instructions.
-struct Pair {
-  unsigned long long w;
-  __device__ __forceinline__ Pair() {}
-  __device__ __forceinline__ Pair(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(w) : "f"(x), "f"(y)); }
-  __device__ __forceinline__ explicit Pair(float x) : Pair(x, x) {}
-  __device__ __forceinline__ float2 Both() const {
-    float2 v;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(w));
-    return v;
-  }
-};
-__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
-  Pair r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.w) : "l"(a.w), "l"(b.w));
-  return r;
-}
-__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
-  Pair r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.w) : "l"(a.w), "l"(b.w));
-  return r;
-}
-__device__ __forceinline__ Pair Fma(Pair a, Pair b, Pair c) {
-  Pair r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.w) : "l"(a.w), "l"(b.w), "l"(c.w));
-  return r;
-}
-
 // The larger of two, the largest of three; NaN where one of them is.
 __device__ __forceinline__ float Larger(float a, float b) {
   float r;
@@ -183,17 +161,8 @@ __device__ __forceinline__ unsigned VCode(float y, float v, unsigned hash) {
 }
 constexpr unsigned kNanCode = 0x7f;
 
-// 8 values of a lane that are neighbours in memory, as they lie there.
-template <class T> struct Packed;
-template <> struct Packed<float> {
-  unsigned w[8];
-  __device__ __forceinline__ float At(int i) const { return __uint_as_float(w[i]); }
-};
-template <> struct Packed<__nv_bfloat16> {
-  unsigned w[4];
-  __device__ __forceinline__ float At(int i) const { return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16); }
-};
-template <> struct Packed<unsigned char> {
+// 8 numbers in e4m3.
+struct Packed8 {
   unsigned w[2];
   __device__ __forceinline__ Pair Decoded(int i) const {  // values 2i and 2i + 1 of e4m3
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i / 2] >> (i & 1) * 16), __NV_E4M3);
@@ -201,27 +170,6 @@ template <> struct Packed<unsigned char> {
     return Pair(v.x, v.y);
   }
 };
-
-template <int kWords> __device__ __forceinline__ void LoadWords(const void* from, unsigned (&w)[kWords]) {
-  if constexpr (kWords == 8) {
-    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(from));
-  } else if constexpr (kWords == 4) {
-    asm volatile("ld.global.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(from));
-  } else {
-    asm volatile("ld.global.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(from));
-  }
-}
-template <int kWords> __device__ __forceinline__ void StoreWords(void* to, const unsigned (&w)[kWords]) {
-  if constexpr (kWords == 8) {
-    asm volatile("st.global.v8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};"
-                 :: "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "l"(to) : "memory");
-  } else if constexpr (kWords == 4) {
-    asm volatile("st.global.v4.b32 [%4], {%0,%1,%2,%3};" :: "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "l"(to) : "memory");
-  } else {
-    asm volatile("st.global.v2.b32 [%2], {%0,%1};" :: "r"(w[0]), "r"(w[1]), "l"(to) : "memory");
-  }
-}
 
 // 8 neighbours of a tensor: a whole vector, or only the first `valid` of them (the others count as 0) and at any address.
 template <bool kWhole, class T> __device__ __forceinline__ void LoadTensor(const T* from, int valid, Packed<T>* to) {
@@ -257,7 +205,7 @@ template <bool kWhole, class T> __device__ __forceinline__ void StoreTensor(T* t
 template <class T, int kBits, bool kWhole>
 __device__ __forceinline__ void StepBlock(const StepArgs& a, const SmlAdamwTensor& x, long long k, long long state, const Factors& f,
                                           float clip, int lane) {
-  using M = std::conditional_t<kBits == 32, float, unsigned char>;
+  using M = std::conditional_t<kBits == 32, Packed<float>, Packed8>;
   constexpr int kMoment = kBits / 8;
   k += lane * 8;
   state += k;
@@ -267,7 +215,7 @@ __device__ __forceinline__ void StepBlock(const StepArgs& a, const SmlAdamwTenso
   char* const v_at = static_cast<char*>(a.state.exp_avg_sq) + state * kMoment;
   Packed<T> p, g;
   Packed<__nv_bfloat16> r;
-  Packed<M> m, v;
+  M m, v;
   unsigned char sm = 0, sv = 0;
   LoadTensor<kWhole>(static_cast<const T*>(x.grad) + k, valid, &g);
   LoadTensor<kWhole>(param, valid, &p);

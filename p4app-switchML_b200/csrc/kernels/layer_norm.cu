@@ -9,10 +9,19 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "kernels/dependent_launch.cuh"
 #include "kernels/layer_norm.h"
+#include "kernels/packed.cuh"
 
+using switchml::kernels::Fma;
 using switchml::kernels::LaunchOverlapped;
+using switchml::kernels::LetNextKernelStart;
+using switchml::kernels::LoadWords;
+using switchml::kernels::Pair;
+using switchml::kernels::StoreWords;
+using switchml::kernels::Sum;
 using switchml::kernels::WaitForEarlierKernels;
 
 namespace {
@@ -45,6 +54,285 @@ __device__ __forceinline__ float WarpSum(float v) {
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+
+// ---- rows that stay in registers ----
+//
+// kThreads of a row, a power of two from 1 to 512, hold kHeld of its values each: vector j of kVec neighbouring values is
+// number j * threads + (the thread's number in the row). A block has several such groups. kVec is what the addresses
+// and the length of the rows allow: 8, 2 or 1.
+
+__device__ __forceinline__ void GroupBarrier(int group, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(threads) : "memory");
+}
+
+// The sums over a group of threads, in all of them. Two calls that follow each other take different `part`s: between two
+// uses of the same one lies the other's barrier.
+__device__ __forceinline__ float2 GroupSum(float2 v, int group, int threads, float2* part) {
+  for (int o = threads < 32 ? threads / 2 : 16; o; o >>= 1) {
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+  }
+  if (threads > 32) {
+    const int warps = threads / 32, first = group * warps;
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    GroupBarrier(group, threads);
+    v = make_float2(0.f, 0.f);
+    for (int w = 0; w < warps; w++) v.x += part[first + w].x, v.y += part[first + w].y;
+  }
+  return v;
+}
+__device__ __forceinline__ float GroupSum(float v, int group, int threads, float2* part) {
+  for (int o = threads < 32 ? threads / 2 : 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (threads > 32) {
+    const int warps = threads / 32, first = group * warps;
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5].x = v;
+    GroupBarrier(group, threads);
+    v = 0.f;
+    for (int w = 0; w < warps; w++) v += part[first + w].x;
+  }
+  return v;
+}
+
+// What arithmetic takes at once of a vector's values: two of them, where there are two.
+template <int kVec> using Num = std::conditional_t<kVec == 1, float, Pair>;
+
+// kVec values of type T in registers, as kVec / 2 pairs or as the one that it is.
+template <class T, int kVec> struct Vector {
+  static constexpr int kWords = kVec * sizeof(T) / 4;  // 0: half a word
+  static constexpr int kNums = kVec == 1 ? 1 : kVec / 2;
+  unsigned w[kWords ? kWords : 1];
+  __device__ __forceinline__ void Load(const T* from) {
+    if constexpr (kWords) LoadWords(from, w);
+    else w[0] = *reinterpret_cast<const unsigned short*>(from);
+  }
+  __device__ __forceinline__ void Store(T* to) const {
+    if constexpr (kWords) StoreWords(to, w);
+    else *reinterpret_cast<unsigned short*>(to) = static_cast<unsigned short>(w[0]);
+  }
+  __device__ __forceinline__ void Clear() {
+#pragma unroll
+    for (int i = 0; i < (kWords ? kWords : 1); i++) w[i] = 0;
+  }
+  __device__ __forceinline__ Num<kVec> At(int i) const {
+    if constexpr (kVec == 1) return __uint_as_float(sizeof(T) == 4 ? w[0] : w[0] << 16);
+    else if constexpr (sizeof(T) == 4) return Pair(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    else return Pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+  }
+  __device__ __forceinline__ void Set(int i, Num<kVec> v) {
+    if constexpr (kVec == 1) {
+      w[0] = sizeof(T) == 4 ? __float_as_uint(v) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
+    } else {
+      const float2 both = v.Both();
+      if constexpr (sizeof(T) == 4) {
+        w[2 * i] = __float_as_uint(both.x), w[2 * i + 1] = __float_as_uint(both.y);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(both.x, both.y);
+        w[i] = *reinterpret_cast<const unsigned*>(&h);
+      }
+    }
+  }
+};
+
+// kVec values of weight or bias, of either type.
+template <int kVec>
+__device__ __forceinline__ void LoadParameter(const Parameter& p, int i, float none, Num<kVec> (&out)[Vector<float, kVec>::kNums]) {
+  constexpr int kNums = Vector<float, kVec>::kNums;
+  if (!p.data) {
+#pragma unroll
+    for (int k = 0; k < kNums; k++) out[k] = Num<kVec>(none);
+  } else if (p.type == SML_NORM_F32) {
+    Vector<float, kVec> v;
+    v.Load(static_cast<const float*>(p.data) + i);
+#pragma unroll
+    for (int k = 0; k < kNums; k++) out[k] = v.At(k);
+  } else {
+    Vector<__nv_bfloat16, kVec> v;
+    v.Load(static_cast<const __nv_bfloat16*>(p.data) + i);
+#pragma unroll
+    for (int k = 0; k < kNums; k++) out[k] = v.At(k);
+  }
+}
+
+// Held by a thread. (Single values and pairs need more addresses and conditions than vectors do.)
+__host__ __device__ constexpr int ForwardHeld(int vec) { return vec == 8 ? 32 : 16; }
+constexpr int kForwardThreads = 256;  // (512 where a row needs them)
+
+template <class T, int kVec>
+__global__ void __launch_bounds__(512)
+ForwardKernel(const T* x, const T* residual, Parameter weight, Parameter bias, T* y, T* sum, float* mean_out, float* rstd_out,
+              long long rows, int n, float eps, int threads) {
+  using N = Num<kVec>;
+  constexpr int kVectors = ForwardHeld(kVec) / kVec, kNums = Vector<T, kVec>::kNums;
+  __shared__ float2 part[2][16];
+  const int group = threadIdx.x / threads, t = threadIdx.x % threads, groups = blockDim.x / threads;
+  WaitForEarlierKernels();
+  for (long long first = static_cast<long long>(blockIdx.x) * groups; first < rows; first += static_cast<long long>(gridDim.x) * groups) {
+    const long long row = first + group;
+    const int columns = row < rows ? n : 0;
+    const T* const x_row = x + row * n;
+    Vector<T, kVec> s[kVectors];
+#pragma unroll
+    for (int j = 0; j < kVectors; j++) {
+      const int c = (j * threads + t) * kVec;
+      s[j].Clear();
+      if (c < columns) s[j].Load(x_row + c);
+    }
+    if (residual) {
+      Vector<T, kVec> r[kVectors];
+#pragma unroll
+      for (int j = 0; j < kVectors; j++) {
+        const int c = (j * threads + t) * kVec;
+        r[j].Clear();
+        if (c < columns) r[j].Load(residual + row * n + c);
+      }
+#pragma unroll
+      for (int j = 0; j < kVectors; j++) {
+        const int c = (j * threads + t) * kVec;
+#pragma unroll
+        for (int i = 0; i < kNums; i++) s[j].Set(i, s[j].At(i) + r[j].At(i));
+        if (c < columns) s[j].Store(sum + row * n + c);
+      }
+    }
+    N total(0.f);
+#pragma unroll
+    for (int j = 0; j < kVectors; j++) {
+#pragma unroll
+      for (int i = 0; i < kNums; i++) total = total + s[j].At(i);
+    }
+    const float mean = GroupSum(Sum(total), group, threads, part[0]) / n;
+    N squares(0.f);
+#pragma unroll
+    for (int j = 0; j < kVectors; j++) {
+      if ((j * threads + t) * kVec < n) {
+#pragma unroll
+        for (int i = 0; i < kNums; i++) {
+          const N d = s[j].At(i) + N(-mean);
+          squares = Fma(d, d, squares);
+        }
+      }
+    }
+    const float rstd = 1.f / sqrtf(GroupSum(Sum(squares), group, threads, part[1]) / n + eps);
+#pragma unroll
+    for (int j = 0; j < kVectors; j++) {
+      const int c = (j * threads + t) * kVec;
+      if (c < columns) {
+        N w[kNums], b[kNums];
+        LoadParameter<kVec>(weight, c, 1.f, w);
+        LoadParameter<kVec>(bias, c, 0.f, b);
+#pragma unroll
+        for (int i = 0; i < kNums; i++) s[j].Set(i, Fma((s[j].At(i) + N(-mean)) * N(rstd), w[i], b[i]));
+        s[j].Store(y + row * n + c);
+      }
+    }
+    if (columns && t == 0 && mean_out) mean_out[row] = mean, rstd_out[row] = rstd;
+  }
+}
+
+// The backward pass of rows that a group holds, and the sums over the rows that each block saw, in the order of the groups.
+__host__ __device__ constexpr int BackwardHeld(int vec, int size) { return vec == 8 && size == 2 ? 32 : 16; }
+constexpr int kBackwardThreads = 512;
+
+template <class T, int kVec>
+__global__ void __launch_bounds__(kBackwardThreads, 1)
+BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const float* mean_in, const float* rstd_in, T* dx,
+               float* workspace, long long rows, int n, int threads) {
+  using N = Num<kVec>;
+  constexpr int kHeld = BackwardHeld(kVec, sizeof(T)), kVectors = kHeld / kVec, kNums = Vector<T, kVec>::kNums, kSums = kVectors * kNums;
+  extern __shared__ __align__(16) unsigned char shared[];
+  N* const sums = reinterpret_cast<N*>(shared);  // [2 * kSums][groups / 2][threads]
+  __shared__ float2 part[2][16];
+  const int group = threadIdx.x / threads, t = threadIdx.x % threads, groups = kBackwardThreads / threads;
+  N dw[kSums], db[kSums];
+#pragma unroll
+  for (int i = 0; i < kSums; i++) dw[i] = db[i] = N(0.f);
+  WaitForEarlierKernels();
+  int turn = 0;
+  for (long long first = static_cast<long long>(blockIdx.x) * groups; first < rows; first += static_cast<long long>(gridDim.x) * groups) {
+    const long long row = first + group;
+    const bool live = row < rows;
+    const int columns = live ? n : 0;
+    Vector<T, kVec> d[kVectors], v[kVectors];
+#pragma unroll
+    for (int j = 0; j < kVectors; j++) {
+      const int c = (j * threads + t) * kVec;
+      d[j].Clear();
+      v[j].Clear();
+      if (c < columns) {
+        d[j].Load(dy + row * n + c);
+        v[j].Load(s + row * n + c);
+      }
+    }
+    const float mean = live ? mean_in[row] : 0.f, rstd = live ? rstd_in[row] : 0.f;
+    N c1(0.f), c2(0.f);
+#pragma unroll
+    for (int j = 0; j < kVectors; j++) {
+      const int c = (j * threads + t) * kVec;
+      if (c < n) {  // (a row that is not there has gradients of 0)
+        N w[kNums];
+        LoadParameter<kVec>(weight, c, 1.f, w);
+#pragma unroll
+        for (int i = 0; i < kNums; i++) {
+          const N xhat = (v[j].At(i) + N(-mean)) * N(rstd), dyi = d[j].At(i), g = dyi * w[i];
+          c1 = c1 + g;
+          c2 = Fma(g, xhat, c2);
+          dw[j * kNums + i] = Fma(dyi, xhat, dw[j * kNums + i]);
+          db[j * kNums + i] = db[j * kNums + i] + dyi;
+        }
+      }
+    }
+    const float2 c12 = GroupSum(make_float2(Sum(c1), Sum(c2)), group, threads, part[turn]);
+    turn ^= 1;
+    const N minus_c1(-c12.x / n), minus_c2(-c12.y / n);
+#pragma unroll
+    for (int j = 0; j < kVectors; j++) {
+      const int c = (j * threads + t) * kVec;
+      if (c < columns) {
+        N w[kNums];
+        LoadParameter<kVec>(weight, c, 1.f, w);
+        Vector<T, kVec> more;
+        more.Clear();
+        if (dsum) more.Load(dsum + row * n + c);
+#pragma unroll
+        for (int i = 0; i < kNums; i++) {
+          const N xhat = (v[j].At(i) + N(-mean)) * N(rstd);
+          v[j].Set(i, Fma(Fma(xhat, minus_c2, Fma(d[j].At(i), w[i], minus_c1)), N(rstd), more.At(i)));
+        }
+        v[j].Store(dx + row * n + c);
+      }
+    }
+  }
+  if (!workspace) return;
+  for (int half = groups / 2; half; half /= 2) {
+    if (group >= half && group < 2 * half) {
+#pragma unroll
+      for (int i = 0; i < kSums; i++) {
+        sums[(i * half + group - half) * threads + t] = dw[i];
+        sums[((kSums + i) * half + group - half) * threads + t] = db[i];
+      }
+    }
+    __syncthreads();
+    if (group < half) {
+#pragma unroll
+      for (int i = 0; i < kSums; i++) {
+        dw[i] = dw[i] + sums[(i * half + group) * threads + t];
+        db[i] = db[i] + sums[((kSums + i) * half + group) * threads + t];
+      }
+    }
+    __syncthreads();
+  }
+  if (group) return;
+  float* const out = workspace + static_cast<long long>(blockIdx.x) * 2 * n;
+#pragma unroll
+  for (int i = 0; i < kSums; i++) {
+    const int c = (i / kNums * threads + t) * kVec + i % kNums * 2;
+    if (c < n) {
+      *reinterpret_cast<N*>(out + c) = dw[i];
+      *reinterpret_cast<N*>(out + n + c) = db[i];  // (pairs: n is even)
+    }
+  }
+}
+
+// ---- rows of any length ----
 
 constexpr int kAnyThreads = 256;
 
@@ -149,7 +437,7 @@ ColumnsAnyKernel(const T* dy, const T* s, const float* mean, const float* rstd, 
   }
 }
 
-constexpr int kFinishColumns = 32, kFinishRows = 16;
+constexpr int kFinishColumns = 32, kFinishRows = 32;
 
 // The sums of `parts` partial sums, in order.
 __global__ void __launch_bounds__(kFinishColumns* kFinishRows)
@@ -159,7 +447,7 @@ FinishColumnsKernel(const float* workspace, void* dweight, void* dbias, int part
   float2 sum = make_float2(0.f, 0.f);
   WaitForEarlierKernels();
   if (column < n) {
-#pragma unroll 4
+#pragma unroll 5
     for (int p = r; p < parts; p += kFinishRows) {
       const float* from = workspace + static_cast<long long>(p) * 2 * n;
       sum.x += from[column];
@@ -193,28 +481,73 @@ int RowShares(long long rows, int n) {
 
 bool Known(int type) { return type == SML_NORM_F32 || type == SML_NORM_BF16; }
 
-template <class T>
-int Forward(const void* x, const void* residual, Parameter weight, Parameter bias, void* y, void* sum, float* mean, float* rstd,
-            long long rows, int n, float eps, cudaStream_t stream) {
-  return Launched(LaunchOverlapped(ForwardAnyKernel<T>, RowBlocks(rows), kAnyThreads, 0, 1, stream, static_cast<const T*>(x),
-                                   static_cast<const T*>(residual), weight, bias, static_cast<T*>(y), static_cast<T*>(sum), mean,
-                                   rstd, rows, n, eps));
+// Values that are read and written at once: what the length of the rows and all addresses allow.
+struct Alignment {
+  uintptr_t bits = 0;
+  template <class T> void Of(const T* tensor) { bits |= reinterpret_cast<uintptr_t>(tensor) * (4 / sizeof(T)); }  // as if it were fp32
+  void Of(const Parameter& p) { bits |= reinterpret_cast<uintptr_t>(p.data) * (p.type == SML_NORM_F32 ? 1 : 2); }
+  int Vec(int n) const { return n % 8 == 0 && bits % 32 == 0 ? 8 : n % 2 == 0 && bits % 8 == 0 ? 2 : 1; }
+};
+
+// Threads of a row, or 0: too long to be held.
+int ThreadsOf(int n, int held) {
+  int threads = 1;
+  while (threads <= 512 && static_cast<long long>(threads) * held < n) threads *= 2;
+  return threads <= 512 ? threads : 0;
+}
+
+unsigned BackwardBlocks(long long rows, int threads) {
+  const long long groups = kBackwardThreads / threads, wanted = (rows + groups - 1) / groups;
+  return static_cast<unsigned>(wanted < 148 ? wanted : 148);
 }
 
 template <class T>
-int Backward(const void* dy, const void* dsum, const void* s, Parameter weight, const float* mean, const float* rstd, void* dx,
-             void* dweight, void* dbias, float* workspace, long long rows, int n, int wtype, cudaStream_t stream) {
-  cudaError_t e = LaunchOverlapped(BackwardAnyKernel<T>, RowBlocks(rows), kAnyThreads, 0, 1, stream, static_cast<const T*>(dy),
-                                   static_cast<const T*>(dsum), static_cast<const T*>(s), weight, mean, rstd, static_cast<T*>(dx),
-                                   rows, n);
-  if (e != cudaSuccess || (!dweight && !dbias)) return Launched(e);
-  const int shares = RowShares(rows, n);
-  const unsigned columns = static_cast<unsigned>((static_cast<long long>(n) + 31) / 32);
-  ColumnsAnyKernel<T><<<dim3(columns, shares), kAnyThreads, 0, stream>>>(static_cast<const T*>(dy), static_cast<const T*>(s), mean,
-                                                                          rstd, workspace, rows, n);
-  if ((e = cudaGetLastError()) != cudaSuccess) return Launched(e);
+int Forward(const void* x_in, const void* residual_in, Parameter weight, Parameter bias, void* y_in, void* sum_in, float* mean,
+            float* rstd, long long rows, int n, float eps, cudaStream_t stream) {
+  const T *x = static_cast<const T*>(x_in), *residual = static_cast<const T*>(residual_in);
+  T *y = static_cast<T*>(y_in), *sum = static_cast<T*>(sum_in);
+  Alignment at;
+  at.Of(x), at.Of(residual), at.Of(weight), at.Of(bias), at.Of(y), at.Of(sum);
+  const int vec = at.Vec(n), threads = ThreadsOf(n, ForwardHeld(vec));
+  if (!threads)
+    return Launched(LaunchOverlapped(ForwardAnyKernel<T>, RowBlocks(rows), kAnyThreads, 0, 1, stream, x, residual, weight, bias, y, sum,
+                                     mean, rstd, rows, n, eps));
+  const int block = threads > kForwardThreads ? threads : kForwardThreads, groups = block / threads;
+  return Launched(LaunchOverlapped(vec == 8 ? ForwardKernel<T, 8> : vec == 2 ? ForwardKernel<T, 2> : ForwardKernel<T, 1>,
+                                   RowBlocks((rows + groups - 1) / groups), block, 0, 1, stream, x, residual, weight, bias, y, sum, mean,
+                                   rstd, rows, n, eps, threads));
+}
+
+template <class T>
+int Backward(const void* dy_in, const void* dsum_in, const void* s_in, Parameter weight, const float* mean, const float* rstd,
+             void* dx_in, void* dweight, void* dbias, float* workspace, long long rows, int n, int wtype, cudaStream_t stream) {
+  const T *dy = static_cast<const T*>(dy_in), *dsum = static_cast<const T*>(dsum_in), *s = static_cast<const T*>(s_in);
+  T* dx = static_cast<T*>(dx_in);
+  if (!dweight && !dbias) workspace = nullptr;
+  Alignment at;
+  at.Of(dy), at.Of(dsum), at.Of(s), at.Of(weight), at.Of(dx);
+  const int vec = at.Vec(n), held = BackwardHeld(vec, sizeof(T)), threads = ThreadsOf(n, held);
+  int parts = 0;
+  cudaError_t e;
+  if (threads) {
+    const auto kernel = vec == 8 ? BackwardKernel<T, 8> : vec == 2 ? BackwardKernel<T, 2> : BackwardKernel<T, 1>;
+    const int shared = kBackwardThreads / 2 * 2 * held * static_cast<int>(sizeof(float));
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
+    if (e != cudaSuccess) return Launched(e);
+    parts = static_cast<int>(BackwardBlocks(rows, threads));
+    e = LaunchOverlapped(kernel, parts, kBackwardThreads, shared, 1, stream, dy, dsum, s, weight, mean, rstd, dx, workspace, rows, n, threads);
+  } else {
+    e = LaunchOverlapped(BackwardAnyKernel<T>, RowBlocks(rows), kAnyThreads, 0, 1, stream, dy, dsum, s, weight, mean, rstd, dx, rows, n);
+    if (e == cudaSuccess && workspace) {
+      parts = RowShares(rows, n);
+      const unsigned columns = static_cast<unsigned>((static_cast<long long>(n) + 31) / 32);
+      ColumnsAnyKernel<T><<<dim3(columns, parts), kAnyThreads, 0, stream>>>(dy, s, mean, rstd, workspace, rows, n);
+      e = cudaGetLastError();
+    }
+  }
+  if (e != cudaSuccess || !workspace) return Launched(e);
   return Launched(LaunchOverlapped(FinishColumnsKernel, (n - 1) / kFinishColumns + 1, kFinishColumns * kFinishRows, 0, 1, stream,
-                                   workspace, dweight, dbias, shares, n, wtype));
+                                   workspace, dweight, dbias, parts, n, wtype));
 }
 
 }  // namespace
@@ -230,7 +563,13 @@ extern "C" int switchml_layer_norm_forward(const void* x, const void* residual, 
 
 extern "C" long long switchml_layer_norm_workspace(long long rows, int features, int type) {
   if (rows <= 0 || features <= 0 || !Known(type)) return 0;
-  return 2ll * features * RowShares(rows, features);
+  // (Which of the kernels it will be depends on the addresses too.)
+  long long parts = RowShares(rows, features);
+  for (const int vec : {1, 8}) {
+    const int threads = ThreadsOf(features, BackwardHeld(vec, type == SML_NORM_F32 ? 4 : 2));
+    if (threads && BackwardBlocks(rows, threads) > parts) parts = BackwardBlocks(rows, threads);
+  }
+  return 2ll * features * parts;
 }
 
 extern "C" int switchml_layer_norm_backward(const void* dy, const void* dsum, const void* s, const void* weight, const float* mean,
