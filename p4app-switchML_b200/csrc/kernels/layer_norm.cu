@@ -57,8 +57,8 @@ __device__ __forceinline__ float WarpSum(float v) {
 
 // ---- rows that stay in registers ----
 //
-// kThreads of a row, a power of two from 1 to 512, hold kHeld of its values each: vector j of kVec neighbouring values is
-// number j * threads + (the thread's number in the row). A block has several such groups. kVec is what the addresses
+// The threads of a row, a power of two from 1 to 512, hold kHeld of its values each: vector j of kVec neighbouring values
+// is number j * threads + (the thread's number in the row). A block has several such groups. kVec is what the addresses
 // and the length of the rows allow: 8, 2 or 1.
 
 __device__ __forceinline__ void GroupBarrier(int group, int threads) {
@@ -109,9 +109,9 @@ template <class T, int kVec> struct Vector {
     if constexpr (kWords) StoreWords(to, w);
     else *reinterpret_cast<unsigned short*>(to) = static_cast<unsigned short>(w[0]);
   }
-  __device__ __forceinline__ void Clear() {
-#pragma unroll
-    for (int i = 0; i < (kWords ? kWords : 1); i++) w[i] = 0;
+  __device__ __forceinline__ void LoadIf(bool there, const T* from) {
+    if constexpr (kWords) switchml::kernels::LoadWordsIf(there, from, w);
+    else w[0] = there ? *reinterpret_cast<const unsigned short*>(from) : 0;
   }
   __device__ __forceinline__ Num<kVec> At(int i) const {
     if constexpr (kVec == 1) return __uint_as_float(sizeof(T) == 4 ? w[0] : w[0] << 16);
@@ -153,152 +153,159 @@ __device__ __forceinline__ void LoadParameter(const Parameter& p, int i, float n
   }
 }
 
-// Held by a thread. (Single values and pairs need more addresses and conditions than vectors do.)
-__host__ __device__ constexpr int ForwardHeld(int vec) { return vec == 8 ? 32 : 16; }
+// Values that a thread holds. kWhole: the row is exactly what its threads hold, nothing has to be asked.
+__host__ __device__ constexpr int ForwardHeld(int vec, int size) { return vec == 8 && size == 2 ? 32 : 16; }
 constexpr int kForwardThreads = 256;  // (512 where a row needs them)
 
-template <class T, int kVec>
-__global__ void __launch_bounds__(512)
+template <class T, int kVec, bool kWhole>
+__global__ void __launch_bounds__(512, 2)
 ForwardKernel(const T* x, const T* residual, Parameter weight, Parameter bias, T* y, T* sum, float* mean_out, float* rstd_out,
               long long rows, int n, float eps, int threads) {
   using N = Num<kVec>;
-  constexpr int kVectors = ForwardHeld(kVec) / kVec, kNums = Vector<T, kVec>::kNums;
+  constexpr int kVectors = ForwardHeld(kVec, sizeof(T)) / kVec, kNums = Vector<T, kVec>::kNums;
   __shared__ float2 part[2][16];
   const int group = threadIdx.x / threads, t = threadIdx.x % threads, groups = blockDim.x / threads;
+  const int step = threads * kVec;
   WaitForEarlierKernels();
   for (long long first = static_cast<long long>(blockIdx.x) * groups; first < rows; first += static_cast<long long>(gridDim.x) * groups) {
     const long long row = first + group;
-    const int columns = row < rows ? n : 0;
-    const T* const x_row = x + row * n;
-    Vector<T, kVec> s[kVectors];
+    const bool live = row < rows;
+    const long long at = row * n + t * kVec;
+    const int left = n - t * kVec;  // vector j is there where j * step < left
+    N s[kVectors][kNums];
+    {
+      Vector<T, kVec> raw[kVectors], more[kVectors];
 #pragma unroll
-    for (int j = 0; j < kVectors; j++) {
-      const int c = (j * threads + t) * kVec;
-      s[j].Clear();
-      if (c < columns) s[j].Load(x_row + c);
-    }
-    if (residual) {
-      Vector<T, kVec> r[kVectors];
+      for (int j = 0; j < kVectors; j++) raw[j].LoadIf(live && (kWhole || j * step < left), x + at + j * step);
+      if (residual) {
 #pragma unroll
-      for (int j = 0; j < kVectors; j++) {
-        const int c = (j * threads + t) * kVec;
-        r[j].Clear();
-        if (c < columns) r[j].Load(residual + row * n + c);
+        for (int j = 0; j < kVectors; j++) more[j].LoadIf(live && (kWhole || j * step < left), residual + at + j * step);
+#pragma unroll
+        for (int j = 0; j < kVectors; j++) {
+#pragma unroll
+          for (int i = 0; i < kNums; i++) raw[j].Set(i, raw[j].At(i) + more[j].At(i));
+          if (live && (kWhole || j * step < left)) raw[j].Store(sum + at + j * step);
+        }
       }
 #pragma unroll
       for (int j = 0; j < kVectors; j++) {
-        const int c = (j * threads + t) * kVec;
 #pragma unroll
-        for (int i = 0; i < kNums; i++) s[j].Set(i, s[j].At(i) + r[j].At(i));
-        if (c < columns) s[j].Store(sum + row * n + c);
+        for (int i = 0; i < kNums; i++) s[j][i] = raw[j].At(i);
       }
     }
     N total(0.f);
 #pragma unroll
     for (int j = 0; j < kVectors; j++) {
 #pragma unroll
-      for (int i = 0; i < kNums; i++) total = total + s[j].At(i);
+      for (int i = 0; i < kNums; i++) total = total + s[j][i];
     }
     const float mean = GroupSum(Sum(total), group, threads, part[0]) / n;
     N squares(0.f);
 #pragma unroll
     for (int j = 0; j < kVectors; j++) {
-      if ((j * threads + t) * kVec < n) {
 #pragma unroll
-        for (int i = 0; i < kNums; i++) {
-          const N d = s[j].At(i) + N(-mean);
-          squares = Fma(d, d, squares);
-        }
+      for (int i = 0; i < kNums; i++) {
+        s[j][i] = s[j][i] + N(-mean);
+        if (kWhole || j * step < left) squares = Fma(s[j][i], s[j][i], squares);
       }
     }
     const float rstd = 1.f / sqrtf(GroupSum(Sum(squares), group, threads, part[1]) / n + eps);
 #pragma unroll
     for (int j = 0; j < kVectors; j++) {
-      const int c = (j * threads + t) * kVec;
-      if (c < columns) {
+      if (live && (kWhole || j * step < left)) {
         N w[kNums], b[kNums];
-        LoadParameter<kVec>(weight, c, 1.f, w);
-        LoadParameter<kVec>(bias, c, 0.f, b);
+        LoadParameter<kVec>(weight, j * step + t * kVec, 1.f, w);
+        LoadParameter<kVec>(bias, j * step + t * kVec, 0.f, b);
+        Vector<T, kVec> out;
 #pragma unroll
-        for (int i = 0; i < kNums; i++) s[j].Set(i, Fma((s[j].At(i) + N(-mean)) * N(rstd), w[i], b[i]));
-        s[j].Store(y + row * n + c);
+        for (int i = 0; i < kNums; i++) out.Set(i, Fma(s[j][i] * N(rstd), w[i], b[i]));
+        out.Store(y + at + j * step);
       }
     }
-    if (columns && t == 0 && mean_out) mean_out[row] = mean, rstd_out[row] = rstd;
+    if (live && t == 0 && mean_out) mean_out[row] = mean, rstd_out[row] = rstd;
   }
 }
 
 // The backward pass of rows that a group holds, and the sums over the rows that each block saw, in the order of the groups.
-__host__ __device__ constexpr int BackwardHeld(int vec, int size) { return vec == 8 && size == 2 ? 32 : 16; }
+// A block per SM goes through the rows; a group reads its next row while it deals with one.
+__host__ __device__ constexpr int BackwardHeld() { return 16; }
 constexpr int kBackwardThreads = 512;
 
-template <class T, int kVec>
+template <class T, int kVec, bool kWhole>
 __global__ void __launch_bounds__(kBackwardThreads, 1)
 BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const float* mean_in, const float* rstd_in, T* dx,
                float* workspace, long long rows, int n, int threads) {
   using N = Num<kVec>;
-  constexpr int kHeld = BackwardHeld(kVec, sizeof(T)), kVectors = kHeld / kVec, kNums = Vector<T, kVec>::kNums, kSums = kVectors * kNums;
+  constexpr int kHeld = BackwardHeld(), kVectors = kHeld / kVec, kNums = Vector<T, kVec>::kNums, kSums = kVectors * kNums;
   extern __shared__ __align__(16) unsigned char shared[];
   N* const sums = reinterpret_cast<N*>(shared);  // [2 * kSums][groups / 2][threads]
   __shared__ float2 part[2][16];
   const int group = threadIdx.x / threads, t = threadIdx.x % threads, groups = kBackwardThreads / threads;
-  N dw[kSums], db[kSums];
+  const int step = threads * kVec, left = n - t * kVec;
+  const long long stride = static_cast<long long>(gridDim.x) * groups;
+  N w[kVectors][kNums], dw[kVectors][kNums], db[kVectors][kNums];
 #pragma unroll
-  for (int i = 0; i < kSums; i++) dw[i] = db[i] = N(0.f);
-  WaitForEarlierKernels();
-  int turn = 0;
-  for (long long first = static_cast<long long>(blockIdx.x) * groups; first < rows; first += static_cast<long long>(gridDim.x) * groups) {
-    const long long row = first + group;
+  for (int j = 0; j < kVectors; j++) {
+#pragma unroll
+    for (int i = 0; i < kNums; i++) w[j][i] = dw[j][i] = db[j][i] = N(0.f);
+  }
+  Vector<T, kVec> d[kVectors], v[kVectors];
+  float mean = 0.f, rstd = 0.f;
+  const auto load = [&](long long row) {
     const bool live = row < rows;
-    const int columns = live ? n : 0;
-    Vector<T, kVec> d[kVectors], v[kVectors];
+    const long long at = row * n + t * kVec;
 #pragma unroll
     for (int j = 0; j < kVectors; j++) {
-      const int c = (j * threads + t) * kVec;
-      d[j].Clear();
-      v[j].Clear();
-      if (c < columns) {
-        d[j].Load(dy + row * n + c);
-        v[j].Load(s + row * n + c);
-      }
+      d[j].LoadIf(live && (kWhole || j * step < left), dy + at + j * step);
+      v[j].LoadIf(live && (kWhole || j * step < left), s + at + j * step);
     }
-    const float mean = live ? mean_in[row] : 0.f, rstd = live ? rstd_in[row] : 0.f;
-    N c1(0.f), c2(0.f);
+    mean = live ? mean_in[row] : 0.f, rstd = live ? rstd_in[row] : 0.f;
+  };
+  WaitForEarlierKernels();
+#pragma unroll
+  for (int j = 0; j < kVectors; j++) {
+    if (kWhole || j * step < left) LoadParameter<kVec>(weight, j * step + t * kVec, 1.f, w[j]);
+  }
+  long long first = static_cast<long long>(blockIdx.x) * groups;
+  load(first + group);
+  int turn = 0;
+  for (; first < rows; first += stride) {
+    const long long row = first + group, at = row * n + t * kVec;
+    const bool live = row < rows;
+    const float r = rstd;
+    N c1(0.f), c2(0.f), xhat[kVectors][kNums], g[kVectors][kNums];
 #pragma unroll
     for (int j = 0; j < kVectors; j++) {
-      const int c = (j * threads + t) * kVec;
-      if (c < n) {  // (a row that is not there has gradients of 0)
-        N w[kNums];
-        LoadParameter<kVec>(weight, c, 1.f, w);
 #pragma unroll
-        for (int i = 0; i < kNums; i++) {
-          const N xhat = (v[j].At(i) + N(-mean)) * N(rstd), dyi = d[j].At(i), g = dyi * w[i];
-          c1 = c1 + g;
-          c2 = Fma(g, xhat, c2);
-          dw[j * kNums + i] = Fma(dyi, xhat, dw[j * kNums + i]);
-          db[j * kNums + i] = db[j * kNums + i] + dyi;
-        }
+      for (int i = 0; i < kNums; i++) {  // (what is not there has gradients of 0)
+        const N dyi = d[j].At(i);
+        xhat[j][i] = (v[j].At(i) + N(-mean)) * N(r);
+        g[j][i] = dyi * w[j][i];
+        c1 = c1 + g[j][i];
+        c2 = Fma(g[j][i], xhat[j][i], c2);
+        dw[j][i] = Fma(dyi, xhat[j][i], dw[j][i]);
+        db[j][i] = db[j][i] + dyi;
       }
     }
+    Vector<T, kVec> more[kVectors];
+    if (dsum) {
+#pragma unroll
+      for (int j = 0; j < kVectors; j++) more[j].LoadIf(live && (kWhole || j * step < left), dsum + at + j * step);
+    }
+    load(row + stride);
     const float2 c12 = GroupSum(make_float2(Sum(c1), Sum(c2)), group, threads, part[turn]);
     turn ^= 1;
     const N minus_c1(-c12.x / n), minus_c2(-c12.y / n);
 #pragma unroll
     for (int j = 0; j < kVectors; j++) {
-      const int c = (j * threads + t) * kVec;
-      if (c < columns) {
-        N w[kNums];
-        LoadParameter<kVec>(weight, c, 1.f, w);
-        Vector<T, kVec> more;
-        more.Clear();
-        if (dsum) more.Load(dsum + row * n + c);
+      Vector<T, kVec> out;
 #pragma unroll
-        for (int i = 0; i < kNums; i++) {
-          const N xhat = (v[j].At(i) + N(-mean)) * N(rstd);
-          v[j].Set(i, Fma(Fma(xhat, minus_c2, Fma(d[j].At(i), w[i], minus_c1)), N(rstd), more.At(i)));
-        }
-        v[j].Store(dx + row * n + c);
+      for (int i = 0; i < kNums; i++) {
+        N e = Fma(xhat[j][i], minus_c2, g[j][i] + minus_c1) * N(r);
+        if (dsum) e = e + more[j].At(i);
+        out.Set(i, e);
       }
+      if (live && (kWhole || j * step < left)) out.Store(dx + at + j * step);
     }
   }
   if (!workspace) return;
@@ -306,28 +313,28 @@ BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const f
     if (group >= half && group < 2 * half) {
 #pragma unroll
       for (int i = 0; i < kSums; i++) {
-        sums[(i * half + group - half) * threads + t] = dw[i];
-        sums[((kSums + i) * half + group - half) * threads + t] = db[i];
+        sums[(i * half + group - half) * threads + t] = dw[i / kNums][i % kNums];
+        sums[((kSums + i) * half + group - half) * threads + t] = db[i / kNums][i % kNums];
       }
     }
     __syncthreads();
     if (group < half) {
 #pragma unroll
       for (int i = 0; i < kSums; i++) {
-        dw[i] = dw[i] + sums[(i * half + group) * threads + t];
-        db[i] = db[i] + sums[((kSums + i) * half + group) * threads + t];
+        dw[i / kNums][i % kNums] = dw[i / kNums][i % kNums] + sums[(i * half + group) * threads + t];
+        db[i / kNums][i % kNums] = db[i / kNums][i % kNums] + sums[((kSums + i) * half + group) * threads + t];
       }
     }
     __syncthreads();
   }
   if (group) return;
-  float* const out = workspace + static_cast<long long>(blockIdx.x) * 2 * n;
+  float* const out = workspace + static_cast<long long>(blockIdx.x) * 2 * n + t * kVec;
 #pragma unroll
   for (int i = 0; i < kSums; i++) {
-    const int c = (i / kNums * threads + t) * kVec + i % kNums * 2;
-    if (c < n) {
-      *reinterpret_cast<N*>(out + c) = dw[i];
-      *reinterpret_cast<N*>(out + n + c) = db[i];  // (pairs: n is even)
+    const int c = i / kNums * step + i % kNums * 2;
+    if (kWhole || i / kNums * step < left) {
+      *reinterpret_cast<N*>(out + c) = dw[i / kNums][i % kNums];
+      *reinterpret_cast<N*>(out + n + c) = db[i / kNums][i % kNums];  // (pairs: n is even)
     }
   }
 }
@@ -508,13 +515,14 @@ int Forward(const void* x_in, const void* residual_in, Parameter weight, Paramet
   T *y = static_cast<T*>(y_in), *sum = static_cast<T*>(sum_in);
   Alignment at;
   at.Of(x), at.Of(residual), at.Of(weight), at.Of(bias), at.Of(y), at.Of(sum);
-  const int vec = at.Vec(n), threads = ThreadsOf(n, ForwardHeld(vec));
+  const int vec = at.Vec(n), held = ForwardHeld(vec, sizeof(T)), threads = ThreadsOf(n, held);
   if (!threads)
     return Launched(LaunchOverlapped(ForwardAnyKernel<T>, RowBlocks(rows), kAnyThreads, 0, 1, stream, x, residual, weight, bias, y, sum,
                                      mean, rstd, rows, n, eps));
   const int block = threads > kForwardThreads ? threads : kForwardThreads, groups = block / threads;
-  return Launched(LaunchOverlapped(vec == 8 ? ForwardKernel<T, 8> : vec == 2 ? ForwardKernel<T, 2> : ForwardKernel<T, 1>,
-                                   RowBlocks((rows + groups - 1) / groups), block, 0, 1, stream, x, residual, weight, bias, y, sum, mean,
+  const auto kernel = vec == 1 ? ForwardKernel<T, 1, false> : vec == 2 ? ForwardKernel<T, 2, false>
+                      : n == threads * held ? ForwardKernel<T, 8, true> : ForwardKernel<T, 8, false>;
+  return Launched(LaunchOverlapped(kernel, RowBlocks((rows + groups - 1) / groups), block, 0, 1, stream, x, residual, weight, bias, y, sum, mean,
                                    rstd, rows, n, eps, threads));
 }
 
@@ -526,11 +534,12 @@ int Backward(const void* dy_in, const void* dsum_in, const void* s_in, Parameter
   if (!dweight && !dbias) workspace = nullptr;
   Alignment at;
   at.Of(dy), at.Of(dsum), at.Of(s), at.Of(weight), at.Of(dx);
-  const int vec = at.Vec(n), held = BackwardHeld(vec, sizeof(T)), threads = ThreadsOf(n, held);
+  const int vec = at.Vec(n), held = BackwardHeld(), threads = ThreadsOf(n, held);
   int parts = 0;
   cudaError_t e;
   if (threads) {
-    const auto kernel = vec == 8 ? BackwardKernel<T, 8> : vec == 2 ? BackwardKernel<T, 2> : BackwardKernel<T, 1>;
+    const auto kernel = vec == 1 ? BackwardKernel<T, 1, false> : vec == 2 ? BackwardKernel<T, 2, false>
+                        : n == threads * held ? BackwardKernel<T, 8, true> : BackwardKernel<T, 8, false>;
     const int shared = kBackwardThreads / 2 * 2 * held * static_cast<int>(sizeof(float));
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
     if (e != cudaSuccess) return Launched(e);
@@ -563,13 +572,8 @@ extern "C" int switchml_layer_norm_forward(const void* x, const void* residual, 
 
 extern "C" long long switchml_layer_norm_workspace(long long rows, int features, int type) {
   if (rows <= 0 || features <= 0 || !Known(type)) return 0;
-  // (Which of the kernels it will be depends on the addresses too.)
-  long long parts = RowShares(rows, features);
-  for (const int vec : {1, 8}) {
-    const int threads = ThreadsOf(features, BackwardHeld(vec, type == SML_NORM_F32 ? 4 : 2));
-    if (threads && BackwardBlocks(rows, threads) > parts) parts = BackwardBlocks(rows, threads);
-  }
-  return 2ll * features * parts;
+  const int threads = ThreadsOf(features, BackwardHeld());
+  return 2ll * features * (threads ? static_cast<int>(BackwardBlocks(rows, threads)) : RowShares(rows, features));
 }
 
 extern "C" int switchml_layer_norm_backward(const void* dy, const void* dsum, const void* s, const void* weight, const float* mean,
