@@ -57,41 +57,44 @@ __device__ __forceinline__ float WarpSum(float v) {
 
 // ---- rows that stay in registers ----
 //
-// The threads of a row, a power of two from 1 to 512, hold kHeld of its values each: vector j of kVec neighbouring values
-// is number j * threads + (the thread's number in the row). A block has several such groups. kVec is what the addresses
-// and the length of the rows allow: 8, 2 or 1.
+// A group of threads holds a row: 8 lanes of a warp, or 1 to 24 whole warps. Each lane has kHeld values: kHeld / kVec
+// vectors of kVec neighbours, between which lie kLanes (8 or 32) * kVec values, so that addresses differ by constants; warp w
+// has the values from w * 32 * kHeld on. kVec is what the addresses and the length of the rows allow: 8, 2 or 1.
+// Groups go through their rows by themselves, and warps of a group meet at a barrier of their own.
 
-__device__ __forceinline__ void GroupBarrier(int group, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(threads) : "memory");
-}
-
-// The sums over a group of threads, in all of them. Two calls that follow each other take different `part`s: between two
-// uses of the same one lies the other's barrier.
-__device__ __forceinline__ float2 GroupSum(float2 v, int group, int threads, float2* part) {
-  for (int o = threads < 32 ? threads / 2 : 16; o; o >>= 1) {
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+template <int kLanes> struct Group {
+  int number, warps, lane, warp;  // number: in the block; warps: of a group; lane, warp: in the group
+  unsigned mask;
+  __device__ __forceinline__ explicit Group(int warps_of_group) : warps(warps_of_group) {
+    const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
+    lane = l % kLanes;
+    mask = kLanes == 32 ? 0xffffffffu : ((1u << kLanes % 32) - 1) << (l - lane);
+    number = kLanes == 32 ? w / warps : threadIdx.x / kLanes;
+    warp = kLanes == 32 ? w - number * warps : 0;
   }
-  if (threads > 32) {
-    const int warps = threads / 32, first = group * warps;
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-    GroupBarrier(group, threads);
-    v = make_float2(0.f, 0.f);
-    for (int w = 0; w < warps; w++) v.x += part[first + w].x, v.y += part[first + w].y;
+  // The first value of this thread's.
+  __device__ __forceinline__ int First(int held, int vec) const { return warp * 32 * held + lane * vec; }
+  // The sum over the group, in all its threads. Two calls that follow each other take different `part`s (a V for each warp of the block): between
+  // two uses of the same one lies the other's barrier.
+  template <class V> __device__ __forceinline__ V Sum(V v, V* part) const {
+#pragma unroll
+    for (int o = kLanes / 2; o; o >>= 1) v = Plus(v, Shuffle(v, o));
+    if (kLanes == 32 && warps > 1) {
+      if (lane == 0) part[number * warps + warp] = v;
+      asm volatile("bar.sync %0, %1;" ::"r"(number + 1), "r"(warps * 32) : "memory");
+      v = lane < warps ? part[number * warps + lane] : V{};
+      for (int o = warps > 16 ? 16 : warps > 8 ? 8 : warps > 4 ? 4 : warps > 2 ? 2 : 1; o; o >>= 1) v = Plus(v, Shuffle(v, o));
+      v = Broadcast(v);
+    }
+    return v;
   }
-  return v;
-}
-__device__ __forceinline__ float GroupSum(float v, int group, int threads, float2* part) {
-  for (int o = threads < 32 ? threads / 2 : 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (threads > 32) {
-    const int warps = threads / 32, first = group * warps;
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5].x = v;
-    GroupBarrier(group, threads);
-    v = 0.f;
-    for (int w = 0; w < warps; w++) v += part[first + w].x;
-  }
-  return v;
-}
+  __device__ __forceinline__ float Shuffle(float v, int o) const { return __shfl_xor_sync(mask, v, o); }
+  __device__ __forceinline__ float2 Shuffle(float2 v, int o) const { return make_float2(Shuffle(v.x, o), Shuffle(v.y, o)); }
+  __device__ __forceinline__ float Broadcast(float v) const { return __shfl_sync(mask, v, 0); }
+  __device__ __forceinline__ float2 Broadcast(float2 v) const { return make_float2(Broadcast(v.x), Broadcast(v.y)); }
+  static __device__ __forceinline__ float Plus(float a, float b) { return a + b; }
+  static __device__ __forceinline__ float2 Plus(float2 a, float2 b) { return make_float2(a.x + b.x, a.y + b.y); }
+};
 
 // What arithmetic takes at once of a vector's values: two of them, where there are two.
 template <int kVec> using Num = std::conditional_t<kVec == 1, float, Pair>;
@@ -155,36 +158,33 @@ __device__ __forceinline__ void LoadParameter(const Parameter& p, int i, float n
 
 // Values that a thread holds. kWhole: the row is exactly what its threads hold, nothing has to be asked.
 __host__ __device__ constexpr int ForwardHeld(int vec, int size) { return vec == 8 && size == 2 ? 32 : 16; }
-constexpr int kForwardThreads = 256;  // (512 where a row needs them)
 
-template <class T, int kVec, bool kWhole>
+template <class T, int kVec, int kLanes, bool kWhole>
 __global__ void __launch_bounds__(512, 2)
 ForwardKernel(const T* x, const T* residual, Parameter weight, Parameter bias, T* y, T* sum, float* mean_out, float* rstd_out,
-              long long rows, int n, float eps, int threads) {
+              long long rows, int n, float eps, int groups, int warps) {
   using N = Num<kVec>;
-  constexpr int kVectors = ForwardHeld(kVec, sizeof(T)) / kVec, kNums = Vector<T, kVec>::kNums;
-  __shared__ float2 part[2][16];
-  const int group = threadIdx.x / threads, t = threadIdx.x % threads, groups = blockDim.x / threads;
-  const int step = threads * kVec;
+  constexpr int kHeld = ForwardHeld(kVec, sizeof(T)), kVectors = kHeld / kVec, kNums = Vector<T, kVec>::kNums, kStep = kLanes * kVec;
+  __shared__ float part[2][16];
+  const Group<kLanes> group(warps);
+  const int column = group.First(kHeld, kVec), left = n - column;  // vector j is there where j * kStep < left
   WaitForEarlierKernels();
-  for (long long first = static_cast<long long>(blockIdx.x) * groups; first < rows; first += static_cast<long long>(gridDim.x) * groups) {
-    const long long row = first + group;
-    const bool live = row < rows;
-    const long long at = row * n + t * kVec;
-    const int left = n - t * kVec;  // vector j is there where j * step < left
+  for (long long row = static_cast<long long>(blockIdx.x) * groups + group.number; row < rows;
+       row += static_cast<long long>(gridDim.x) * groups) {
+    const long long at = row * n + column;
     N s[kVectors][kNums];
     {
       Vector<T, kVec> raw[kVectors], more[kVectors];
 #pragma unroll
-      for (int j = 0; j < kVectors; j++) raw[j].LoadIf(live && (kWhole || j * step < left), x + at + j * step);
+      for (int j = 0; j < kVectors; j++) raw[j].LoadIf(kWhole || j * kStep < left, x + at + j * kStep);
       if (residual) {
 #pragma unroll
-        for (int j = 0; j < kVectors; j++) more[j].LoadIf(live && (kWhole || j * step < left), residual + at + j * step);
+        for (int j = 0; j < kVectors; j++) more[j].LoadIf(kWhole || j * kStep < left, residual + at + j * kStep);
 #pragma unroll
         for (int j = 0; j < kVectors; j++) {
 #pragma unroll
           for (int i = 0; i < kNums; i++) raw[j].Set(i, raw[j].At(i) + more[j].At(i));
-          if (live && (kWhole || j * step < left)) raw[j].Store(sum + at + j * step);
+          if (kWhole || j * kStep < left) raw[j].Store(sum + at + j * kStep);
         }
       }
 #pragma unroll
@@ -199,50 +199,53 @@ ForwardKernel(const T* x, const T* residual, Parameter weight, Parameter bias, T
 #pragma unroll
       for (int i = 0; i < kNums; i++) total = total + s[j][i];
     }
-    const float mean = GroupSum(Sum(total), group, threads, part[0]) / n;
+    const float mean = group.Sum(Sum(total), part[0]) / n;
     N squares(0.f);
 #pragma unroll
     for (int j = 0; j < kVectors; j++) {
 #pragma unroll
       for (int i = 0; i < kNums; i++) {
         s[j][i] = s[j][i] + N(-mean);
-        if (kWhole || j * step < left) squares = Fma(s[j][i], s[j][i], squares);
+        if (kWhole || j * kStep < left) squares = Fma(s[j][i], s[j][i], squares);
       }
     }
-    const float rstd = 1.f / sqrtf(GroupSum(Sum(squares), group, threads, part[1]) / n + eps);
+    const float rstd = 1.f / sqrtf(group.Sum(Sum(squares), part[1]) / n + eps);
 #pragma unroll
     for (int j = 0; j < kVectors; j++) {
-      if (live && (kWhole || j * step < left)) {
+      if (kWhole || j * kStep < left) {
         N w[kNums], b[kNums];
-        LoadParameter<kVec>(weight, j * step + t * kVec, 1.f, w);
-        LoadParameter<kVec>(bias, j * step + t * kVec, 0.f, b);
+        LoadParameter<kVec>(weight, column + j * kStep, 1.f, w);
+        LoadParameter<kVec>(bias, column + j * kStep, 0.f, b);
         Vector<T, kVec> out;
 #pragma unroll
         for (int i = 0; i < kNums; i++) out.Set(i, Fma(s[j][i] * N(rstd), w[i], b[i]));
-        out.Store(y + at + j * step);
+        out.Store(y + at + j * kStep);
       }
     }
-    if (live && t == 0 && mean_out) mean_out[row] = mean, rstd_out[row] = rstd;
+    if (column == 0 && mean_out) mean_out[row] = mean, rstd_out[row] = rstd;
   }
 }
 
 // The backward pass of rows that a group holds, and the sums over the rows that each block saw, in the order of the groups.
 // A block per SM goes through the rows; a group reads its next row while it deals with one.
-__host__ __device__ constexpr int BackwardHeld() { return 16; }
-constexpr int kBackwardThreads = 512;
+// Sums, normalised values, gradients and what is read ahead take 6 to 8 registers per value: 16 bf16 values in vectors fit
+// the 128 registers of 16 warps, of the others 8 fit the 85 of 24 warps. (16 of those, for rows that need them, spill.)
+__host__ __device__ constexpr int BackwardThreads(int held) { return held == 16 ? 512 : 768; }
+int BackwardHeld(int n, int vec, int size) { return (vec == 8 && size == 2) || n > BackwardThreads(8) / 32 * 32 * 8 ? 16 : 8; }
 
-template <class T, int kVec, bool kWhole>
-__global__ void __launch_bounds__(kBackwardThreads, 1)
+template <class T, int kVec, int kLanes, bool kWhole, int kHeld>
+__global__ void __launch_bounds__(BackwardThreads(kHeld), 1)
 BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const float* mean_in, const float* rstd_in, T* dx,
-               float* workspace, long long rows, int n, int threads) {
+               float* workspace, long long rows, int n, int groups, int warps) {
   using N = Num<kVec>;
-  constexpr int kHeld = BackwardHeld(), kVectors = kHeld / kVec, kNums = Vector<T, kVec>::kNums, kSums = kVectors * kNums;
+  constexpr int kVectors = kHeld / kVec, kNums = Vector<T, kVec>::kNums, kStep = kLanes * kVec;
   extern __shared__ __align__(16) unsigned char shared[];
-  N* const sums = reinterpret_cast<N*>(shared);  // [2 * kSums][groups / 2][threads]
-  __shared__ float2 part[2][16];
-  const int group = threadIdx.x / threads, t = threadIdx.x % threads, groups = kBackwardThreads / threads;
-  const int step = threads * kVec, left = n - t * kVec;
+  __shared__ float2 part[2][BackwardThreads(kHeld) / 32];
+  const Group<kLanes> group(warps);
+  const int column = group.First(kHeld, kVec), left = n - column;
   const long long stride = static_cast<long long>(gridDim.x) * groups;
+  // The weight stays in registers where these suffice, else it comes from L1 for every row.
+  constexpr bool kKeepWeight = sizeof(T) == 2 && kVec > 1;
   N w[kVectors][kNums], dw[kVectors][kNums], db[kVectors][kNums];
 #pragma unroll
   for (int j = 0; j < kVectors; j++) {
@@ -252,30 +255,34 @@ BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const f
   Vector<T, kVec> d[kVectors], v[kVectors];
   float mean = 0.f, rstd = 0.f;
   const auto load = [&](long long row) {
-    const bool live = row < rows;
-    const long long at = row * n + t * kVec;
+    const long long at = row * n + column;
 #pragma unroll
     for (int j = 0; j < kVectors; j++) {
-      d[j].LoadIf(live && (kWhole || j * step < left), dy + at + j * step);
-      v[j].LoadIf(live && (kWhole || j * step < left), s + at + j * step);
+      d[j].LoadIf(kWhole || j * kStep < left, dy + at + j * kStep);
+      v[j].LoadIf(kWhole || j * kStep < left, s + at + j * kStep);
     }
-    mean = live ? mean_in[row] : 0.f, rstd = live ? rstd_in[row] : 0.f;
+    mean = mean_in[row], rstd = rstd_in[row];
   };
   WaitForEarlierKernels();
+  if constexpr (kKeepWeight) {
 #pragma unroll
-  for (int j = 0; j < kVectors; j++) {
-    if (kWhole || j * step < left) LoadParameter<kVec>(weight, j * step + t * kVec, 1.f, w[j]);
+    for (int j = 0; j < kVectors; j++) {
+      if (kWhole || j * kStep < left) LoadParameter<kVec>(weight, column + j * kStep, 1.f, w[j]);
+    }
   }
-  long long first = static_cast<long long>(blockIdx.x) * groups;
-  load(first + group);
+  // (Groups that do not fit into the block any more have no row.)
+  long long row = group.number < groups ? static_cast<long long>(blockIdx.x) * groups + group.number : rows;
+  if (row < rows) load(row);
   int turn = 0;
-  for (; first < rows; first += stride) {
-    const long long row = first + group, at = row * n + t * kVec;
-    const bool live = row < rows;
+  for (; row < rows; row += stride) {
+    const long long at = row * n + column;
     const float r = rstd;
     N c1(0.f), c2(0.f), xhat[kVectors][kNums], g[kVectors][kNums];
 #pragma unroll
     for (int j = 0; j < kVectors; j++) {
+      if constexpr (!kKeepWeight) {
+        if (kWhole || j * kStep < left) LoadParameter<kVec>(weight, column + j * kStep, 1.f, w[j]);
+      }
 #pragma unroll
       for (int i = 0; i < kNums; i++) {  // (what is not there has gradients of 0)
         const N dyi = d[j].At(i);
@@ -290,10 +297,10 @@ BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const f
     Vector<T, kVec> more[kVectors];
     if (dsum) {
 #pragma unroll
-      for (int j = 0; j < kVectors; j++) more[j].LoadIf(live && (kWhole || j * step < left), dsum + at + j * step);
+      for (int j = 0; j < kVectors; j++) more[j].LoadIf(kWhole || j * kStep < left, dsum + at + j * kStep);
     }
-    load(row + stride);
-    const float2 c12 = GroupSum(make_float2(Sum(c1), Sum(c2)), group, threads, part[turn]);
+    if (row + stride < rows) load(row + stride);
+    const float2 c12 = group.Sum(make_float2(Sum(c1), Sum(c2)), part[turn]);
     turn ^= 1;
     const N minus_c1(-c12.x / n), minus_c2(-c12.y / n);
 #pragma unroll
@@ -305,34 +312,39 @@ BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const f
         if (dsum) e = e + more[j].At(i);
         out.Set(i, e);
       }
-      if (live && (kWhole || j * step < left)) out.Store(dx + at + j * step);
+      if (kWhole || j * kStep < left) out.Store(dx + at + j * kStep);
     }
   }
   if (!workspace) return;
-  for (int half = groups / 2; half; half /= 2) {
-    if (group >= half && group < 2 * half) {
+  // The upper half of the groups gives its sums to the lower one until one has all.
+  N* const sums = reinterpret_cast<N*>(shared);
+  const int width = kLanes == 32 ? warps * 32 : kLanes, t = kLanes == 32 ? group.warp * 32 + group.lane : group.lane;
+  for (int there = groups; there > 1;) {
+    const int half = (there + 1) / 2;
+    __syncthreads();
+    if (group.number >= half && group.number < there) {
 #pragma unroll
-      for (int i = 0; i < kSums; i++) {
-        sums[(i * half + group - half) * threads + t] = dw[i / kNums][i % kNums];
-        sums[((kSums + i) * half + group - half) * threads + t] = db[i / kNums][i % kNums];
+      for (int i = 0; i < kVectors * kNums; i++) {
+        sums[(2 * i * half + group.number - half) * width + t] = dw[i / kNums][i % kNums];
+        sums[((2 * i + 1) * half + group.number - half) * width + t] = db[i / kNums][i % kNums];
       }
     }
     __syncthreads();
-    if (group < half) {
+    if (group.number < there - half) {
 #pragma unroll
-      for (int i = 0; i < kSums; i++) {
-        dw[i / kNums][i % kNums] = dw[i / kNums][i % kNums] + sums[(i * half + group) * threads + t];
-        db[i / kNums][i % kNums] = db[i / kNums][i % kNums] + sums[((kSums + i) * half + group) * threads + t];
+      for (int i = 0; i < kVectors * kNums; i++) {
+        dw[i / kNums][i % kNums] = dw[i / kNums][i % kNums] + sums[(2 * i * half + group.number) * width + t];
+        db[i / kNums][i % kNums] = db[i / kNums][i % kNums] + sums[((2 * i + 1) * half + group.number) * width + t];
       }
     }
-    __syncthreads();
+    there = half;
   }
-  if (group) return;
-  float* const out = workspace + static_cast<long long>(blockIdx.x) * 2 * n + t * kVec;
+  if (group.number) return;
+  float* const out = workspace + static_cast<long long>(blockIdx.x) * 2 * n + column;
 #pragma unroll
-  for (int i = 0; i < kSums; i++) {
-    const int c = i / kNums * step + i % kNums * 2;
-    if (kWhole || i / kNums * step < left) {
+  for (int i = 0; i < kVectors * kNums; i++) {
+    const int c = i / kNums * kStep + i % kNums * 2;
+    if (kWhole || i / kNums * kStep < left) {
       *reinterpret_cast<N*>(out + c) = dw[i / kNums][i % kNums];
       *reinterpret_cast<N*>(out + n + c) = db[i / kNums][i % kNums];  // (pairs: n is even)
     }
@@ -496,16 +508,34 @@ struct Alignment {
   int Vec(int n) const { return n % 8 == 0 && bits % 32 == 0 ? 8 : n % 2 == 0 && bits % 8 == 0 ? 2 : 1; }
 };
 
-// Threads of a row, or 0: too long to be held.
-int ThreadsOf(int n, int held) {
-  int threads = 1;
-  while (threads <= 512 && static_cast<long long>(threads) * held < n) threads *= 2;
-  return threads <= 512 ? threads : 0;
+// How rows of n values are held by groups of a block of up to `warps` warps, with `held` values per lane.
+struct Geometry {
+  int lanes = 0, warps = 0, groups = 0, blocks = 0;  // warps: of a group; lanes = 0: the rows are too long
+  bool whole = false;
+  Geometry(long long rows, int n, int held, int block_warps, int most_warps, int most_blocks) {
+    if (n > most_warps * 32 * held) return;
+    lanes = n <= 8 * held ? 8 : 32;
+    warps = lanes == 8 ? 1 : (n - 1) / (32 * held) + 1;
+    groups = lanes == 8 ? block_warps * 4 : block_warps / warps > 0 ? block_warps / warps : 1;
+    whole = lanes == 32 && n == warps * 32 * held;
+    const long long wanted = (rows + groups - 1) / groups;
+    blocks = static_cast<int>(wanted < most_blocks ? wanted : most_blocks);
+  }
+  int Threads() const { return lanes == 8 ? groups * 8 : groups * warps * 32; }
+};
+
+constexpr int kForwardWarps = 8;  // of a block, where a row does not need more
+
+Geometry BackwardGeometry(long long rows, int n, int held) {
+  const int warps = BackwardThreads(held) / 32;
+  return Geometry(rows, n, held, warps, warps, 148);
 }
 
-unsigned BackwardBlocks(long long rows, int threads) {
-  const long long groups = kBackwardThreads / threads, wanted = (rows + groups - 1) / groups;
-  return static_cast<unsigned>(wanted < 148 ? wanted : 148);
+template <class T, int kHeld> auto BackwardKernelOf(const Geometry& g, int vec) {
+  if (g.lanes == 8)
+    return vec == 1 ? BackwardKernel<T, 1, 8, false, kHeld> : vec == 2 ? BackwardKernel<T, 2, 8, false, kHeld> : BackwardKernel<T, 8, 8, false, kHeld>;
+  return vec == 1 ? BackwardKernel<T, 1, 32, false, kHeld> : vec == 2 ? BackwardKernel<T, 2, 32, false, kHeld>
+         : g.whole ? BackwardKernel<T, 8, 32, true, kHeld> : BackwardKernel<T, 8, 32, false, kHeld>;
 }
 
 template <class T>
@@ -515,15 +545,16 @@ int Forward(const void* x_in, const void* residual_in, Parameter weight, Paramet
   T *y = static_cast<T*>(y_in), *sum = static_cast<T*>(sum_in);
   Alignment at;
   at.Of(x), at.Of(residual), at.Of(weight), at.Of(bias), at.Of(y), at.Of(sum);
-  const int vec = at.Vec(n), held = ForwardHeld(vec, sizeof(T)), threads = ThreadsOf(n, held);
-  if (!threads)
+  const int vec = at.Vec(n);
+  const Geometry g(rows, n, ForwardHeld(vec, sizeof(T)), kForwardWarps, 16, 1 << 30);
+  if (!g.lanes)
     return Launched(LaunchOverlapped(ForwardAnyKernel<T>, RowBlocks(rows), kAnyThreads, 0, 1, stream, x, residual, weight, bias, y, sum,
                                      mean, rstd, rows, n, eps));
-  const int block = threads > kForwardThreads ? threads : kForwardThreads, groups = block / threads;
-  const auto kernel = vec == 1 ? ForwardKernel<T, 1, false> : vec == 2 ? ForwardKernel<T, 2, false>
-                      : n == threads * held ? ForwardKernel<T, 8, true> : ForwardKernel<T, 8, false>;
-  return Launched(LaunchOverlapped(kernel, RowBlocks((rows + groups - 1) / groups), block, 0, 1, stream, x, residual, weight, bias, y, sum, mean,
-                                   rstd, rows, n, eps, threads));
+  const auto kernel = g.lanes == 8 ? (vec == 1 ? ForwardKernel<T, 1, 8, false> : vec == 2 ? ForwardKernel<T, 2, 8, false> : ForwardKernel<T, 8, 8, false>)
+                      : vec == 1 ? ForwardKernel<T, 1, 32, false> : vec == 2 ? ForwardKernel<T, 2, 32, false>
+                      : g.whole ? ForwardKernel<T, 8, 32, true> : ForwardKernel<T, 8, 32, false>;
+  return Launched(LaunchOverlapped(kernel, g.blocks, g.Threads(), 0, 1, stream, x, residual, weight, bias, y, sum, mean, rstd, rows, n,
+                                   eps, g.groups, g.warps));
 }
 
 template <class T>
@@ -534,17 +565,21 @@ int Backward(const void* dy_in, const void* dsum_in, const void* s_in, Parameter
   if (!dweight && !dbias) workspace = nullptr;
   Alignment at;
   at.Of(dy), at.Of(dsum), at.Of(s), at.Of(weight), at.Of(dx);
-  const int vec = at.Vec(n), held = BackwardHeld(), threads = ThreadsOf(n, held);
+  const int vec = at.Vec(n);
+  const int held = BackwardHeld(n, vec, sizeof(T));
+  const Geometry g = BackwardGeometry(rows, n, held);
   int parts = 0;
   cudaError_t e;
-  if (threads) {
-    const auto kernel = vec == 1 ? BackwardKernel<T, 1, false> : vec == 2 ? BackwardKernel<T, 2, false>
-                        : n == threads * held ? BackwardKernel<T, 8, true> : BackwardKernel<T, 8, false>;
-    const int shared = kBackwardThreads / 2 * 2 * held * static_cast<int>(sizeof(float));
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
-    if (e != cudaSuccess) return Launched(e);
-    parts = static_cast<int>(BackwardBlocks(rows, threads));
-    e = LaunchOverlapped(kernel, parts, kBackwardThreads, shared, 1, stream, dy, dsum, s, weight, mean, rstd, dx, workspace, rows, n, threads);
+  if (g.lanes) {
+    const auto kernel = held == 16 ? BackwardKernelOf<T, 16>(g, vec) : BackwardKernelOf<T, 8>(g, vec);
+    const int shared = workspace && g.groups > 1 ? (g.groups + 1) / 2 * (g.Threads() / g.groups) * 2 * held * static_cast<int>(sizeof(float)) : 0;
+    if (shared > 32 << 10) {
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
+      if (e != cudaSuccess) return Launched(e);
+    }
+    parts = g.blocks;
+    e = LaunchOverlapped(kernel, parts, BackwardThreads(held), shared, 1, stream, dy, dsum, s, weight, mean, rstd, dx, workspace, rows, n,
+                         g.groups, g.warps);
   } else {
     e = LaunchOverlapped(BackwardAnyKernel<T>, RowBlocks(rows), kAnyThreads, 0, 1, stream, dy, dsum, s, weight, mean, rstd, dx, rows, n);
     if (e == cudaSuccess && workspace) {
@@ -572,8 +607,10 @@ extern "C" int switchml_layer_norm_forward(const void* x, const void* residual, 
 
 extern "C" long long switchml_layer_norm_workspace(long long rows, int features, int type) {
   if (rows <= 0 || features <= 0 || !Known(type)) return 0;
-  const int threads = ThreadsOf(features, BackwardHeld());
-  return 2ll * features * (threads ? static_cast<int>(BackwardBlocks(rows, threads)) : RowShares(rows, features));
+  // (Which it will be depends on the addresses too.)
+  const Geometry g = BackwardGeometry(rows, features, 8), h = BackwardGeometry(rows, features, 16);
+  const int held = g.blocks > h.blocks ? g.blocks : h.blocks;
+  return 2ll * features * (h.lanes ? held : RowShares(rows, features));
 }
 
 extern "C" int switchml_layer_norm_backward(const void* dy, const void* dsum, const void* s, const void* weight, const float* mean,
