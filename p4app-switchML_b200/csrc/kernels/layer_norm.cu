@@ -17,7 +17,6 @@
 
 using switchml::kernels::Fma;
 using switchml::kernels::LaunchOverlapped;
-using switchml::kernels::LetNextKernelStart;
 using switchml::kernels::LoadWords;
 using switchml::kernels::Pair;
 using switchml::kernels::StoreWords;
@@ -136,11 +135,17 @@ template <class T, int kVec> struct Vector {
   }
 };
 
-// kVec values of weight or bias, of either type.
-template <int kVec>
+// kVec values of weight or bias. W: their type where that is known (and both are there), else void. (To find out for every
+// vector which of three values it is costs as much as the rest of the forward pass.)
+template <int kVec, class W>
 __device__ __forceinline__ void LoadParameter(const Parameter& p, int i, float none, Num<kVec> (&out)[Vector<float, kVec>::kNums]) {
   constexpr int kNums = Vector<float, kVec>::kNums;
-  if (!p.data) {
+  if constexpr (!std::is_void_v<W>) {
+    Vector<W, kVec> v;
+    v.Load(static_cast<const W*>(p.data) + i);
+#pragma unroll
+    for (int k = 0; k < kNums; k++) out[k] = v.At(k);
+  } else if (!p.data) {
 #pragma unroll
     for (int k = 0; k < kNums; k++) out[k] = Num<kVec>(none);
   } else if (p.type == SML_NORM_F32) {
@@ -159,7 +164,7 @@ __device__ __forceinline__ void LoadParameter(const Parameter& p, int i, float n
 // Values that a thread holds. kWhole: the row is exactly what its threads hold, nothing has to be asked.
 __host__ __device__ constexpr int ForwardHeld(int vec, int size) { return vec == 8 && size == 2 ? 32 : 16; }
 
-template <class T, int kVec, int kLanes, bool kWhole>
+template <class T, int kVec, int kLanes, bool kWhole, class W>
 __global__ void __launch_bounds__(512, 2)
 ForwardKernel(const T* x, const T* residual, Parameter weight, Parameter bias, T* y, T* sum, float* mean_out, float* rstd_out,
               long long rows, int n, float eps, int groups, int warps) {
@@ -214,8 +219,8 @@ ForwardKernel(const T* x, const T* residual, Parameter weight, Parameter bias, T
     for (int j = 0; j < kVectors; j++) {
       if (kWhole || j * kStep < left) {
         N w[kNums], b[kNums];
-        LoadParameter<kVec>(weight, column + j * kStep, 1.f, w);
-        LoadParameter<kVec>(bias, column + j * kStep, 0.f, b);
+        LoadParameter<kVec, W>(weight, column + j * kStep, 1.f, w);
+        LoadParameter<kVec, W>(bias, column + j * kStep, 0.f, b);
         Vector<T, kVec> out;
 #pragma unroll
         for (int i = 0; i < kNums; i++) out.Set(i, Fma(s[j][i] * N(rstd), w[i], b[i]));
@@ -233,7 +238,7 @@ ForwardKernel(const T* x, const T* residual, Parameter weight, Parameter bias, T
 __host__ __device__ constexpr int BackwardThreads(int held) { return held == 16 ? 512 : 768; }
 int BackwardHeld(int n, int vec, int size) { return (vec == 8 && size == 2) || n > BackwardThreads(8) / 32 * 32 * 8 ? 16 : 8; }
 
-template <class T, int kVec, int kLanes, bool kWhole, int kHeld>
+template <class T, int kVec, int kLanes, bool kWhole, int kHeld, class W>
 __global__ void __launch_bounds__(BackwardThreads(kHeld), 1)
 BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const float* mean_in, const float* rstd_in, T* dx,
                float* workspace, long long rows, int n, int groups, int warps) {
@@ -243,7 +248,7 @@ BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const f
   __shared__ float2 part[2][BackwardThreads(kHeld) / 32];
   const Group<kLanes> group(warps);
   const int column = group.First(kHeld, kVec), left = n - column;
-  const long long stride = static_cast<long long>(gridDim.x) * groups;
+  const long long stride = static_cast<long long>(gridDim.x) * groups;  // (of rows)
   // The weight stays in registers where these suffice, else it comes from L1 for every row.
   constexpr bool kKeepWeight = sizeof(T) == 2 && kVec > 1;
   N w[kVectors][kNums], dw[kVectors][kNums], db[kVectors][kNums];
@@ -267,7 +272,7 @@ BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const f
   if constexpr (kKeepWeight) {
 #pragma unroll
     for (int j = 0; j < kVectors; j++) {
-      if (kWhole || j * kStep < left) LoadParameter<kVec>(weight, column + j * kStep, 1.f, w[j]);
+      if (kWhole || j * kStep < left) LoadParameter<kVec, W>(weight, column + j * kStep, 1.f, w[j]);
     }
   }
   // (Groups that do not fit into the block any more have no row.)
@@ -281,7 +286,7 @@ BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const f
 #pragma unroll
     for (int j = 0; j < kVectors; j++) {
       if constexpr (!kKeepWeight) {
-        if (kWhole || j * kStep < left) LoadParameter<kVec>(weight, column + j * kStep, 1.f, w[j]);
+        if (kWhole || j * kStep < left) LoadParameter<kVec, W>(weight, column + j * kStep, 1.f, w[j]);
       }
 #pragma unroll
       for (int i = 0; i < kNums; i++) {  // (what is not there has gradients of 0)
@@ -303,17 +308,17 @@ BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const f
     const float2 c12 = group.Sum(make_float2(Sum(c1), Sum(c2)), part[turn]);
     turn ^= 1;
     const N minus_c1(-c12.x / n), minus_c2(-c12.y / n);
+    const auto store = [&](auto plus) {
 #pragma unroll
-    for (int j = 0; j < kVectors; j++) {
-      Vector<T, kVec> out;
+      for (int j = 0; j < kVectors; j++) {
+        Vector<T, kVec> out;
 #pragma unroll
-      for (int i = 0; i < kNums; i++) {
-        N e = Fma(xhat[j][i], minus_c2, g[j][i] + minus_c1) * N(r);
-        if (dsum) e = e + more[j].At(i);
-        out.Set(i, e);
+        for (int i = 0; i < kNums; i++) out.Set(i, plus(Fma(xhat[j][i], minus_c2, g[j][i] + minus_c1) * N(r), j, i));
+        if (kWhole || j * kStep < left) out.Store(dx + at + j * kStep);
       }
-      if (kWhole || j * kStep < left) out.Store(dx + at + j * kStep);
-    }
+    };
+    if (dsum) store([&](N e, int j, int i) { return e + more[j].At(i); });
+    else store([](N e, int, int) { return e; });
   }
   if (!workspace) return;
   // The upper half of the groups gives its sums to the lower one until one has all.
@@ -531,11 +536,30 @@ Geometry BackwardGeometry(long long rows, int n, int held) {
   return Geometry(rows, n, held, warps, warps, 148);
 }
 
-template <class T, int kHeld> auto BackwardKernelOf(const Geometry& g, int vec) {
+// The type of weight and bias, for kernels that want to know it.
+enum class Kind { kF32, kBf16, kNo };
+template <class T> Kind TypeOf(const Parameter& a, const Parameter& b) {
+  if (!a.data || !b.data || (sizeof(T) == 4 && a.type != SML_NORM_F32)) return Kind::kNo;
+  return a.type == SML_NORM_F32 ? Kind::kF32 : Kind::kBf16;
+}
+
+template <class T, int kHeld> auto BackwardKernelOf(const Geometry& g, int vec, Kind type) {
   if (g.lanes == 8)
-    return vec == 1 ? BackwardKernel<T, 1, 8, false, kHeld> : vec == 2 ? BackwardKernel<T, 2, 8, false, kHeld> : BackwardKernel<T, 8, 8, false, kHeld>;
-  return vec == 1 ? BackwardKernel<T, 1, 32, false, kHeld> : vec == 2 ? BackwardKernel<T, 2, 32, false, kHeld>
-         : g.whole ? BackwardKernel<T, 8, 32, true, kHeld> : BackwardKernel<T, 8, 32, false, kHeld>;
+    return vec == 1 ? BackwardKernel<T, 1, 8, false, kHeld, void> : vec == 2 ? BackwardKernel<T, 2, 8, false, kHeld, void>
+           : BackwardKernel<T, 8, 8, false, kHeld, void>;
+  if (vec < 8) return vec == 1 ? BackwardKernel<T, 1, 32, false, kHeld, void> : BackwardKernel<T, 2, 32, false, kHeld, void>;
+  if (!g.whole) return type == Kind::kF32 ? BackwardKernel<T, 8, 32, false, kHeld, float> : BackwardKernel<T, 8, 32, false, kHeld, void>;
+  return type == Kind::kF32 ? BackwardKernel<T, 8, 32, true, kHeld, float> : type == Kind::kBf16 ? BackwardKernel<T, 8, 32, true, kHeld, T>
+         : BackwardKernel<T, 8, 32, true, kHeld, void>;
+}
+template <class T> auto ForwardKernelOf(const Geometry& g, int vec, Kind type) {
+  if (g.lanes == 8)
+    return vec == 1 ? ForwardKernel<T, 1, 8, false, void> : vec == 2 ? ForwardKernel<T, 2, 8, false, void>
+           : type == Kind::kF32 ? ForwardKernel<T, 8, 8, false, float> : ForwardKernel<T, 8, 8, false, void>;
+  if (vec < 8) return vec == 1 ? ForwardKernel<T, 1, 32, false, void> : ForwardKernel<T, 2, 32, false, void>;
+  if (!g.whole) return type == Kind::kF32 ? ForwardKernel<T, 8, 32, false, float> : ForwardKernel<T, 8, 32, false, void>;
+  return type == Kind::kF32 ? ForwardKernel<T, 8, 32, true, float> : type == Kind::kBf16 ? ForwardKernel<T, 8, 32, true, T>
+         : ForwardKernel<T, 8, 32, true, void>;
 }
 
 template <class T>
@@ -550,10 +574,7 @@ int Forward(const void* x_in, const void* residual_in, Parameter weight, Paramet
   if (!g.lanes)
     return Launched(LaunchOverlapped(ForwardAnyKernel<T>, RowBlocks(rows), kAnyThreads, 0, 1, stream, x, residual, weight, bias, y, sum,
                                      mean, rstd, rows, n, eps));
-  const auto kernel = g.lanes == 8 ? (vec == 1 ? ForwardKernel<T, 1, 8, false> : vec == 2 ? ForwardKernel<T, 2, 8, false> : ForwardKernel<T, 8, 8, false>)
-                      : vec == 1 ? ForwardKernel<T, 1, 32, false> : vec == 2 ? ForwardKernel<T, 2, 32, false>
-                      : g.whole ? ForwardKernel<T, 8, 32, true> : ForwardKernel<T, 8, 32, false>;
-  return Launched(LaunchOverlapped(kernel, g.blocks, g.Threads(), 0, 1, stream, x, residual, weight, bias, y, sum, mean, rstd, rows, n,
+  return Launched(LaunchOverlapped(ForwardKernelOf<T>(g, vec, TypeOf<T>(weight, bias)), g.blocks, g.Threads(), 0, 1, stream, x, residual, weight, bias, y, sum, mean, rstd, rows, n,
                                    eps, g.groups, g.warps));
 }
 
@@ -571,7 +592,7 @@ int Backward(const void* dy_in, const void* dsum_in, const void* s_in, Parameter
   int parts = 0;
   cudaError_t e;
   if (g.lanes) {
-    const auto kernel = held == 16 ? BackwardKernelOf<T, 16>(g, vec) : BackwardKernelOf<T, 8>(g, vec);
+    const auto kernel = held == 16 ? BackwardKernelOf<T, 16>(g, vec, TypeOf<T>(weight, weight)) : BackwardKernelOf<T, 8>(g, vec, TypeOf<T>(weight, weight));
     const int shared = workspace && g.groups > 1 ? (g.groups + 1) / 2 * (g.Threads() / g.groups) * 2 * held * static_cast<int>(sizeof(float)) : 0;
     if (shared > 32 << 10) {
       e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
