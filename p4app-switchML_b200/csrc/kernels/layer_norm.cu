@@ -58,7 +58,7 @@ __device__ __forceinline__ float WarpSum(float v) {
 //
 // A group of threads holds a row: 8 lanes of a warp, or 1 to 24 whole warps. Each lane has kHeld values: kHeld / kVec
 // vectors of kVec neighbours, between which lie kLanes (8 or 32) * kVec values, so that addresses differ by constants; warp w
-// has the values from w * 32 * kHeld on. kVec is what the addresses and the length of the rows allow: 8, 2 or 1.
+// has the values from w * 32 * kHeld on. kVec is what the addresses and the length of the rows allow: 16 bytes of them, 2 or 1.
 // Groups go through their rows by themselves, and warps of a group meet at a barrier of their own.
 
 template <int kLanes> struct Group {
@@ -95,6 +95,9 @@ template <int kLanes> struct Group {
   static __device__ __forceinline__ float2 Plus(float2 a, float2 b) { return make_float2(a.x + b.x, a.y + b.y); }
 };
 
+// Values of 16 bytes: what a thread reads at once where addresses and the length of the rows allow it.
+template <class T> constexpr int kWide = 16 / sizeof(T);
+
 // What arithmetic takes at once of a vector's values: two of them, where there are two.
 template <int kVec> using Num = std::conditional_t<kVec == 1, float, Pair>;
 
@@ -110,6 +113,10 @@ template <class T, int kVec> struct Vector {
   __device__ __forceinline__ void Store(T* to) const {
     if constexpr (kWords) StoreWords(to, w);
     else *reinterpret_cast<unsigned short*>(to) = static_cast<unsigned short>(w[0]);
+  }
+  __device__ __forceinline__ void LoadShared(const uint4* from) {  // 16 bytes
+    const uint4 v = *from;
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
   }
   __device__ __forceinline__ void LoadIf(bool there, const T* from) {
     if constexpr (kWords) switchml::kernels::LoadWordsIf(there, from, w);
@@ -162,7 +169,7 @@ __device__ __forceinline__ void LoadParameter(const Parameter& p, int i, float n
 }
 
 // Values that a thread holds. kWhole: the row is exactly what its threads hold, nothing has to be asked.
-__host__ __device__ constexpr int ForwardHeld(int vec, int size) { return vec == 8 && size == 2 ? 32 : 16; }
+__host__ __device__ constexpr int ForwardHeld(int vec, int size) { return vec == 8 ? 32 : 16; }
 
 template <class T, int kVec, int kLanes, bool kWhole, class W>
 __global__ void __launch_bounds__(512, 2)
@@ -236,7 +243,21 @@ ForwardKernel(const T* x, const T* residual, Parameter weight, Parameter bias, T
 // Sums, normalised values, gradients and what is read ahead take 6 to 8 registers per value: 16 bf16 values in vectors fit
 // the 128 registers of 16 warps, of the others 8 fit the 85 of 24 warps. (16 of those, for rows that need them, spill.)
 __host__ __device__ constexpr int BackwardThreads(int held) { return held == 16 ? 512 : 768; }
-int BackwardHeld(int n, int vec, int size) { return (vec == 8 && size == 2) || n > BackwardThreads(8) / 32 * 32 * 8 ? 16 : 8; }
+int BackwardHeld(int n, int vec) { return (vec == 8 && n > 256) || n > BackwardThreads(8) * 8 ? 16 : 8; }
+
+// Rows that a thread reads ahead, in vectors: through shared memory, where it alone reads what it has copied itself, so that
+// nothing has to be waited for but its own copies. (Registers hold one row: 8192 x 1024 fp32 25.4 us with those.)
+__host__ __device__ constexpr int BackwardRowBytes(int held, int size) { return 3 * held * size * BackwardThreads(held); }  // of dy, s and dsum
+__host__ __device__ constexpr int BackwardStages(int vec, int held, int size) {
+  return vec * size < 16 ? 0 : 216 * 1024 / BackwardRowBytes(held, size) < 4 ? 216 * 1024 / BackwardRowBytes(held, size) : 4;
+}
+
+__device__ __forceinline__ void CopyAsync(uint4* to, const void* from, bool there) {  // zeros where nothing is there
+  const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void CommitCopies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft> __device__ __forceinline__ void WaitForCopies() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
 
 template <class T, int kVec, int kLanes, bool kWhole, int kHeld, class W>
 __global__ void __launch_bounds__(BackwardThreads(kHeld), 1)
@@ -257,7 +278,7 @@ BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const f
 #pragma unroll
     for (int i = 0; i < kNums; i++) w[j][i] = dw[j][i] = db[j][i] = N(0.f);
   }
-  Vector<T, kVec> d[kVectors], v[kVectors];
+  Vector<T, kVec> d[kVectors], v[kVectors], more[kVectors];
   float mean = 0.f, rstd = 0.f;
   const auto load = [&](long long row) {
     const long long at = row * n + column;
@@ -266,7 +287,24 @@ BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const f
       d[j].LoadIf(kWhole || j * kStep < left, dy + at + j * kStep);
       v[j].LoadIf(kWhole || j * kStep < left, s + at + j * kStep);
     }
-    mean = mean_in[row], rstd = rstd_in[row];
+  };
+  // The ring: kStages rows of kVectors vectors of dy, s and, if there is one, dsum for every thread.
+  constexpr int kStages = BackwardStages(kVec, kHeld, sizeof(T)), kThreads = BackwardThreads(kHeld);
+  uint4* const ring = reinterpret_cast<uint4*>(shared) + threadIdx.x;
+  const auto copy = [&](long long row, int stage) {
+    if (row < rows) {
+      const long long at = row * n + column;
+      uint4* const to = ring + stage * 3 * kVectors * kThreads;
+#pragma unroll
+      for (int j = 0; j < kVectors; j++) {
+        const bool there = kWhole || j * kStep < left;
+        const long long from = there ? at + j * kStep : 0;
+        CopyAsync(to + j * kThreads, dy + from, there);
+        CopyAsync(to + (kVectors + j) * kThreads, s + from, there);
+        if (dsum) CopyAsync(to + (2 * kVectors + j) * kThreads, dsum + from, there);
+      }
+    }
+    CommitCopies();
   };
   WaitForEarlierKernels();
   if constexpr (kKeepWeight) {
@@ -277,11 +315,27 @@ BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const f
   }
   // (Groups that do not fit into the block any more have no row.)
   long long row = group.number < groups ? static_cast<long long>(blockIdx.x) * groups + group.number : rows;
-  if (row < rows) load(row);
-  int turn = 0;
+  if constexpr (kStages > 0) {
+#pragma unroll
+    for (int i = 0; i < kStages - 1; i++) copy(row + i * stride, i);
+  } else if (row < rows) {
+    load(row);
+  }
+  if (row < rows) mean = mean_in[row], rstd = rstd_in[row];
+  int turn = 0, stage = 0;
   for (; row < rows; row += stride) {
     const long long at = row * n + column;
     const float r = rstd;
+    if constexpr (kStages > 0) {
+      copy(row + (kStages - 1) * stride, stage ? stage - 1 : kStages - 1);
+      WaitForCopies<kStages - 1>();
+      const uint4* const from = ring + stage * 3 * kVectors * kThreads;
+#pragma unroll
+      for (int j = 0; j < kVectors; j++) {
+        d[j].LoadShared(from + j * kThreads);
+        v[j].LoadShared(from + (kVectors + j) * kThreads);
+      }
+    }
     N c1(0.f), c2(0.f), xhat[kVectors][kNums], g[kVectors][kNums];
 #pragma unroll
     for (int j = 0; j < kVectors; j++) {
@@ -299,12 +353,14 @@ BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const f
         db[j][i] = db[j][i] + dyi;
       }
     }
-    Vector<T, kVec> more[kVectors];
-    if (dsum) {
+    if constexpr (kStages == 0) {
+      if (dsum) {
 #pragma unroll
-      for (int j = 0; j < kVectors; j++) more[j].LoadIf(kWhole || j * kStep < left, dsum + at + j * kStep);
+        for (int j = 0; j < kVectors; j++) more[j].LoadIf(kWhole || j * kStep < left, dsum + at + j * kStep);
+      }
+      if (row + stride < rows) load(row + stride);
     }
-    if (row + stride < rows) load(row + stride);
+    if (row + stride < rows) mean = mean_in[row + stride], rstd = rstd_in[row + stride];
     const float2 c12 = group.Sum(make_float2(Sum(c1), Sum(c2)), part[turn]);
     turn ^= 1;
     const N minus_c1(-c12.x / n), minus_c2(-c12.y / n);
@@ -317,11 +373,20 @@ BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const f
         if (kWhole || j * kStep < left) out.Store(dx + at + j * kStep);
       }
     };
-    if (dsum) store([&](N e, int j, int i) { return e + more[j].At(i); });
-    else store([](N e, int, int) { return e; });
+    if (dsum) {
+      if constexpr (kStages > 0) {
+#pragma unroll
+        for (int j = 0; j < kVectors; j++) more[j].LoadShared(ring + (stage * 3 * kVectors + 2 * kVectors + j) * kThreads);
+      }
+      store([&](N e, int j, int i) { return e + more[j].At(i); });
+    } else {
+      store([](N e, int, int) { return e; });
+    }
+    stage = stage + 1 < kStages ? stage + 1 : 0;
   }
   if (!workspace) return;
-  // The upper half of the groups gives its sums to the lower one until one has all.
+  // The upper half of the groups gives its sums to the lower one until one has all. (In the ring's place, after a barrier: no
+  // thread has copies under way that are for rows, and what it has of empty ones counts for nothing.)
   N* const sums = reinterpret_cast<N*>(shared);
   const int width = kLanes == 32 ? warps * 32 : kLanes, t = kLanes == 32 ? group.warp * 32 + group.lane : group.lane;
   for (int there = groups; there > 1;) {
@@ -510,7 +575,7 @@ struct Alignment {
   uintptr_t bits = 0;
   template <class T> void Of(const T* tensor) { bits |= reinterpret_cast<uintptr_t>(tensor) * (4 / sizeof(T)); }  // as if it were fp32
   void Of(const Parameter& p) { bits |= reinterpret_cast<uintptr_t>(p.data) * (p.type == SML_NORM_F32 ? 1 : 2); }
-  int Vec(int n) const { return n % 8 == 0 && bits % 32 == 0 ? 8 : n % 2 == 0 && bits % 8 == 0 ? 2 : 1; }
+  int Vec(int n, int wide) const { return n % wide == 0 && bits % (4 * wide) == 0 ? wide : n % 2 == 0 && bits % 8 == 0 ? 2 : 1; }
 };
 
 // How rows of n values are held by groups of a block of up to `warps` warps, with `held` values per lane.
@@ -546,20 +611,20 @@ template <class T> Kind TypeOf(const Parameter& a, const Parameter& b) {
 template <class T, int kHeld> auto BackwardKernelOf(const Geometry& g, int vec, Kind type) {
   if (g.lanes == 8)
     return vec == 1 ? BackwardKernel<T, 1, 8, false, kHeld, void> : vec == 2 ? BackwardKernel<T, 2, 8, false, kHeld, void>
-           : BackwardKernel<T, 8, 8, false, kHeld, void>;
-  if (vec < 8) return vec == 1 ? BackwardKernel<T, 1, 32, false, kHeld, void> : BackwardKernel<T, 2, 32, false, kHeld, void>;
-  if (!g.whole) return type == Kind::kF32 ? BackwardKernel<T, 8, 32, false, kHeld, float> : BackwardKernel<T, 8, 32, false, kHeld, void>;
-  return type == Kind::kF32 ? BackwardKernel<T, 8, 32, true, kHeld, float> : type == Kind::kBf16 ? BackwardKernel<T, 8, 32, true, kHeld, T>
-         : BackwardKernel<T, 8, 32, true, kHeld, void>;
+           : BackwardKernel<T, kWide<T>, 8, false, kHeld, void>;
+  if (vec <= 2) return vec == 1 ? BackwardKernel<T, 1, 32, false, kHeld, void> : BackwardKernel<T, 2, 32, false, kHeld, void>;
+  if (!g.whole) return type == Kind::kF32 ? BackwardKernel<T, kWide<T>, 32, false, kHeld, float> : BackwardKernel<T, kWide<T>, 32, false, kHeld, void>;
+  return type == Kind::kF32 ? BackwardKernel<T, kWide<T>, 32, true, kHeld, float> : type == Kind::kBf16 ? BackwardKernel<T, kWide<T>, 32, true, kHeld, T>
+         : BackwardKernel<T, kWide<T>, 32, true, kHeld, void>;
 }
 template <class T> auto ForwardKernelOf(const Geometry& g, int vec, Kind type) {
   if (g.lanes == 8)
     return vec == 1 ? ForwardKernel<T, 1, 8, false, void> : vec == 2 ? ForwardKernel<T, 2, 8, false, void>
-           : type == Kind::kF32 ? ForwardKernel<T, 8, 8, false, float> : ForwardKernel<T, 8, 8, false, void>;
-  if (vec < 8) return vec == 1 ? ForwardKernel<T, 1, 32, false, void> : ForwardKernel<T, 2, 32, false, void>;
-  if (!g.whole) return type == Kind::kF32 ? ForwardKernel<T, 8, 32, false, float> : ForwardKernel<T, 8, 32, false, void>;
-  return type == Kind::kF32 ? ForwardKernel<T, 8, 32, true, float> : type == Kind::kBf16 ? ForwardKernel<T, 8, 32, true, T>
-         : ForwardKernel<T, 8, 32, true, void>;
+           : type == Kind::kF32 ? ForwardKernel<T, kWide<T>, 8, false, float> : ForwardKernel<T, kWide<T>, 8, false, void>;
+  if (vec <= 2) return vec == 1 ? ForwardKernel<T, 1, 32, false, void> : ForwardKernel<T, 2, 32, false, void>;
+  if (!g.whole) return type == Kind::kF32 ? ForwardKernel<T, kWide<T>, 32, false, float> : ForwardKernel<T, kWide<T>, 32, false, void>;
+  return type == Kind::kF32 ? ForwardKernel<T, kWide<T>, 32, true, float> : type == Kind::kBf16 ? ForwardKernel<T, kWide<T>, 32, true, T>
+         : ForwardKernel<T, kWide<T>, 32, true, void>;
 }
 
 template <class T>
@@ -569,7 +634,7 @@ int Forward(const void* x_in, const void* residual_in, Parameter weight, Paramet
   T *y = static_cast<T*>(y_in), *sum = static_cast<T*>(sum_in);
   Alignment at;
   at.Of(x), at.Of(residual), at.Of(weight), at.Of(bias), at.Of(y), at.Of(sum);
-  const int vec = at.Vec(n);
+  const int vec = at.Vec(n, kWide<T>);
   const Geometry g(rows, n, ForwardHeld(vec, sizeof(T)), kForwardWarps, 16, 1 << 30);
   if (!g.lanes)
     return Launched(LaunchOverlapped(ForwardAnyKernel<T>, RowBlocks(rows), kAnyThreads, 0, 1, stream, x, residual, weight, bias, y, sum,
@@ -586,14 +651,16 @@ int Backward(const void* dy_in, const void* dsum_in, const void* s_in, Parameter
   if (!dweight && !dbias) workspace = nullptr;
   Alignment at;
   at.Of(dy), at.Of(dsum), at.Of(s), at.Of(weight), at.Of(dx);
-  const int vec = at.Vec(n);
-  const int held = BackwardHeld(n, vec, sizeof(T));
+  const int vec = at.Vec(n, kWide<T>);
+  const int held = BackwardHeld(n, vec);
   const Geometry g = BackwardGeometry(rows, n, held);
   int parts = 0;
   cudaError_t e;
   if (g.lanes) {
     const auto kernel = held == 16 ? BackwardKernelOf<T, 16>(g, vec, TypeOf<T>(weight, weight)) : BackwardKernelOf<T, 8>(g, vec, TypeOf<T>(weight, weight));
-    const int shared = workspace && g.groups > 1 ? (g.groups + 1) / 2 * (g.Threads() / g.groups) * 2 * held * static_cast<int>(sizeof(float)) : 0;
+    const int ring = BackwardStages(vec, held, sizeof(T)) * BackwardRowBytes(held, sizeof(T));
+    const int ends = workspace && g.groups > 1 ? (g.groups + 1) / 2 * (g.Threads() / g.groups) * 2 * held * static_cast<int>(sizeof(float)) : 0;
+    const int shared = ring > ends ? ring : ends;
     if (shared > 32 << 10) {
       e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
       if (e != cudaSuccess) return Launched(e);
