@@ -17,6 +17,7 @@
 
 using switchml::kernels::Fma;
 using switchml::kernels::LaunchOverlapped;
+using switchml::kernels::LetNextKernelStart;
 using switchml::kernels::LoadWords;
 using switchml::kernels::Pair;
 using switchml::kernels::StoreWords;
@@ -120,7 +121,8 @@ template <class T, int kVec> struct Vector {
   }
   __device__ __forceinline__ void LoadIf(bool there, const T* from) {
     if constexpr (kWords) switchml::kernels::LoadWordsIf(there, from, w);
-    else w[0] = there ? *reinterpret_cast<const unsigned short*>(from) : 0;
+    else asm volatile("{.reg .pred p; .reg .b16 h; mov.b16 h, 0; setp.ne.b32 p, %2, 0; @p ld.global.b16 h, [%1]; cvt.u32.u16 %0, h;}"
+                      : "=r"(w[0]) : "l"(from), "r"(static_cast<int>(there)));
   }
   __device__ __forceinline__ Num<kVec> At(int i) const {
     if constexpr (kVec == 1) return __uint_as_float(sizeof(T) == 4 ? w[0] : w[0] << 16);
@@ -385,6 +387,7 @@ BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const f
     stage = stage + 1 < kStages ? stage + 1 : 0;
   }
   if (!workspace) return;
+  LetNextKernelStart();  // (what finishes the sums)
   // The upper half of the groups gives its sums to the lower one until one has all. (In the ring's place, after a barrier: no
   // thread has copies under way that are for rows, and what it has of empty ones counts for nothing.)
   N* const sums = reinterpret_cast<N*>(shared);
@@ -526,36 +529,41 @@ ColumnsAnyKernel(const T* dy, const T* s, const float* mean, const float* rstd, 
   }
 }
 
-constexpr int kFinishColumns = 32, kFinishRows = 32;
+// The sums of `parts` partial sums, in a fixed order. A block takes 8 columns (a 32-byte sector of each part), a warp 4 parts at
+// a time: with 148 parts every thread has all its loads in flight at once.
+constexpr int kFinishColumns = 8, kFinishThreads = 256, kFinishParts = kFinishThreads / kFinishColumns;
 
-// The sums of `parts` partial sums, in order.
-__global__ void __launch_bounds__(kFinishColumns* kFinishRows)
+__global__ void __launch_bounds__(kFinishThreads)
 FinishColumnsKernel(const float* workspace, void* dweight, void* dbias, int parts, int n, int wtype) {
-  __shared__ float2 part[kFinishRows][kFinishColumns];
-  const int lane = threadIdx.x % kFinishColumns, r = threadIdx.x / kFinishColumns, column = blockIdx.x * kFinishColumns + lane;
+  __shared__ float2 part[kFinishThreads / 32][kFinishColumns];
+  const int c = threadIdx.x % kFinishColumns, column = blockIdx.x * kFinishColumns + c;
   float2 sum = make_float2(0.f, 0.f);
   WaitForEarlierKernels();
   if (column < n) {
 #pragma unroll 5
-    for (int p = r; p < parts; p += kFinishRows) {
+    for (int p = threadIdx.x / kFinishColumns; p < parts; p += kFinishParts) {
       const float* from = workspace + static_cast<long long>(p) * 2 * n;
       sum.x += from[column];
       sum.y += from[n + column];
     }
   }
-  part[r][lane] = sum;
-  __syncthreads();
-  if (r == 0 && column < n) {
-    sum = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < kFinishRows; i++) sum.x += part[i][lane].x, sum.y += part[i][lane].y;
-    if (wtype == SML_NORM_F32) {
-      if (dweight) static_cast<float*>(dweight)[column] = sum.x;
-      if (dbias) static_cast<float*>(dbias)[column] = sum.y;
-    } else {
-      if (dweight) static_cast<__nv_bfloat16*>(dweight)[column] = __float2bfloat16_rn(sum.x);
-      if (dbias) static_cast<__nv_bfloat16*>(dbias)[column] = __float2bfloat16_rn(sum.y);
-    }
+  for (int o = kFinishColumns; o < 32; o *= 2) {
+    sum.x += __shfl_xor_sync(0xffffffffu, sum.x, o);
+    sum.y += __shfl_xor_sync(0xffffffffu, sum.y, o);
+  }
+  if (threadIdx.x % 32 < kFinishColumns) part[threadIdx.x / 32][c] = sum;
+  __syncthreads();
+  if (threadIdx.x >= kFinishColumns || column >= n) return;
+  sum = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < kFinishThreads / 32; i++) sum.x += part[i][c].x, sum.y += part[i][c].y;
+  if (wtype == SML_NORM_F32) {
+    if (dweight) static_cast<float*>(dweight)[column] = sum.x;
+    if (dbias) static_cast<float*>(dbias)[column] = sum.y;
+  } else {
+    if (dweight) static_cast<__nv_bfloat16*>(dweight)[column] = __float2bfloat16_rn(sum.x);
+    if (dbias) static_cast<__nv_bfloat16*>(dbias)[column] = __float2bfloat16_rn(sum.y);
   }
 }
 
@@ -586,6 +594,7 @@ struct Geometry {
     if (n > most_warps * 32 * held) return;
     lanes = n <= 8 * held ? 8 : 32;
     warps = lanes == 8 ? 1 : (n - 1) / (32 * held) + 1;
+    if (block_warps % warps && block_warps < 16) block_warps = 16;  // (a block reserves all barriers: 4 of them to an SM)
     groups = lanes == 8 ? block_warps * 4 : block_warps / warps > 0 ? block_warps / warps : 1;
     whole = lanes == 32 && n == warps * 32 * held;
     const long long wanted = (rows + groups - 1) / groups;
@@ -608,23 +617,28 @@ template <class T> Kind TypeOf(const Parameter& a, const Parameter& b) {
   return a.type == SML_NORM_F32 ? Kind::kF32 : Kind::kBf16;
 }
 
+template <class T, int kVec, int kLanes, int kHeld> auto BackwardKernelOf(Kind type) {
+  return type == Kind::kF32 ? BackwardKernel<T, kVec, kLanes, false, kHeld, float> : BackwardKernel<T, kVec, kLanes, false, kHeld, void>;
+}
 template <class T, int kHeld> auto BackwardKernelOf(const Geometry& g, int vec, Kind type) {
   if (g.lanes == 8)
-    return vec == 1 ? BackwardKernel<T, 1, 8, false, kHeld, void> : vec == 2 ? BackwardKernel<T, 2, 8, false, kHeld, void>
-           : BackwardKernel<T, kWide<T>, 8, false, kHeld, void>;
-  if (vec <= 2) return vec == 1 ? BackwardKernel<T, 1, 32, false, kHeld, void> : BackwardKernel<T, 2, 32, false, kHeld, void>;
-  if (!g.whole) return type == Kind::kF32 ? BackwardKernel<T, kWide<T>, 32, false, kHeld, float> : BackwardKernel<T, kWide<T>, 32, false, kHeld, void>;
-  return type == Kind::kF32 ? BackwardKernel<T, kWide<T>, 32, true, kHeld, float> : type == Kind::kBf16 ? BackwardKernel<T, kWide<T>, 32, true, kHeld, T>
-         : BackwardKernel<T, kWide<T>, 32, true, kHeld, void>;
+    return vec == 1 ? BackwardKernelOf<T, 1, 8, kHeld>(type) : vec == 2 ? BackwardKernelOf<T, 2, 8, kHeld>(type)
+           : BackwardKernelOf<T, kWide<T>, 8, kHeld>(type);
+  if (vec <= 2) return vec == 1 ? BackwardKernelOf<T, 1, 32, kHeld>(type) : BackwardKernelOf<T, 2, 32, kHeld>(type);
+  if (!g.whole) return BackwardKernelOf<T, kWide<T>, 32, kHeld>(type);
+  return type == Kind::kF32 ? BackwardKernel<T, kWide<T>, 32, true, kHeld, float>
+         : type == Kind::kBf16 ? BackwardKernel<T, kWide<T>, 32, true, kHeld, T> : BackwardKernel<T, kWide<T>, 32, true, kHeld, void>;
+}
+template <class T, int kVec, int kLanes> auto ForwardKernelOf(Kind type) {
+  return type == Kind::kF32 ? ForwardKernel<T, kVec, kLanes, false, float> : ForwardKernel<T, kVec, kLanes, false, void>;
 }
 template <class T> auto ForwardKernelOf(const Geometry& g, int vec, Kind type) {
   if (g.lanes == 8)
-    return vec == 1 ? ForwardKernel<T, 1, 8, false, void> : vec == 2 ? ForwardKernel<T, 2, 8, false, void>
-           : type == Kind::kF32 ? ForwardKernel<T, kWide<T>, 8, false, float> : ForwardKernel<T, kWide<T>, 8, false, void>;
-  if (vec <= 2) return vec == 1 ? ForwardKernel<T, 1, 32, false, void> : ForwardKernel<T, 2, 32, false, void>;
-  if (!g.whole) return type == Kind::kF32 ? ForwardKernel<T, kWide<T>, 32, false, float> : ForwardKernel<T, kWide<T>, 32, false, void>;
-  return type == Kind::kF32 ? ForwardKernel<T, kWide<T>, 32, true, float> : type == Kind::kBf16 ? ForwardKernel<T, kWide<T>, 32, true, T>
-         : ForwardKernel<T, kWide<T>, 32, true, void>;
+    return vec == 1 ? ForwardKernelOf<T, 1, 8>(type) : vec == 2 ? ForwardKernelOf<T, 2, 8>(type) : ForwardKernelOf<T, kWide<T>, 8>(type);
+  if (vec <= 2) return vec == 1 ? ForwardKernelOf<T, 1, 32>(type) : ForwardKernelOf<T, 2, 32>(type);
+  if (!g.whole) return ForwardKernelOf<T, kWide<T>, 32>(type);
+  return type == Kind::kF32 ? ForwardKernel<T, kWide<T>, 32, true, float>
+         : type == Kind::kBf16 ? ForwardKernel<T, kWide<T>, 32, true, T> : ForwardKernel<T, kWide<T>, 32, true, void>;
 }
 
 template <class T>
@@ -678,7 +692,7 @@ int Backward(const void* dy_in, const void* dsum_in, const void* s_in, Parameter
     }
   }
   if (e != cudaSuccess || !workspace) return Launched(e);
-  return Launched(LaunchOverlapped(FinishColumnsKernel, (n - 1) / kFinishColumns + 1, kFinishColumns * kFinishRows, 0, 1, stream,
+  return Launched(LaunchOverlapped(FinishColumnsKernel, (n - 1) / kFinishColumns + 1, kFinishThreads, 0, 1, stream,
                                    workspace, dweight, dbias, parts, n, wtype));
 }
 
