@@ -38,15 +38,19 @@ constexpr int kBlock = SML_ADAMW_ALIGN;  // values that a warp takes at once: 8 
 constexpr int kScaled = 32;              // values that share a scale
 constexpr long long kMaxNumel = 1ll << 38;  // of a tensor: the number of its tiles fits 31 bits
 constexpr int kMaxTensors = SML_ADAMW_TENSORS;
+constexpr int kFewTensors = 32;          // a launch of so few takes kernel parameters of 1 instead of 12 KB
 
-struct StepArgs {
-  SmlAdamwTensor tensor[kMaxTensors];
-  unsigned first_tile[kMaxTensors + 1];
+struct StepFactors {
   int count;
   int tile_blocks;  // kBlock's of a tile
   SmlAdamwState state;
   float lr, beta1, one_minus_beta1, beta2, one_minus_beta2, eps, decay, log_beta1, log_beta2, max_norm, minus_zero;
   const float *lr_tensor, *norm;
+};
+template <int kMax> struct StepArgs {
+  StepFactors all;
+  SmlAdamwTensor tensor[kMax];
+  unsigned first_tile[kMax + 1];
 };
 
 // The last i with first[i] <= tile.
@@ -76,7 +80,7 @@ struct Factors {
   unsigned key;
 };
 
-__device__ __forceinline__ Factors FactorsOf(const StepArgs& a, int t, float lr) {
+__device__ __forceinline__ Factors FactorsOf(const StepFactors& a, int t, float lr) {
   Factors f;
   // 1 - beta^t = -expm1(t log beta): the logarithm comes from the host in more than fp32, and expm1 keeps what a
   // difference from 1 would lose.
@@ -88,7 +92,7 @@ __device__ __forceinline__ Factors FactorsOf(const StepArgs& a, int t, float lr)
 }
 
 // What is hashed for the value at `place` of the flat buffers; for the next 255 behind a multiple of 256 it counts on.
-__device__ __forceinline__ unsigned HashedAt(const StepArgs& a, const Factors& f, long long place) {
+__device__ __forceinline__ unsigned HashedAt(const StepFactors& a, const Factors& f, long long place) {
   const unsigned long long value = a.state.first + place;
   return static_cast<unsigned>(value) + Mix(f.key + static_cast<unsigned>(value >> 32));
 }
@@ -127,7 +131,7 @@ __device__ __forceinline__ float Largest(float a, float b, float c) {
 }
 
 // One step of two values.
-__device__ __forceinline__ void Update(const StepArgs& a, const Factors& f, float clip, Pair g, Pair* p, Pair* m, Pair* v) {
+__device__ __forceinline__ void Update(const StepFactors& a, const Factors& f, float clip, Pair g, Pair* p, Pair* m, Pair* v) {
   g = g * Pair(clip);
   // Products that are rounded before they are added: ptxas makes one operation with one rounding of mul.rn.f32x2 and
   // add.rn.f32x2, but not of this, as long as it does not know that what is added is -0.
@@ -203,7 +207,7 @@ template <bool kWhole, class T> __device__ __forceinline__ void StoreTensor(T* t
 // kBlock values of a tensor from k on: 8 neighbours per lane, a scale for 4 lanes. State is there for whole blocks, and what
 // lies behind a tensor's end in it stays 0 (with the smallest scale).
 template <class T, int kBits, bool kWhole>
-__device__ __forceinline__ void StepBlock(const StepArgs& a, const SmlAdamwTensor& x, long long k, long long state, const Factors& f,
+__device__ __forceinline__ void StepBlock(const StepFactors& a, const SmlAdamwTensor& x, long long k, long long state, const Factors& f,
                                           float clip, int lane) {
   using M = std::conditional_t<kBits == 32, Packed<float>, Packed8>;
   constexpr int kMoment = kBits / 8;
@@ -291,35 +295,36 @@ __device__ __forceinline__ void StepBlock(const StepArgs& a, const SmlAdamwTenso
 }
 
 // For tensors at other addresses and for ends: out of the way of the other's registers and instructions.
-template <class T, int kBits>
-__device__ __noinline__ void StepAnyBlock(const StepArgs& a, const SmlAdamwTensor& x, long long k, long long state, Factors f,
+template <class T, int kBits, int kMax>  // (one for each kernel: ptxas 12.9 falls over one that two share)
+__device__ __noinline__ void StepAnyBlock(const StepFactors& a, const SmlAdamwTensor& x, long long k, long long state, Factors f,
                                           float clip, int lane) {
   StepBlock<T, kBits, false>(a, x, k, state, f, clip, lane);
 }
 
-template <class T, int kBits>
-__global__ void __launch_bounds__(kThreads, kBits == 8 ? 7 : 8) AdamwKernel(const __grid_constant__ StepArgs a) {
+template <class T, int kBits, int kMax>
+__global__ void __launch_bounds__(kThreads, kBits == 8 ? 7 : 8) AdamwKernel(const __grid_constant__ StepArgs<kMax> a) {
+  const StepFactors& all = a.all;
   WaitForEarlierKernels();
   const int lane = threadIdx.x & 31;
   float clip = 1.f;
-  if (a.norm) {
-    const float norm = *a.norm;
+  if (all.norm) {
+    const float norm = *all.norm;
     if (!(norm <= 3.402823466e38f)) return;  // infinite or NaN, the same for every thread: nothing changes
-    clip = fminf(__fdiv_rn(a.max_norm, __fadd_rn(norm, 1e-6f)), 1.f);
+    clip = fminf(__fdiv_rn(all.max_norm, __fadd_rn(norm, 1e-6f)), 1.f);
   }
-  const float lr = a.lr_tensor ? *a.lr_tensor : a.lr;
+  const float lr = all.lr_tensor ? *all.lr_tensor : all.lr;
   const unsigned tile = blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (tile < a.first_tile[a.count]) {
-    const int i = TensorOfTile(a.first_tile, a.count, tile);
+  if (tile < a.first_tile[all.count]) {
+    const int i = TensorOfTile(a.first_tile, all.count, tile);
     const SmlAdamwTensor& x = a.tensor[i];
-    const long long start = static_cast<long long>(tile - a.first_tile[i]) * a.tile_blocks * kBlock;
-    const long long end = min(x.numel, start + static_cast<long long>(a.tile_blocks) * kBlock);
+    const long long start = static_cast<long long>(tile - a.first_tile[i]) * all.tile_blocks * kBlock;
+    const long long end = min(x.numel, start + static_cast<long long>(all.tile_blocks) * kBlock);
     const long long state = static_cast<long long>(x.place) * kBlock;
-    const Factors f = FactorsOf(a, a.state.steps[x.step] + 1, lr);
+    const Factors f = FactorsOf(all, all.state.steps[x.step] + 1, lr);
     const bool vectors = ((reinterpret_cast<uintptr_t>(x.param) | reinterpret_cast<uintptr_t>(x.grad)) & (8 * sizeof(T) - 1)) == 0;
     for (long long k = start; k < end; k += kBlock) {
-      if (vectors && k + kBlock <= end) StepBlock<T, kBits, true>(a, x, k, state, f, clip, lane);
-      else StepAnyBlock<T, kBits>(a, x, k, state, f, clip, lane);
+      if (vectors && k + kBlock <= end) StepBlock<T, kBits, true>(all, x, k, state, f, clip, lane);
+      else StepAnyBlock<T, kBits, kMax>(all, x, k, state, f, clip, lane);
     }
   }
   // The block that ends last counts the step: every block has read the counts by then.
@@ -327,25 +332,25 @@ __global__ void __launch_bounds__(kThreads, kBits == 8 ? 7 : 8) AdamwKernel(cons
   __shared__ bool last;
   if (threadIdx.x == 0) {
     __threadfence();
-    last = atomicAdd(a.state.ticket, 1) == static_cast<int>(gridDim.x) - 1;
+    last = atomicAdd(all.state.ticket, 1) == static_cast<int>(gridDim.x) - 1;
   }
   __syncthreads();
   if (!last) return;
-  for (int i = threadIdx.x; i < a.count; i += kThreads) a.state.steps[a.tensor[i].step]++;
-  if (threadIdx.x == 0) *a.state.ticket = 0;
+  for (int i = threadIdx.x; i < all.count; i += kThreads) all.state.steps[a.tensor[i].step]++;
+  if (threadIdx.x == 0) *all.state.ticket = 0;
 }
 
-struct MasterArgs {
-  SmlAdamwTensor tensor[kMaxTensors];
-  unsigned first_tile[kMaxTensors + 1];
+template <int kMax> struct MasterArgs {
+  SmlAdamwTensor tensor[kMax];
+  unsigned first_tile[kMax + 1];
   int count;
   const short* remainder;
   float* out;
 };
 
 // A warp per kBlock values; `out` is written up to the end of a tensor's last block, with zeros there.
-template <class T>
-__global__ void __launch_bounds__(kThreads) MastersKernel(const __grid_constant__ MasterArgs a) {
+template <class T, int kMax>
+__global__ void __launch_bounds__(kThreads) MastersKernel(const __grid_constant__ MasterArgs<kMax> a) {
   WaitForEarlierKernels();
   const unsigned tile = blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (tile >= a.first_tile[a.count]) return;
@@ -377,9 +382,9 @@ constexpr int kNormThreads = 256;
 constexpr int kNormBlocks = 148 * 8;  // partial sums of a launch, at most: the blocks that the GPU holds
 constexpr int kNormTile = 4096;       // values that a block takes at once
 
-struct NormArgs {
-  SmlNormTensor tensor[kMaxTensors];
-  unsigned first_tile[kMaxTensors + 1];
+template <int kMax> struct NormArgs {
+  SmlNormTensor tensor[kMax];
+  unsigned first_tile[kMax + 1];
   int count;
   double* partial;  // one for each block of this launch
   const double* all;  // of all launches: the last one's last block sums them, if there is a ticket
@@ -439,7 +444,7 @@ __device__ __forceinline__ void Finish(const double* partial, int parts, float* 
 
 // Squares are summed in fp64: 2^-53 of a sum over 10^9 values still leaves the result right to its last fp32 bit, and no
 // gradient's square overflows or vanishes.
-__global__ void __launch_bounds__(kNormThreads, 8) NormKernel(const __grid_constant__ NormArgs a) {
+template <int kMax> __global__ void __launch_bounds__(kNormThreads, 8) NormKernel(const __grid_constant__ NormArgs<kMax> a) {
   WaitForEarlierKernels();
   LetNextKernelStart();
   double sum = 0.0;
@@ -473,17 +478,18 @@ __global__ void __launch_bounds__(kNormThreads) FinishNormKernel(const double* p
 
 // Fills in one launch's share of `tensors` from `*at` on and returns the number of its tiles. Empty tensors take none.
 template <class Args, class Tensor>
-unsigned TakeTensors(const Tensor* tensors, int count, long long tile, int* at, Args* a) {
+unsigned TakeTensors(const Tensor* tensors, int count, long long tile, int* at, Args* a, int* taken) {
+  constexpr int kMax = sizeof(a->tensor) / sizeof(a->tensor[0]);
   unsigned long long tiles = 0;
-  a->count = 0;
-  for (; *at < count && a->count < kMaxTensors; ++*at) {
+  *taken = 0;
+  for (; *at < count && *taken < kMax; ++*at) {
     const unsigned long long more = static_cast<unsigned long long>((tensors[*at].numel + tile - 1) / tile);
-    if (tiles + more > 0x7fffffffull && a->count > 0) break;
-    a->tensor[a->count] = tensors[*at];
-    a->first_tile[a->count++] = static_cast<unsigned>(tiles);
+    if (tiles + more > 0x7fffffffull && *taken > 0) break;
+    a->tensor[*taken] = tensors[*at];
+    a->first_tile[(*taken)++] = static_cast<unsigned>(tiles);
     tiles += more;
   }
-  a->first_tile[a->count] = static_cast<unsigned>(tiles);
+  a->first_tile[*taken] = static_cast<unsigned>(tiles);
   return static_cast<unsigned>(tiles);
 }
 
@@ -499,6 +505,55 @@ int TileBlocks(const SmlAdamwTensor* tensors, int count, int bits) {
   return tile;
 }
 
+template <int kMax> int Step(const SmlAdamwTensor* tensors, int count, const StepFactors& factors, int type, cudaStream_t stream) {
+  StepArgs<kMax> a;
+  a.all = factors;
+  for (int at = 0; at < count;) {
+    const unsigned tiles = TakeTensors(tensors, count, static_cast<long long>(factors.tile_blocks) * kBlock, &at, &a, &a.all.count);
+    const unsigned blocks = tiles ? (tiles + kWarps - 1) / kWarps : 1;  // (empty tensors' steps count too)
+    void (*kernel)(StepArgs<kMax>) = AdamwKernel<float, 32, kMax>;
+    if (type == SML_ADAMW_F32 && factors.state.bits == 8) kernel = AdamwKernel<float, 8, kMax>;
+    if (type == SML_ADAMW_BF16) kernel = factors.state.bits == 8 ? AdamwKernel<__nv_bfloat16, 8, kMax> : AdamwKernel<__nv_bfloat16, 32, kMax>;
+    const cudaError_t e = LaunchOverlapped(kernel, blocks, kThreads, 0, 1, stream, a);
+    if (e != cudaSuccess) return Launched(e);
+  }
+  return 0;
+}
+
+template <int kMax>
+int Masters(const SmlAdamwTensor* tensors, int count, const short* remainder, float* out, int type, cudaStream_t stream) {
+  MasterArgs<kMax> a;
+  a.remainder = remainder, a.out = out;
+  for (int at = 0; at < count;) {
+    const unsigned tiles = TakeTensors(tensors, count, kBlock, &at, &a, &a.count);
+    if (!tiles) continue;
+    const cudaError_t e = LaunchOverlapped(type == SML_ADAMW_F32 ? MastersKernel<float, kMax> : MastersKernel<__nv_bfloat16, kMax>,
+                                           (tiles + kWarps - 1) / kWarps, kThreads, 0, 1, stream, a);
+    if (e != cudaSuccess) return Launched(e);
+  }
+  return 0;
+}
+
+template <int kMax>
+int GradNorm(const SmlNormTensor* tensors, int count, double* workspace, int* ticket, float* out, cudaStream_t stream) {
+  NormArgs<kMax> a;
+  a.all = workspace, a.out = out, a.parts = 0;
+  int at = 0;
+  do {
+    const unsigned tiles = TakeTensors(tensors, count, kNormTile, &at, &a, &a.count);
+    if (!tiles && !(ticket && at == count)) continue;
+    const unsigned each = (tiles + kNormBlocks - 1) / kNormBlocks;  // tiles of a block: the same number for all but the last
+    const unsigned blocks = tiles ? (tiles + each - 1) / each : 1;
+    a.partial = workspace + a.parts;
+    a.parts += blocks;
+    a.ticket = at == count ? ticket : nullptr;
+    const cudaError_t e = LaunchOverlapped(NormKernel<kMax>, blocks, kNormThreads, 0, 1, stream, a);
+    if (e != cudaSuccess) return Launched(e);
+  } while (at < count);
+  if (ticket) return 0;
+  return Launched(LaunchOverlapped(FinishNormKernel, 1, kNormThreads, 0, 1, stream, a.all, a.parts, out));
+}
+
 }  // namespace
 
 extern "C" int switchml_adamw_step(const SmlAdamwTensor* tensors, int count, const SmlAdamwState* state, const SmlAdamwStep* step,
@@ -509,7 +564,7 @@ extern "C" int switchml_adamw_step(const SmlAdamwTensor* tensors, int count, con
     return -1;
   for (int i = 0; i < count; i++)
     if (tensors[i].numel < 0 || tensors[i].numel > kMaxNumel || (tensors[i].numel && (!tensors[i].param || !tensors[i].grad))) return -1;
-  StepArgs a;
+  StepFactors a;
   a.state = *state;
   a.lr = static_cast<float>(step->lr);
   a.beta1 = static_cast<float>(step->beta1), a.one_minus_beta1 = static_cast<float>(1.0 - step->beta1);
@@ -519,31 +574,16 @@ extern "C" int switchml_adamw_step(const SmlAdamwTensor* tensors, int count, con
   a.minus_zero = -0.f;
   a.max_norm = step->max_norm, a.lr_tensor = step->lr_tensor, a.norm = step->norm;
   a.tile_blocks = TileBlocks(tensors, count, state->bits);
-  for (int at = 0; at < count;) {
-    const unsigned tiles = TakeTensors(tensors, count, static_cast<long long>(a.tile_blocks) * kBlock, &at, &a);
-    const unsigned blocks = tiles ? (tiles + kWarps - 1) / kWarps : 1;  // (empty tensors' steps count too)
-    void (*kernel)(StepArgs) = type == SML_ADAMW_F32 ? (state->bits == 32 ? AdamwKernel<float, 32> : AdamwKernel<float, 8>)
-                                                     : (state->bits == 32 ? AdamwKernel<__nv_bfloat16, 32> : AdamwKernel<__nv_bfloat16, 8>);
-    const cudaError_t e = LaunchOverlapped(kernel, blocks, kThreads, 0, 1, static_cast<cudaStream_t>(stream), a);
-    if (e != cudaSuccess) return Launched(e);
-  }
-  return 0;
+  if (count <= kFewTensors) return Step<kFewTensors>(tensors, count, a, type, static_cast<cudaStream_t>(stream));
+  return Step<kMaxTensors>(tensors, count, a, type, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int switchml_adamw_masters(const SmlAdamwTensor* tensors, int count, const short* remainder, float* out, int type, void* stream) {
   if (!tensors || count < 0 || !out || (type != SML_ADAMW_F32 && (type != SML_ADAMW_BF16 || !remainder))) return -1;
   for (int i = 0; i < count; i++)
     if (tensors[i].numel < 0 || tensors[i].numel > kMaxNumel || (tensors[i].numel && !tensors[i].param)) return -1;
-  MasterArgs a;
-  a.remainder = remainder, a.out = out;
-  for (int at = 0; at < count;) {
-    const unsigned tiles = TakeTensors(tensors, count, kBlock, &at, &a);
-    if (!tiles) continue;
-    const cudaError_t e = LaunchOverlapped(type == SML_ADAMW_F32 ? MastersKernel<float> : MastersKernel<__nv_bfloat16>,
-                                           (tiles + kWarps - 1) / kWarps, kThreads, 0, 1, static_cast<cudaStream_t>(stream), a);
-    if (e != cudaSuccess) return Launched(e);
-  }
-  return 0;
+  if (count <= kFewTensors) return Masters<kFewTensors>(tensors, count, remainder, out, type, static_cast<cudaStream_t>(stream));
+  return Masters<kMaxTensors>(tensors, count, remainder, out, type, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" long long switchml_grad_norm_workspace(int count) {
@@ -556,20 +596,6 @@ extern "C" int switchml_grad_norm(const SmlNormTensor* tensors, int count, doubl
     if (tensors[i].numel < 0 || tensors[i].numel > kMaxNumel || (tensors[i].numel && !tensors[i].data) ||
         (tensors[i].type != SML_ADAMW_F32 && tensors[i].type != SML_ADAMW_BF16))
       return -1;
-  NormArgs a;
-  a.all = workspace, a.out = out, a.parts = 0;
-  int at = 0;
-  do {
-    const unsigned tiles = TakeTensors(tensors, count, kNormTile, &at, &a);
-    if (!tiles && !(ticket && at == count)) continue;
-    const unsigned each = (tiles + kNormBlocks - 1) / kNormBlocks;  // tiles of a block: the same number for all but the last
-    const unsigned blocks = tiles ? (tiles + each - 1) / each : 1;
-    a.partial = workspace + a.parts;
-    a.parts += blocks;
-    a.ticket = at == count ? ticket : nullptr;
-    const cudaError_t e = LaunchOverlapped(NormKernel, blocks, kNormThreads, 0, 1, static_cast<cudaStream_t>(stream), a);
-    if (e != cudaSuccess) return Launched(e);
-  } while (at < count);
-  if (ticket) return 0;
-  return Launched(LaunchOverlapped(FinishNormKernel, 1, kNormThreads, 0, 1, static_cast<cudaStream_t>(stream), a.all, a.parts, out));
+  if (count <= kFewTensors) return GradNorm<kFewTensors>(tensors, count, workspace, ticket, out, static_cast<cudaStream_t>(stream));
+  return GradNorm<kMaxTensors>(tensors, count, workspace, ticket, out, static_cast<cudaStream_t>(stream));
 }

@@ -46,32 +46,45 @@ void CheckParameter(const Tensor& p, const char* name, const Tensor& x, const Te
 
 class LayerNorm : public torch::autograd::Function<LayerNorm> {
  public:
-  static variable_list forward(AutogradContext* ctx, const Tensor& x_in, const OptTensor& residual_in, const OptTensor& weight_in,
-                               const OptTensor& bias_in, double eps, bool backward_comes) {
+  // y, with a residual the sum, and with `stats` mean and 1 / deviation of every row.
+  struct Result {
+    Tensor y, sum, stats, x, weight, bias;  // the inputs as they were read
+  };
+  static Result Run(const Tensor& x_in, const OptTensor& residual_in, const OptTensor& weight_in, const OptTensor& bias_in, double eps,
+                    bool with_stats) {
     const c10::cuda::OptionalCUDAGuard device(x_in.device());
     const bool add = residual_in.has_value();
-    const Tensor x = x_in.contiguous(), residual = add ? residual_in->contiguous() : Tensor();
-    const Tensor weight = weight_in ? weight_in->contiguous() : Tensor(), bias = bias_in ? bias_in->contiguous() : Tensor();
-    const int64_t n = x.size(-1), rows = x.numel() / n;
-    Tensor y = at::empty_like(x), sum = add ? at::empty_like(x) : Tensor(), stats;
-    if (backward_comes) stats = at::empty({2, rows}, x.options().dtype(at::kFloat));
-    float* mean = backward_comes ? stats.data_ptr<float>() : nullptr;
+    Result r;
+    r.x = x_in.contiguous();
+    const Tensor residual = add ? residual_in->contiguous() : Tensor();
+    if (weight_in) r.weight = weight_in->contiguous();
+    if (bias_in) r.bias = bias_in->contiguous();
+    const int64_t n = r.x.size(-1), rows = r.x.numel() / n;
+    r.y = at::empty_like(r.x);
+    if (add) r.sum = at::empty_like(r.x);
+    if (with_stats) r.stats = at::empty({2, rows}, r.x.options().dtype(at::kFloat));
+    float* mean = with_stats ? r.stats.data_ptr<float>() : nullptr;
     if (rows > 0) {
-      const Tensor& p = weight.defined() ? weight : bias;
-      Check(switchml_layer_norm_forward(Data(x), Data(residual), Data(weight), Data(bias), y.data_ptr(), Data(sum), mean,
-                                        mean ? mean + rows : nullptr, rows, static_cast<int>(n), static_cast<float>(eps), NormType(x),
+      const Tensor& p = r.weight.defined() ? r.weight : r.bias;
+      Check(switchml_layer_norm_forward(Data(r.x), Data(residual), Data(r.weight), Data(r.bias), r.y.data_ptr(), Data(r.sum), mean,
+                                        mean ? mean + rows : nullptr, rows, static_cast<int>(n), static_cast<float>(eps), NormType(r.x),
                                         p.defined() ? NormType(p) : SML_NORM_F32, CurrentStream()),
             "layer_norm");
     }
-    if (backward_comes) {
-      ctx->save_for_backward({add ? sum : x, weight, stats});
-      ctx->saved_data["residual"] = add;
-      ctx->saved_data["bias"] = bias.defined();
-      ctx->saved_data["bias_bf16"] = bias.defined() && bias.scalar_type() == at::kBFloat16;
-      ctx->set_materialize_grads(false);
-    }
-    if (add) return {y, sum};
-    return {y};
+    return r;
+  }
+
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual, const OptTensor& weight,
+                               const OptTensor& bias, double eps) {
+    const Result r = Run(x, residual, weight, bias, eps, true);
+    const bool add = residual.has_value();
+    ctx->save_for_backward({add ? r.sum : r.x, r.weight, r.stats});
+    ctx->saved_data["residual"] = add;
+    ctx->saved_data["bias"] = r.bias.defined();
+    ctx->saved_data["bias_bf16"] = r.bias.defined() && r.bias.scalar_type() == at::kBFloat16;
+    ctx->set_materialize_grads(false);
+    if (add) return {r.y, r.sum};
+    return {r.y};
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -109,7 +122,7 @@ class LayerNorm : public torch::autograd::Function<LayerNorm> {
       }
     }
     const bool want_residual = weight_edge == 2 && ctx->needs_input_grad(residual_edge);
-    return {ctx->needs_input_grad(0) ? dx : Tensor(), want_residual ? dx : Tensor(), dweight, dbias, Tensor(), Tensor()};
+    return {ctx->needs_input_grad(0) ? dx : Tensor(), want_residual ? dx : Tensor(), dweight, dbias, Tensor()};
   }
 };
 
@@ -135,7 +148,11 @@ variable_list LayerNormForward(Tensor x, OptTensor residual, const OptTensor& we
   CheckParameter(bias.value_or(Tensor()), "bias", x, weight.value_or(Tensor()));
   const auto wants = [](const OptTensor& t) { return t && t->requires_grad(); };
   const bool backward_comes = at::GradMode::is_enabled() && (x.requires_grad() || wants(residual) || wants(weight) || wants(bias));
-  return LayerNorm::apply(x, residual, weight, bias, eps, backward_comes);
+  if (backward_comes) return LayerNorm::apply(x, residual, weight, bias, eps);
+  at::AutoDispatchBelowADInplaceOrView below_autograd;
+  const auto r = LayerNorm::Run(x, residual, weight, bias, eps, false);
+  if (residual) return {r.y, r.sum};
+  return {r.y};
 }
 
 // ---- gradient norm ----
@@ -164,7 +181,7 @@ Tensor GradNorm(const py::list& tensors) {
   std::optional<c10::cuda::CUDAGuard> device;
   for (Py_ssize_t i = 0; i < count; i++) {
     PyObject* const item = PyList_GET_ITEM(tensors.ptr(), i);
-    TORCH_CHECK_TYPE(THPVariable_Check(item), "grad_norm: tensors are wanted");
+    TORCH_CHECK_TYPE(THPVariable_CheckExact(item) || THPVariable_Check(item), "grad_norm: tensors are wanted");
     const Tensor* t = &THPVariable_Unpack(item);
     TORCH_CHECK_TYPE(t->layout() == at::kStrided && Known(*t), "grad_norm: a tensor is ", t->layout(), " ", t->scalar_type(),
                      ": strided float32 or bfloat16 is wanted");

@@ -185,18 +185,29 @@ class FusedAdamW(torch.optim.Optimizer):
                     group[key].copy_(torch.as_tensor(value))  # a captured step reads it
                 else:
                     group[key] = value.clone().to(self._device) if isinstance(value, torch.Tensor) else value
+        copies, fills = ([], []), []
         for entry, p in plans:
             state = self.state[p]
-            state["step"].fill_(int(entry.get("step", 0)))
+            fills.append(int(entry.get("step", 0)))
             if "remainder" in state:
                 if "remainder" in entry:
-                    state["remainder"].copy_(entry["remainder"])
+                    copies[0].append(state["remainder"])
+                    copies[1].append(entry["remainder"])
                 else:
                     state["remainder"].zero_()
             for name in _MOMENTS:
-                self._load(entry, state, name, p)
+                self._load(entry, state, name, p, copies)
+        if copies[0]:
+            torch._foreach_copy_(*copies)
+        at = 0
+        for group in self.param_groups:
+            n = len(group["params"])
+            if n:
+                steps = self.state[group["params"][0]]["step"]._base
+                steps[:n].copy_(torch.tensor(fills[at:at + n], dtype=torch.int32))
+            at += n
 
-    def _load(self, entry, state, name, p):
+    def _load(self, entry, state, name, p, copies):
         new, scale = state[name], state.get(name + "_scale")
         old = entry.get(name)
         if old is None:
@@ -206,13 +217,14 @@ class FusedAdamW(torch.optim.Optimizer):
             return
         eight = old.dtype == torch.float8_e4m3fn
         if eight and self._bits == 8 and old.stride() == new.stride():
-            new.view(torch.uint8).copy_(old.view(torch.uint8))
-            scale.view(torch.uint8).copy_(entry[name + "_scale"].view(torch.uint8))
+            copies[0].extend((new.view(torch.uint8), scale.view(torch.uint8)))
+            copies[1].extend((old.view(torch.uint8), entry[name + "_scale"].view(torch.uint8)))
             return
         if eight:
             old = dequantized(old, entry[name + "_scale"])
         if self._bits == 32:
-            new.copy_(old)
+            copies[0].append(new)
+            copies[1].append(old)
             return
         flat = torch.empty_strided(p.shape, p.stride(), dtype=torch.float32, device=p.device).copy_(old).as_strided((p.numel(),), (1,))
         blocks = torch.nn.functional.pad(flat, (0, -p.numel() % _SCALED)).view(-1, _SCALED)
