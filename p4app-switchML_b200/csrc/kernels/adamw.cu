@@ -348,7 +348,9 @@ template <int kMax> struct MasterArgs {
   float* out;
 };
 
-// A warp per kBlock values; `out` is written up to the end of a tensor's last block, with zeros there.
+constexpr int kMasterBlocks = 4;  // kBlock's of a warp
+
+// `out` is written up to the end of a tensor's last block, with zeros there.
 template <class T, int kMax>
 __global__ void __launch_bounds__(kThreads) MastersKernel(const __grid_constant__ MasterArgs<kMax> a) {
   WaitForEarlierKernels();
@@ -356,26 +358,30 @@ __global__ void __launch_bounds__(kThreads) MastersKernel(const __grid_constant_
   if (tile >= a.first_tile[a.count]) return;
   const int i = TensorOfTile(a.first_tile, a.count, tile);
   const SmlAdamwTensor& x = a.tensor[i];
-  const long long start = static_cast<long long>(tile - a.first_tile[i]) * kBlock, state = static_cast<long long>(x.place) * kBlock;
-  const long long k = start + (threadIdx.x & 31) * 8;
-  Packed<T> p;
-  if (k + 8 <= x.numel && (reinterpret_cast<uintptr_t>(x.param) & (8 * sizeof(T) - 1)) == 0)
-    LoadTensor<true>(static_cast<const T*>(x.param) + k, 8, &p);
-  else
-    LoadTensor<false>(static_cast<const T*>(x.param) + k, static_cast<int>(max(min(x.numel - k, 8ll), 0ll)), &p);
-  Packed<float> out;
-  if constexpr (sizeof(T) == 2) {
-    Packed<__nv_bfloat16> r;
-    LoadWords(a.remainder + state + k, r.w);
+  const long long state = static_cast<long long>(x.place) * kBlock;
+  const long long start = static_cast<long long>(tile - a.first_tile[i]) * kMasterBlocks * kBlock;
+  const bool vectors = (reinterpret_cast<uintptr_t>(x.param) & (8 * sizeof(T) - 1)) == 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      out.w[2 * i] = __float_as_uint(WithRemainder(p.w[i] & 0xffff, r.w[i]));
-      out.w[2 * i + 1] = __float_as_uint(WithRemainder(p.w[i] >> 16, r.w[i] >> 16));
+  for (int j = 0; j < kMasterBlocks; j++) {
+    if (start + j * kBlock >= x.numel) break;
+    const long long k = start + j * kBlock + (threadIdx.x & 31) * 8;
+    Packed<T> p;
+    if (vectors && k + 8 <= x.numel) LoadTensor<true>(static_cast<const T*>(x.param) + k, 8, &p);
+    else LoadTensor<false>(static_cast<const T*>(x.param) + k, static_cast<int>(max(min(x.numel - k, 8ll), 0ll)), &p);
+    Packed<float> out;
+    if constexpr (sizeof(T) == 2) {
+      Packed<__nv_bfloat16> r;
+      LoadWords(a.remainder + state + k, r.w);
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        out.w[2 * u] = __float_as_uint(WithRemainder(p.w[u] & 0xffff, r.w[u]));
+        out.w[2 * u + 1] = __float_as_uint(WithRemainder(p.w[u] >> 16, r.w[u] >> 16));
+      }
+    } else {
+      out = p;
     }
-  } else {
-    out = p;
+    StoreWords(a.out + state + k, out.w);
   }
-  StoreWords(a.out + state + k, out.w);
 }
 
 constexpr int kNormThreads = 256;
@@ -409,24 +415,21 @@ __device__ __forceinline__ double BlockSum(double v) {
 // Over this thread's share of the values from start to end, at most kNormTile.
 template <class T>
 __device__ __forceinline__ double SquaresOf(const T* x, long long start, long long end) {
+  constexpr int kVectors = kNormTile / (kNormThreads * 8);
+  const bool vectors = (reinterpret_cast<uintptr_t>(x) & (8 * sizeof(T) - 1)) == 0;
   double sum = 0.0;
-  if (end - start == kNormTile && (reinterpret_cast<uintptr_t>(x) & (8 * sizeof(T) - 1)) == 0) {
-    constexpr int kVectors = kNormTile / (kNormThreads * 8);
-    Packed<T> v[kVectors];
+  Packed<T> v[kVectors];
 #pragma unroll
-    for (int u = 0; u < kVectors; u++) LoadWords(x + start + (u * kNormThreads + threadIdx.x) * 8, v[u].w);
+  for (int u = 0; u < kVectors; u++) {
+    const long long k = start + (u * kNormThreads + threadIdx.x) * 8;
+    if (vectors && k + 8 <= end) LoadTensor<true>(x + k, 8, &v[u]);
+    else LoadTensor<false>(x + k, static_cast<int>(max(min(end - k, 8ll), 0ll)), &v[u]);
+  }
 #pragma unroll
-    for (int u = 0; u < kVectors; u++) {
+  for (int u = 0; u < kVectors; u++) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const double g = v[u].At(i);
-        sum += g * g;
-      }
-    }
-  } else {
-#pragma unroll 4
-    for (long long k = start + threadIdx.x; k < end; k += kNormThreads) {
-      const double g = static_cast<float>(x[k]);
+    for (int i = 0; i < 8; i++) {
+      const double g = v[u].At(i);
       sum += g * g;
     }
   }
@@ -494,15 +497,21 @@ unsigned TakeTensors(const Tensor* tensors, int count, long long tile, int* at, 
 }
 
 // A warp's tile, in kBlock's. What a tile costs by itself (finding its tensor, the factors, a place among the resident
-// warps) is shared by its blocks: 2^28 fp32 parameters with moments in 8 bits took 943, 771, 693 and 726 us with tiles
-// of 4, 8, 16 and 32 blocks, with fp32 moments 1104, 1120, 1125 and 1131 us (there the memory is the limit, which likes short ones).
-// Few values make smaller tiles, so that every warp that the GPU holds gets one.
+// warps) is shared by its blocks: 2^28 fp32 parameters with moments in 8 bits took 943, 771, 669 and 675 us with tiles
+// of 4, 8, 16 and 32 blocks, with fp32 moments 1104, 1120, 1125 and 1131 us (there the memory is the limit, which likes short
+// ones). Fewer values make smaller tiles: as many as the GPU holds warps, so that all run at once.
 int TileBlocks(const SmlAdamwTensor* tensors, int count, int bits) {
+  const int most = bits == 8 ? 16 : 4;
+  const long long resident = 148ll * kWarps * (bits == 8 ? 7 : 8);
   long long blocks = 0;
   for (int i = 0; i < count; i++) blocks += (tensors[i].numel + kBlock - 1) / kBlock;
-  int tile = bits == 8 ? 16 : 4;
-  while (tile > 1 && blocks < static_cast<long long>(tile) * 148 * 32) tile /= 2;
-  return tile;
+  for (long long tile = (blocks + resident - 1) / resident; tile < most; tile++) {
+    if (tile < 1) return 1;
+    long long tiles = 0;
+    for (int i = 0; i < count; i++) tiles += ((tensors[i].numel + kBlock - 1) / kBlock + tile - 1) / tile;
+    if (tiles <= resident || (tile == 1 && blocks < resident)) return static_cast<int>(tile);
+  }
+  return most;
 }
 
 template <int kMax> int Step(const SmlAdamwTensor* tensors, int count, const StepFactors& factors, int type, cudaStream_t stream) {
@@ -525,7 +534,7 @@ int Masters(const SmlAdamwTensor* tensors, int count, const short* remainder, fl
   MasterArgs<kMax> a;
   a.remainder = remainder, a.out = out;
   for (int at = 0; at < count;) {
-    const unsigned tiles = TakeTensors(tensors, count, kBlock, &at, &a, &a.count);
+    const unsigned tiles = TakeTensors(tensors, count, kMasterBlocks * kBlock, &at, &a, &a.count);
     if (!tiles) continue;
     const cudaError_t e = LaunchOverlapped(type == SML_ADAMW_F32 ? MastersKernel<float, kMax> : MastersKernel<__nv_bfloat16, kMax>,
                                            (tiles + kWarps - 1) / kWarps, kThreads, 0, 1, stream, a);
