@@ -10,7 +10,7 @@ Public surface (mirrors ``switchml::Context`` of the reference, client_lib/src/c
     ctx.wait_for_all_jobs(); ctx.get_stats(); ctx.stop()
 
 Sub-packages: ``parallel`` (context, DDP hook, gradient bucketing, process group),
-``ops`` (kernel wrappers: allreduce emulation, oracle, weight-gradient GEMM),
+``ops`` (kernel wrappers: allreduce emulation, oracle, weight-gradient GEMM, layer norm, AdamW),
 ``models`` (ResNet-50, VGG-19, BERT-large), ``utils`` (config files, timing, clocks, CLI).
 """
 from ._native import lib, library_path, NativeError  # noqa: F401

@@ -10,7 +10,10 @@ AdamW. Weights and gradients are float32, the forward/backward math runs under b
 autocast. ``--ddp sml`` uses this library (gradient buckets in the symmetric heap reduced
 in place while backward continues; with ``--fused-wgrad 1`` the largest Linear layers
 compute their weight gradients with the tcgen05 GEMM that reduces across GPUs in its own
-epilogue). ``--ddp torch`` is PyTorch DDP over NCCL, the baseline. Times are CUDA-event
+epilogue; with ``--fused-norm 1`` BERT's layer norms take the residual sums in front of them into
+their kernels). ``--optimizer fused`` takes AdamW's step in one launch over all tensors
+(``ops.adamw.FusedAdamW``), ``fused8`` with moments in 8 bits, ``--max-norm`` clips by the norm of
+all gradients within it. ``--ddp torch`` is PyTorch DDP over NCCL, the baseline. Times are CUDA-event
 times, maximum over ranks; the end-to-end figure also counts the host→device copy of each
 batch from pinned memory and the device→host read of the loss.
 """
@@ -31,13 +34,13 @@ if ROOT not in sys.path:
 DEFAULT_BATCH = {"resnet50": 64, "vgg19": 32, "bert": 16}
 
 
-def build(model_name, fused):
+def build(model_name, fused, fused_norm=False):
     from switchml_b200.models import resnet50, vgg19, bert_large
     if model_name == "resnet50":
         return resnet50()
     if model_name == "vgg19":
         return vgg19(fused_fc=fused)
-    return bert_large(fused_ffn=fused)
+    return bert_large(fused_ffn=fused, fused_norm=fused_norm)
 
 
 def make_batch(model_name, batch, seq, gen):
@@ -73,7 +76,8 @@ def bench_training(args):
     if world > 1:
         dist.init_process_group("nccl", rank=rank, world_size=world, device_id=dev)
     torch.manual_seed(0)  # identical initial weights on every rank
-    model = build(model_name, fused).to(dev)
+    fused_norm = bool(getattr(args, "fused_norm", 0)) and model_name == "bert"
+    model = build(model_name, fused, fused_norm).to(dev)
     nparams = sum(p.numel() for p in model.parameters())
 
     ctx = None
@@ -97,10 +101,23 @@ def bench_training(args):
                                                         gradient_as_bucket_view=True)
     else:
         net = model
-    if model_name == "bert":
+    optimizer = getattr(args, "optimizer", "torch")
+    max_norm = getattr(args, "max_norm", 0.0) or None
+    if optimizer == "torch" and max_norm:
+        raise SystemExit("--max-norm needs --optimizer fused or fused8")
+    if optimizer != "torch":
+        from switchml_b200.ops.adamw import FusedAdamW
+        opt = FusedAdamW(model.parameters(), lr=1e-4, state_bits=8 if optimizer == "fused8" else 32, max_norm=max_norm)
+    elif model_name == "bert":
         opt = torch.optim.AdamW(model.parameters(), lr=1e-4, fused=True)
     else:
         opt = torch.optim.SGD(model.parameters(), lr=0.01, momentum=0.9)
+
+    if fused_norm:  # forward, backward and the sums over its blocks, of every layer norm
+        from switchml_b200.ops.layer_norm import FusedLayerNorm
+        launches_per_step += 3 * sum(isinstance(m, FusedLayerNorm) for m in model.modules())
+    if optimizer != "torch":
+        launches_per_step += -(-len(list(model.parameters())) // 384) * (2 if max_norm else 1)
 
     gen = torch.Generator().manual_seed(100 + rank)
     host_batches = [make_batch(model_name, batch, seq, gen) for _ in range(2)]
@@ -172,7 +189,9 @@ def bench_training(args):
         "config": {"model": {"resnet50": "ResNet-50", "vgg19": "VGG-19", "bert": "BERT-large MLM"}[model_name],
                    "global_batch": batch * world, "seq_len": seq if model_name == "bert" else None,
                    "parallelism": "dp%d" % world, "params_m": nparams / 1e6, "ddp": ddp_kind,
-                   "fused_wgrad": fused, "optimizer": "AdamW" if model_name == "bert" else "SGD-m0.9",
+                   "fused_wgrad": fused, "fused_norm": fused_norm,
+                   "optimizer": "AdamW" + {"torch": "", "fused": " fused", "fused8": " fused, 8-bit moments"}[optimizer]
+                   if model_name == "bert" or optimizer != "torch" else "SGD-m0.9",
                    "l2": "activations and gradients of a step exceed the 126 MB L2"},
         "e2e": {"value": per_step / (e2e_ms * 1e-3), "unit": "tokens/s" if model_name == "bert" else "images/s",
                 "ms_per_step": e2e_ms, "h2d_bytes_per_step": h2d, "d2h_bytes_per_step": 4},
@@ -187,6 +206,9 @@ if __name__ == "__main__":
     ap.add_argument("--model", default="resnet50", choices=["resnet50", "vgg19", "bert"])
     ap.add_argument("--ddp", default="sml", choices=["sml", "torch"])
     ap.add_argument("--fused-wgrad", type=int, default=0)
+    ap.add_argument("--fused-norm", type=int, default=0)
+    ap.add_argument("--optimizer", default="torch", choices=["torch", "fused", "fused8"])
+    ap.add_argument("--max-norm", type=float, default=0.0)
     ap.add_argument("--steps", type=int, default=10)
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--batch", type=int, default=0)

@@ -507,3 +507,19 @@ def test_a_training_step_with_aggregated_gradients():
                 torch.testing.assert_close(q[1], p, rtol=1e-5, atol=1e-6, msg=name)
     finally:
         ctx.stop()
+
+
+def test_training_command():
+    """ddp_train.py with everything fused: runs, and says what it ran."""
+    import json
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    cmd = [sys.executable, os.path.join(root, "p4app-switchML_b200", "benchmarks", "ddp_train.py"), "--model", "bert", "--batch", "2",
+           "--steps", "2", "--warmup", "1", "--fused-norm", "1", "--fused-wgrad", "1", "--optimizer", "fused8", "--max-norm", "1"]
+    r = subprocess.run(cmd, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-2000:]
+    out = json.loads([line for line in r.stdout.splitlines() if line.startswith("{")][-1])
+    assert out["config"]["optimizer"] == "AdamW fused, 8-bit moments" and out["config"]["fused_norm"]
+    assert 0 < out["final_loss"] < 100
