@@ -162,10 +162,12 @@ int AdamwType(const Tensor& t) { return t.scalar_type() == at::kFloat ? SML_ADAM
 // Same values in the same places of memory, without gaps: what an elementwise pass over memory may take.
 bool Dense(const Tensor& t) { return t.is_non_overlapping_and_dense(); }
 
-void NormOf(const std::vector<SmlNormTensor>& list, Tensor* workspace, int* ticket, const Tensor& out) {
-  const int64_t doubles = switchml_grad_norm_workspace(static_cast<int>(list.size()));
-  if (!workspace->defined() || workspace->numel() < doubles) *workspace = at::empty({doubles}, out.options().dtype(at::kDouble));
-  Check(switchml_grad_norm(list.data(), static_cast<int>(list.size()), workspace->data_ptr<double>(), ticket, out.data_ptr<float>(), CurrentStream()),
+Tensor NormWorkspace(size_t tensors, const at::TensorOptions& where) {
+  return at::empty({switchml_grad_norm_workspace(static_cast<int>(tensors))}, where.dtype(at::kDouble));
+}
+
+void NormOf(const std::vector<SmlNormTensor>& list, const Tensor& workspace, int* ticket, const Tensor& out) {
+  Check(switchml_grad_norm(list.data(), static_cast<int>(list.size()), workspace.data_ptr<double>(), ticket, out.data_ptr<float>(), CurrentStream()),
         "grad_norm");
 }
 
@@ -194,8 +196,8 @@ Tensor GradNorm(const py::list& tensors) {
     }
     list.push_back({Data(*t), t->numel(), AdamwType(*t)});
   }
-  Tensor out = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(where)), workspace;
-  NormOf(list, &workspace, nullptr, out);
+  const Tensor out = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(where));
+  NormOf(list, NormWorkspace(list.size(), out.options()), nullptr, out);
   return out;
 }
 
@@ -220,6 +222,9 @@ class Adamw {
     g.exp_avg = std::move(exp_avg), g.exp_avg_sq = std::move(exp_avg_sq), g.steps = std::move(steps), g.first = first;
     g.exp_avg_scale = exp_avg_scale.value_or(Tensor()), g.exp_avg_sq_scale = exp_avg_sq_scale.value_or(Tensor());
     g.remainder = remainder.value_or(Tensor());
+    // Steps may have been captured with the workspace that there was: it stays.
+    count_ += g.params.size();
+    workspaces_.push_back(NormWorkspace(count_, g.exp_avg.options()));
     if (!ticket_.defined()) {
       ticket_ = at::zeros({1}, g.exp_avg.options().dtype(at::kInt));
       norm_ = at::zeros({}, g.exp_avg.options().dtype(at::kFloat));
@@ -252,12 +257,11 @@ class Adamw {
           }
           tensors_.push_back({Data(p), Data(grad), g.numel[i], static_cast<unsigned>(g.place[i]), static_cast<int>(i)});
           if (max_norm) norms_.push_back({Data(grad), g.numel[i], type});
-          p.unsafeGetTensorImpl()->bump_version();
         }
         if (tensors_.size() > begin) runs.push_back({k, {begin, tensors_.size(), type}});
       }
     }
-    if (max_norm) NormOf(norms_, &workspace_, ticket_.data_ptr<int>(), norm_);
+    if (max_norm) NormOf(norms_, workspaces_.back(), ticket_.data_ptr<int>(), norm_);
     for (const auto& [k, run] : runs) {
       const Group& g = groups_[k];
       const auto bytes = [](const Tensor& t) { return static_cast<unsigned char*>(Data(t)); };
@@ -268,6 +272,11 @@ class Adamw {
                               max_norm ? norm_.data_ptr<float>() : nullptr, static_cast<float>(max_norm.value_or(0.0))};
       Check(switchml_adamw_step(&tensors_[run.begin], static_cast<int>(run.end - run.begin), &state, &step, run.type, CurrentStream()),
             "FusedAdamW");
+    }
+    for (const Group& g : groups_) {
+      for (const Tensor& p : g.params) {
+        if (p.grad().defined()) p.unsafeGetTensorImpl()->bump_version();
+      }
     }
   }
 
@@ -308,7 +317,9 @@ class Adamw {
   const int bits_;
   const unsigned seed_;
   std::vector<Group> groups_;
-  Tensor ticket_, norm_, workspace_;
+  Tensor ticket_, norm_;
+  std::vector<Tensor> workspaces_;  // the last one is for all groups
+  size_t count_ = 0;                // of all parameters
   std::vector<SmlAdamwTensor> tensors_;
   std::vector<SmlNormTensor> norms_;
 };

@@ -53,6 +53,7 @@ class FusedAdamW(torch.optim.Optimizer):
         self._bits, self._max_norm = state_bits, max_norm
         self._native = _ops().Adamw(state_bits, seed)
         self._buffers = []   # of every group: flat tensors
+        self._steps = []     # of every group: the parameters' counts of steps
         self._values = 0     # in the flat buffers of all groups
         self._device = None
         self._checked = []   # settings that have been found in order
@@ -72,6 +73,9 @@ class FusedAdamW(torch.optim.Optimizer):
             del self.param_groups[first:]
             raise
 
+    def __getstate__(self):
+        raise TypeError("FusedAdamW is neither copied nor pickled: take its state_dict()")
+
     def _check(self, group, device):
         lr, betas = group["lr"], group["betas"]
         if isinstance(lr, torch.Tensor):
@@ -87,6 +91,8 @@ class FusedAdamW(torch.optim.Optimizer):
     def _allocate(self, group):
         params = group["params"]
         device = self._device
+        if not params:
+            raise ValueError("a group has no parameters")
         for p in params:
             if p.dtype not in (torch.float32, torch.bfloat16):
                 raise TypeError("a parameter is %s: float32 or bfloat16 is wanted" % p.dtype)
@@ -95,12 +101,18 @@ class FusedAdamW(torch.optim.Optimizer):
             if not torch.ops.aten.is_non_overlapping_and_dense(p):
                 raise ValueError("a parameter of the shape %s has gaps or overlaps in memory" % (tuple(p.shape),))
             device = p.device
+        # Tensors are taken side by side: two that share memory would be written by both.
+        ends = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size())
+                      for g in self.param_groups for p in g["params"] if p.numel())
+        if any(a[1] > b[0] for a, b in zip(ends, ends[1:])):
+            raise ValueError("two parameters share memory")
         self._check(group, device)
         align = _ops().ALIGN
         places, total = [], 0
         for p in params:
             places.append(total)
             total += -(-p.numel() // align)
+        total = max(total, 1)
         if total >= 1 << 32:
             raise ValueError("a group of %d values is too large" % (total * align))
         values = total * align
@@ -113,7 +125,7 @@ class FusedAdamW(torch.optim.Optimizer):
                     flat[name + "_scale"] = torch.ones(values // _SCALED, dtype=torch.uint8, device=device).view(torch.float8_e8m0fnu)
             if any(p.dtype == torch.bfloat16 for p in params):
                 flat["remainder"] = torch.zeros(values, dtype=torch.int16, device=device)
-            steps = torch.zeros(max(1, len(params)), dtype=torch.int32, device=device)
+            steps = torch.zeros(len(params), dtype=torch.int32, device=device)
             for i, (p, place) in enumerate(zip(params, places)):
                 at, n = place * align, p.numel()
                 state = self.state[p]
@@ -129,6 +141,7 @@ class FusedAdamW(torch.optim.Optimizer):
         self._device = device
         self._values += values
         self._buffers.append(flat)
+        self._steps.append(steps)
 
     def state_buffers(self):
         """What the optimizer keeps, for every group as a dict of few flat tensors (``exp_avg``, ``exp_avg_sq``, their
@@ -199,13 +212,10 @@ class FusedAdamW(torch.optim.Optimizer):
                 self._load(entry, state, name, p, copies)
         if copies[0]:
             torch._foreach_copy_(*copies)
-        at = 0
-        for group in self.param_groups:
-            n = len(group["params"])
-            if n:
-                steps = self.state[group["params"][0]]["step"]._base
-                steps[:n].copy_(torch.tensor(fills[at:at + n], dtype=torch.int32))
-            at += n
+        for steps in self._steps:
+            n = steps.numel()
+            steps.copy_(torch.tensor(fills[:n], dtype=torch.int32))
+            del fills[:n]
 
     def _load(self, entry, state, name, p, copies):
         new, scale = state[name], state.get(name + "_scale")

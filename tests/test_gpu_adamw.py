@@ -40,9 +40,9 @@ def value(opt, p):
 class Checker:
     """A plain optimizer of every parameter beside `opt`."""
 
-    def __init__(self, opt, bits, seed=0):
-        self.opt, self.plain, first = opt, [], 0
-        for group in opt.param_groups:
+    def __init__(self, opt, bits, seed=0, first=0, groups=None):
+        self.opt, self.plain = opt, []
+        for group in groups or opt.param_groups:
             for p in group["params"]:
                 plain = ref.Adamw(p, bits, seed, first)
                 plain.p = value(opt, p).clone()
@@ -101,6 +101,37 @@ def test_only_some_tensors_behind_an_aligned_address(bits, dtype):
         checker = Checker(FusedAdamW(params, state_bits=bits), bits)
         checker.step()
         checker.step()
+
+
+def test_places_beyond_32_bits():
+    """The random bits of values around number 2^32."""
+    opt = FusedAdamW(make([10], F32), state_bits=8, seed=3)
+    opt._values = first = (1 << 32) - 1024
+    params = make([700, 5000, 300], F32, 2)
+    opt.add_param_group({"params": params})
+    checker = Checker(opt, 8, 3, first, opt.param_groups[1:])
+    checker.step()
+    checker.step()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_betas_of_zero(bits):
+    checker = Checker(FusedAdamW(make([100, 3000], F32), betas=(0.0, 0.0), state_bits=bits), bits)
+    checker.step()
+    checker.step()
+
+
+def test_a_second_moment_that_overflows_takes_its_parameter_along():
+    """v = inf while m is finite: in 8 bits the block of v is NaN from then on, and so are the parameters' values."""
+    for dtype in (F32, BF16):
+        p = torch.zeros(64, device="cuda", dtype=dtype, requires_grad=True)
+        p.grad = torch.full_like(p, 1e-3)
+        p.grad[3] = 1e25
+        opt = FusedAdamW([p], state_bits=8, weight_decay=0.0)
+        opt.step()
+        p.grad[3] = 1e-3
+        opt.step()
+        assert p[:32].isnan().all() and not p[32:].isnan().any()
 
 
 @pytest.mark.parametrize("bits", [32, 8])
@@ -339,6 +370,11 @@ def test_state_dict(bits, dtype):
         assert torch.equal(mine.state[q]["exp_avg"], torch_s.state[p]["exp_avg"])
     with pytest.raises(ValueError):
         mine.load_state_dict(FusedAdamW(make([4], F32)).state_dict())
+    for p, q in zip(params, others):
+        q.data.copy_(p.data)
+    other.load_state_dict({"state": {k: {n: t.cpu() for n, t in v.items()} for k, v in opt.state_dict()["state"].items()},
+                           "param_groups": opt.state_dict()["param_groups"]})
+    assert all(torch.equal(a, b) for a, b in zip(once(opt), once(other)))
 
 
 def test_state_of_another_layout_is_put_in_order():
@@ -465,9 +501,15 @@ def test_refusals_on_the_gpu():
     with pytest.raises(RuntimeError, match="another size"):
         opt.step()
     assert torch.equal(opt.state[p]["exp_avg"], before)
-    with pytest.raises(ValueError):
-        opt.add_param_group({"params": [torch.zeros(3)]})
+    flat = torch.zeros(20, device="cuda")
+    for bad in ([torch.zeros(3)], [], [flat[:10].requires_grad_(), flat[9:].requires_grad_()], [p.detach().requires_grad_()]):
+        with pytest.raises(ValueError):
+            opt.add_param_group({"params": bad})
+    with pytest.warns(UserWarning), pytest.raises(ValueError, match="share memory"):
+        FusedAdamW([flat.requires_grad_(), flat])
     assert len(opt.param_groups) == 1
+    with pytest.raises(TypeError):
+        copy.deepcopy(opt)
     p.data, p.grad = torch.zeros(8, device="cuda"), torch.ones(8, device="cuda")
     opt.step()
     assert int(opt.state[p]["step"]) == 1

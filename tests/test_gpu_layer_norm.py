@@ -178,6 +178,42 @@ def test_inputs_that_are_not_contiguous():
     check("dx", torch.autograd.grad(y, x, dev["dy"])[0], values["dx"].reshape(x.shape), bounds["dx"].reshape(x.shape))
 
 
+def test_residual_that_is_the_input_itself():
+    x = torch.randn(6, 320, device="cuda", requires_grad=True)
+    dy = torch.randn(6, 320, device="cuda")
+    y, s = layer_norm(x, residual=x)
+    got, = torch.autograd.grad(y, x, dy)
+    values, bounds = layer_norm64(x.detach().cpu(), x.detach().cpu(), None, None, 1e-5, dy.cpu())
+    check("y", y, values["y"], bounds["y"])
+    check("dx", got, 2 * values["dx"], 2 * bounds["dx"])
+
+
+def test_gradients_of_input_and_residual_are_two_tensors():
+    data, dev = make((6, 320), F32, F32, True, True)
+    x, r = dev["x"].requires_grad_(), dev["residual"].requires_grad_()
+    layer_norm(x, dev["weight"], dev["bias"], residual=r)[0].backward(dev["dy"])
+    kept = r.grad.clone()
+    x.grad.zero_()
+    assert torch.equal(r.grad, kept)
+
+
+@pytest.mark.parametrize("n", [8192, 8200])
+def test_more_values_than_31_bits_count(n):
+    """The last rows of 2^31 and some values, forward and backward, against the formula."""
+    rows = 262150
+    x = torch.empty(rows, n, device="cuda", dtype=BF16).normal_().requires_grad_()
+    w = (1 + 0.1 * torch.randn(n, device="cuda")).requires_grad_()
+    y = layer_norm(x, w)
+    dy = torch.zeros_like(y)
+    dy[-3:] = torch.randn(3, n, device="cuda")
+    dx, dw = torch.autograd.grad(y, [x, w], dy)
+    values, bounds = layer_norm64(x[-3:].detach().cpu(), None, w.detach().cpu(), None, 1e-5, dy[-3:].cpu())
+    check("y", y[-3:], values["y"], bounds["y"])
+    check("dx", dx[-3:], values["dx"], bounds["dx"])
+    check("dweight", dw, values["dweight"], bounds["dweight"])
+    assert not dx[:-3].any()
+
+
 def test_the_same_bits_in_every_run():
     _, dev = make((4099, 1024), BF16, F32, True, True)
     leaves = [dev[k].requires_grad_() for k in ("x", "weight", "bias")]
