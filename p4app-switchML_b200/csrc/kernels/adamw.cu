@@ -3,6 +3,14 @@
 // A launch takes its tensors' addresses and sizes as kernel parameters: nothing has to be copied to the device, a captured
 // launch keeps its own, and two of them share nothing. The parameters' memory is read through the constant cache; a warp
 // finds the tensor of its tile by halving.
+//
+// The step is one pass over memory: 28 bytes per value with fp32 parameters and moments, 16.06 with moments in 8 bits (bf16
+// parameters: 26 and 14.06). A lane takes 8 neighbours, whole sectors of every array; tiles go to the warps in the order of
+// the addresses (blocks that stay and stride over the tiles: 1200 instead of 1096 us). 2^28 values:
+//   fp32, moments in 32 bits 1096 us = 6.86 TB/s, in 8 bits 669 us = 6.47 TB/s; bf16 1043 us = 6.69 and 655 us = 5.79 TB/s
+// (a plain copy: 6.55 TB/s). With 32 bits memory is the limit. With 8 bits it is nearly so: 51 instructions per value, of
+// which hashing takes 9 and each of the two codes 6; one value per lane took 4 times, scalar arithmetic 1.4 times as long. Reading
+// the next block ahead gained 1 % there (bf16: 5 %) and lost as much with 32 bits and on a few million values.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
@@ -446,7 +454,8 @@ __device__ __forceinline__ void Finish(const double* partial, int parts, float* 
 }
 
 // Squares are summed in fp64: 2^-53 of a sum over 10^9 values still leaves the result right to its last fp32 bit, and no
-// gradient's square overflows or vanishes.
+// gradient's square overflows or vanishes. Converting takes 16 values per cycle and SM, where memory brings 6. Bound by reading:
+// 335 M values 205 us = 6.5 TB/s, the 25.6 M of ResNet-50 18.5 us = 5.5 TB/s.
 template <int kMax> __global__ void __launch_bounds__(kNormThreads, 8) NormKernel(const __grid_constant__ NormArgs<kMax> a) {
   WaitForEarlierKernels();
   LetNextKernelStart();
