@@ -393,8 +393,10 @@ __global__ void __launch_bounds__(kThreads) MastersKernel(const __grid_constant_
 }
 
 constexpr int kNormThreads = 256;
-constexpr int kNormBlocks = 148 * 8;  // partial sums of a launch, at most: the blocks that the GPU holds
-constexpr int kNormTile = 4096;       // values that a block takes at once
+// Values that a block takes at once: 4 vectors per thread in flight. ResNet-50's 161 gradients, a bucket's 28 and 301 ragged
+// bf16 ones took 23.6, 7.9 and 11.8 us with 2048, 19.6, 6.6 and 9.1 with 4096, 19.4, 5.8 and 7.9 with 8192.
+constexpr int kNormTile = 8192;
+constexpr int kNormBlocks = 148 * 5;  // partial sums of a launch, at most: the blocks that the GPU holds
 
 template <int kMax> struct NormArgs {
   SmlNormTensor tensor[kMax];
@@ -455,8 +457,8 @@ __device__ __forceinline__ void Finish(const double* partial, int parts, float* 
 
 // Squares are summed in fp64: 2^-53 of a sum over 10^9 values still leaves the result right to its last fp32 bit, and no
 // gradient's square overflows or vanishes. Converting takes 16 values per cycle and SM, where memory brings 6. Bound by reading:
-// 335 M values 205 us = 6.5 TB/s, the 25.6 M of ResNet-50 18.5 us = 5.5 TB/s.
-template <int kMax> __global__ void __launch_bounds__(kNormThreads, 8) NormKernel(const __grid_constant__ NormArgs<kMax> a) {
+// 335 M values 205 us = 6.5 TB/s, the 25.6 M of ResNet-50 19.4 us = 5.3 TB/s.
+template <int kMax> __global__ void __launch_bounds__(kNormThreads, 5) NormKernel(const __grid_constant__ NormArgs<kMax> a) {
   WaitForEarlierKernels();
   LetNextKernelStart();
   double sum = 0.0;
