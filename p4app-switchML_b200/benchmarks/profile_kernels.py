@@ -15,7 +15,9 @@ wgrad_split (the same with K split over two pairs of CTAs per tile, 8192 x 1024 
 wgrad_fc6 (VGG fc6 shape, K = 32: output-bandwidth bound);
 local_copy (what `bench.py --gpus 1` times: a one-worker, out-of-place float_sum allreduce of
 2^26 elements through the Context, i.e. LocalCopyKernel over 256 MiB in and 256 MiB out);
-local_quant (the same in the exact mode: LocalQuantRowsKernel).
+local_quant (the same in the exact mode: LocalQuantRowsKernel);
+layer_norm (ForwardKernel and BackwardKernel, 16384 x 2048 bf16 behind a residual sum);
+adamw / adamw8 (NormKernel and AdamwKernel over 64 tensors of 2^20 float32 values, moments in 32 / 8 bits).
 The plain GEMMs are the kernels WgradWideKernel (one CTA) and WgradPairKernel (two).
 Prints CUDA-event timings.
 """
@@ -69,6 +71,21 @@ def main():
         assert torch.allclose(x, y, rtol=0, atol=2.0 ** -30 if exact else 0.0)  # (blocks below 1: a grid of 2^-31)
         ctx.stop()
         print("%s: %d elements, %.4f ms, %.0f GB/s read+write" % (a.kernel, numel, ms, 2 * numel * 4 / ms / 1e6))
+    elif a.kernel == "layer_norm":
+        from switchml_b200.ops.layer_norm import layer_norm
+        x, r = (torch.randn(16384, 2048, device="cuda").bfloat16().requires_grad_() for _ in range(2))
+        w, b = (torch.randn(2048, device="cuda").requires_grad_() for _ in range(2))
+        dy = torch.randn_like(x)
+        ms = timed(lambda: torch.autograd.grad(layer_norm(x, w, b, residual=r)[0], [x, r, w, b], dy), a.iters)
+        print("layer_norm: 16384 x 2048 bf16, forward and backward, %.4f ms" % ms)
+    elif a.kernel.startswith("adamw"):
+        from switchml_b200.ops.adamw import FusedAdamW
+        params = [torch.randn(1 << 20, device="cuda").requires_grad_() for _ in range(64)]
+        for p in params:
+            p.grad = torch.randn_like(p)
+        optimizer = FusedAdamW(params, state_bits=8 if a.kernel == "adamw8" else 32, max_norm=1.0)
+        ms = timed(optimizer.step, a.iters)
+        print("%s: 2^26 values, %.4f ms" % (a.kernel, ms))
     elif a.kernel.startswith("allreduce"):
         from switchml_b200.ops.emulation import emulated_allreduce
         numel = 1 << a.log2_numel
