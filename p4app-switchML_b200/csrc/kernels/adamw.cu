@@ -105,12 +105,17 @@ __device__ __forceinline__ unsigned HashedAt(const StepFactors& a, const Factors
   return static_cast<unsigned>(value) + Mix(f.key + static_cast<unsigned>(value >> 32));
 }
 
-// The fp32 value of a parameter, and back.
-__device__ __forceinline__ float WithRemainder(unsigned param, unsigned remainder) {  // 16 bits each
-  return __uint_as_float((param << 16) + static_cast<unsigned>(static_cast<int>(static_cast<short>(remainder))));
+// The fp32 values of two parameters with their remainders: parameter << 16 plus the signed remainder, which is the unsigned
+// remainder + 0x8000 less 0x8000.
+__device__ __forceinline__ Pair WithRemainders(unsigned params, unsigned remainders) {
+  remainders ^= 0x80008000u;
+  return Pair(__uint_as_float(__byte_perm(params, remainders, 0x1054) - 0x8000u),
+              __uint_as_float(__byte_perm(params, remainders, 0x3276) - 0x8000u));
 }
-__device__ __forceinline__ unsigned PlusHalf(float p) {  // the parameter is the high half, the remainder the low half ^ 0x8000
-  return (isnan(p) ? 0x7fc00000u : __float_as_uint(p)) + 0x8000u;
+// Back: the parameter is the high half of this, the remainder the low half ^ 0x8000. (Arithmetic makes 0x7fffffff of every NaN:
+// that one would wrap around.)
+__device__ __forceinline__ unsigned PlusHalf(float p) {
+  return static_cast<unsigned>(min(static_cast<int>(__float_as_uint(p)), 0x7fff7fff)) + 0x8000u;
 }
 
 // The root and the reciprocal of an update come from the SM's approximations (2^-23 and 2^-23 of the result, by the PTX
@@ -245,7 +250,7 @@ __device__ __forceinline__ void StepBlock(const StepFactors& a, const SmlAdamwTe
     }
     Pair pf(p.At(2 * i), p.At(2 * i + 1));
     if constexpr (sizeof(T) == 2)
-      pf = Pair(WithRemainder(p.w[i] & 0xffff, r.w[i]), WithRemainder(p.w[i] >> 16, r.w[i] >> 16));
+      pf = WithRemainders(p.w[i], r.w[i]);
     Update(a, f, clip, Pair(g.At(2 * i), g.At(2 * i + 1)), &pf, &mf[i], &vf[i]);
     const float2 both = pf.Both();
     if constexpr (sizeof(T) == 2) {
@@ -382,8 +387,8 @@ __global__ void __launch_bounds__(kThreads) MastersKernel(const __grid_constant_
       LoadWords(a.remainder + state + k, r.w);
 #pragma unroll
       for (int u = 0; u < 4; u++) {
-        out.w[2 * u] = __float_as_uint(WithRemainder(p.w[u] & 0xffff, r.w[u]));
-        out.w[2 * u + 1] = __float_as_uint(WithRemainder(p.w[u] >> 16, r.w[u] >> 16));
+        const float2 both = WithRemainders(p.w[u], r.w[u]).Both();
+        out.w[2 * u] = __float_as_uint(both.x), out.w[2 * u + 1] = __float_as_uint(both.y);
       }
     } else {
       out = p;
