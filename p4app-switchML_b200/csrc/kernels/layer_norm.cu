@@ -74,13 +74,14 @@ template <int kLanes> struct Group {
   }
   // The first value of this thread's.
   __device__ __forceinline__ int First(int held, int vec) const { return warp * 32 * held + lane * vec; }
-  // The sum over the group, in all its threads. Two calls that follow each other take different `part`s (a V for each warp of the block): between
-  // two uses of the same one lies the other's barrier.
+  // The sum over the group, in all its threads. Two calls that follow each other take different `part`s (a V for each warp
+  // of the block): between two uses of the same one lies the other's barrier.
   template <class V> __device__ __forceinline__ V Sum(V v, V* part) const {
 #pragma unroll
     for (int o = kLanes / 2; o; o >>= 1) v = Plus(v, Shuffle(v, o));
     if (kLanes == 32 && warps > 1) {
       if (lane == 0) part[number * warps + warp] = v;
+      __syncwarp();  // (bar.sync wants the warp's threads together)
       asm volatile("bar.sync %0, %1;" ::"r"(number + 1), "r"(warps * 32) : "memory");
       v = lane < warps ? part[number * warps + lane] : V{};
       for (int o = warps > 16 ? 16 : warps > 8 ? 8 : warps > 4 ? 4 : warps > 2 ? 2 : 1; o; o >>= 1) v = Plus(v, Shuffle(v, o));
@@ -349,11 +350,10 @@ BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const f
     N c1(0.f), c2(0.f), xhat[kVectors][kNums], g[kVectors][kNums];
 #pragma unroll
     for (int j = 0; j < kVectors; j++) {
-      if constexpr (!kKeepWeight) {
-        if (kWhole || j * kStep < left) LoadParameter<kVec, W>(weight, column + j * kStep, 1.f, w[j]);
-      }
+      if (!kWhole && j * kStep >= left) continue;  // (what is not there has gradients of 0, but 0 times infinity is NaN)
+      if constexpr (!kKeepWeight) LoadParameter<kVec, W>(weight, column + j * kStep, 1.f, w[j]);
 #pragma unroll
-      for (int i = 0; i < kNums; i++) {  // (what is not there has gradients of 0)
+      for (int i = 0; i < kNums; i++) {
         const N dyi = d[j].At(i);
         xhat[j][i] = (v[j].At(i) + N(-mean)) * N(r);
         g[j][i] = dyi * w[j][i];
@@ -377,10 +377,11 @@ BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const f
     const auto store = [&](auto plus) {
 #pragma unroll
       for (int j = 0; j < kVectors; j++) {
+        if (!kWhole && j * kStep >= left) continue;
         Vector<T, kVec> out;
 #pragma unroll
         for (int i = 0; i < kNums; i++) out.Set(i, plus(Fma(xhat[j][i], minus_c2, g[j][i] + minus_c1) * N(r), j, i));
-        if (kWhole || j * kStep < left) out.Store(dx + at + j * kStep);
+        out.Store(dx + at + j * kStep);
       }
     };
     if (dsum) {

@@ -115,6 +115,20 @@ def test_rows_without_spread():
     assert torch.isfinite(dx).all()
 
 
+@pytest.mark.parametrize("n", [96, 100, 101, 1000, 1001, 6600])
+def test_large_rows_without_spread(n):
+    """2^112 everywhere: centred values are 0, but what lies behind a row's end, taken as 0, would be infinitely far from the mean."""
+    x = torch.full((5, n), 2.0 ** 112, device="cuda", requires_grad=True)
+    w, dy = (1 + torch.rand(n)).requires_grad_(), torch.randn(5, n)
+    y = layer_norm(x, w.cuda(), None, 1e-12)
+    dx, = torch.autograd.grad(y, x, dy.cuda())
+    assert not y.any()
+    g = dy.double() * w.detach().double()
+    want = 1e6 * (g - g.mean(1, keepdim=True))
+    bound = 1e6 * 2.0 ** -24 * (n / 32 + 24) * (g.abs() + g.abs().mean(1, keepdim=True))
+    check("dx", dx, want, bound)
+
+
 def test_values_that_are_not_finite_stay_in_their_row():
     data, dev = make((6, 1024), BF16, F32, False, True)
     dev["x"][2, 5], dev["x"][4, 1000] = float("nan"), float("inf")
