@@ -225,6 +225,7 @@ Tensor GradNorm(const py::list& tensors) {
 struct Group {
   std::vector<Tensor> params;
   std::vector<int64_t> numel, place;  // place: in units of SML_ADAMW_ALIGN values
+  std::vector<at::ScalarType> type;
   Tensor exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, remainder, steps;
   int64_t first = 0;
 };
@@ -236,7 +237,7 @@ class Adamw {
   void AddGroup(std::vector<Tensor> params, std::vector<int64_t> place, Tensor exp_avg, Tensor exp_avg_sq, OptTensor exp_avg_scale,
                 OptTensor exp_avg_sq_scale, OptTensor remainder, Tensor steps, int64_t first) {
     Group g;
-    for (const Tensor& p : params) g.numel.push_back(p.numel());
+    for (const Tensor& p : params) g.numel.push_back(p.numel()), g.type.push_back(p.scalar_type());
     g.params = std::move(params), g.place = std::move(place);
     g.exp_avg = std::move(exp_avg), g.exp_avg_sq = std::move(exp_avg_sq), g.steps = std::move(steps), g.first = first;
     g.exp_avg_scale = exp_avg_scale.value_or(Tensor()), g.exp_avg_sq_scale = exp_avg_sq_scale.value_or(Tensor());
@@ -266,10 +267,11 @@ class Adamw {
         const size_t begin = tensors_.size();
         for (size_t i = 0; i < g.params.size(); i++) {
           const Tensor& p = g.params[i];
-          if (AdamwType(p) != type) continue;
+          if (TypeOf(g, i) != type) continue;
           Tensor grad = p.grad();
           if (!grad.defined()) continue;
-          CheckGrad(p, grad, g.numel[i]);
+          CheckParam(g, i);
+          CheckGrad(p, grad);
           if (!(p.is_contiguous() && grad.is_contiguous()) && p.strides() != grad.strides()) {
             grad = at::empty_strided(p.sizes(), p.strides(), grad.options()).copy_(grad);
             keep.push_back(grad);
@@ -307,8 +309,8 @@ class Adamw {
     for (const int type : {SML_ADAMW_F32, SML_ADAMW_BF16}) {
       tensors_.clear();
       for (size_t i = 0; i < g.params.size(); i++) {
-        CheckParam(g.params[i], g.numel[i]);
-        if (AdamwType(g.params[i]) == type)
+        CheckParam(g, i);
+        if (TypeOf(g, i) == type)
           tensors_.push_back({Data(g.params[i]), nullptr, g.numel[i], static_cast<unsigned>(g.place[i]), static_cast<int>(i)});
       }
       if (tensors_.empty()) continue;
@@ -322,15 +324,18 @@ class Adamw {
   Tensor norm() const { return norm_; }
 
  private:
-  static void CheckParam(const Tensor& p, int64_t numel) {
-    TORCH_CHECK(p.numel() == numel && Dense(p), "FusedAdamW: a parameter has another size or other strides than when its state was made");
+  static int TypeOf(const Group& g, size_t i) { return g.type[i] == at::kFloat ? SML_ADAMW_F32 : SML_ADAMW_BF16; }
+  // What a parameter's storage has become: p.data may have been exchanged.
+  void CheckParam(const Group& g, size_t i) const {
+    const Tensor& p = g.params[i];
+    TORCH_CHECK(p.numel() == g.numel[i] && Dense(p) && p.scalar_type() == g.type[i] && p.device() == ticket_.device(),
+                "FusedAdamW: a parameter has another size, type or device than when its state was made, or gaps in memory");
   }
-  static void CheckGrad(const Tensor& p, const Tensor& grad, int64_t numel) {
+  static void CheckGrad(const Tensor& p, const Tensor& grad) {
     TORCH_CHECK(grad.layout() == at::kStrided, "FusedAdamW: a gradient is ", grad.layout(), ": strided is wanted");
     TORCH_CHECK(grad.scalar_type() == p.scalar_type() && grad.device() == p.device() && grad.sizes() == p.sizes(),
                 "FusedAdamW: a parameter is ", p.scalar_type(), " ", p.sizes(), " on ", p.device(), ", its gradient ", grad.scalar_type(), " ",
                 grad.sizes(), " on ", grad.device());
-    CheckParam(p, numel);
   }
 
   const int bits_;

@@ -500,6 +500,20 @@ def test_refusals_on_the_gpu():
     p.grad = torch.zeros(9, device="cuda")
     with pytest.raises(RuntimeError, match="another size"):
         opt.step()
+    p.grad = None
+    p.data = torch.zeros(8)
+    p.grad = torch.ones(8)
+    with pytest.raises(RuntimeError, match="another size, type or device"):
+        opt.step()
+    with pytest.raises(RuntimeError, match="another size, type or device"):
+        opt.master_buffers()
+    p.grad = None
+    p.data = torch.zeros(8, device="cuda", dtype=torch.float16)
+    p.grad = torch.ones_like(p)
+    with pytest.raises(RuntimeError, match="another size, type or device"):
+        opt.step()
+    p.grad = None
+    p.data = torch.zeros(8, device="cuda")
     assert torch.equal(opt.state[p]["exp_avg"], before)
     flat = torch.zeros(20, device="cuda")
     for bad in ([torch.zeros(3)], [], [flat[:10].requires_grad_(), flat[9:].requires_grad_()], [p.detach().requires_grad_()]):
