@@ -5,7 +5,7 @@
  *   m  = m * beta1 + g' * (1 - beta1)
  *   v  = v * beta2 + (g' * (1 - beta2)) * g'
  *   p  = p * (1 - lr * decay) - lr / (1 - beta1^t) * (m / (sqrt(v) / sqrt(1 - beta2^t) + eps))
- * (the line for p may be a few units in the last place of its second term off).
+ * (the line for p may be a few units in the last place of its second term off, and a v below 2^-126 counts as 2^-126 there).
  *
  * Moments are fp32 or take 8 bits each. Then 32 values share a scale 2^(e - 134), stored as the byte e - 7 (e8m0), where
  * e is the exponent field of the largest magnitude among the 32, at least 8; the largest of them comes to lie in
