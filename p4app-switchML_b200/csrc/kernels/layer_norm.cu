@@ -57,35 +57,70 @@ __device__ __forceinline__ float WarpSum(float v) {
 
 // ---- rows that stay in registers ----
 //
-// A group of threads holds a row: 8 lanes of a warp, or 1 to 24 whole warps. Each lane has kHeld values: kHeld / kVec
-// vectors of kVec neighbours, between which lie kLanes (8 or 32) * kVec values, so that addresses differ by constants; warp w
-// has the values from w * 32 * kHeld on. kVec is what the addresses and the length of the rows allow: 16 bytes of them, 2 or 1.
-// Groups go through their rows by themselves, and warps of a group meet at a barrier of their own.
+// A group of threads holds a row: 8 lanes of a warp, 1 to 24 whole warps, or 16 warps of each of 2, 4 or 8 blocks of a cluster. Each
+// lane has kHeld values in vectors of kVec neighbours, between which lie kLanes (8 or 32) * kVec values, so that addresses
+// differ by constants; warp w has the values from w * 32 * kHeld on. kVec is what the addresses and the length of the rows
+// allow: 16 bytes of them, 2, or 1, of which two that are kLanes apart make a vector. Groups go through their rows by
+// themselves, and warps of a group meet at a barrier of their own.
 
-template <int kLanes> struct Group {
-  int number, warps, lane, warp;  // number: in the block; warps: of a group; lane, warp: in the group
+// Whether a warp looks if all its columns exist, to leave out the questions where they do. Single values ask twice as often as
+// vectors (forward and backward, bf16, with and without: 20000 x 5001 220 and 236, 298 and 311 us; 16384 x 2047 71 and 72, 101 and
+// 106; the one loss found is 16384 x 2047 fp32, backward, 110 and 99), and in a cluster's long rows most warps are whole (backward,
+// 8192 x 12000 fp32: 416 and 470). Elsewhere the second copy of the code costs more (16384 x 2046 bf16, forward: 61 and 55).
+__host__ __device__ constexpr bool WarpAsks(int vec, bool split) { return vec == 1 || split; }
+
+__device__ __forceinline__ uint32_t SharedAddress(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+template <int kLanes, bool kSplit> struct Group {  // kSplit: over the blocks of a cluster
+  int number, warps, ranks, lane, warp;  // number: in the block; warps: of a group in a block; ranks: blocks of a group; lane, warp: in the group
   unsigned mask;
-  __device__ __forceinline__ explicit Group(int warps_of_group) : warps(warps_of_group) {
+  __device__ __forceinline__ Group(int warps_of_group, int blocks_of_group) : warps(warps_of_group), ranks(kSplit ? blocks_of_group : 1) {
     const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
     lane = l % kLanes;
     mask = kLanes == 32 ? 0xffffffffu : ((1u << kLanes % 32) - 1) << (l - lane);
     number = kLanes == 32 ? w / warps : threadIdx.x / kLanes;
-    warp = kLanes == 32 ? w - number * warps : 0;
+    warp = kLanes == 32 ? w - number * warps + Rank() * warps : 0;
   }
+  // Of this block among those of the group.
+  __device__ __forceinline__ int Rank() const { return kSplit ? static_cast<int>(blockIdx.x) % ranks : 0; }
   // The first value of this thread's.
   __device__ __forceinline__ int First(int held, int vec) const { return warp * 32 * held + lane * vec; }
+  // Whether all values of this warp's exist in a row of n.
+  __device__ __forceinline__ bool Whole(int held, int n) const { return kLanes == 32 && (warp + 1) * 32 * held <= n; }
+  // Row of the first turn, and the distance to the next.
+  __device__ __forceinline__ long long FirstRow(int groups) const { return static_cast<long long>(kSplit ? blockIdx.x / ranks : blockIdx.x) * groups + number; }
+  __device__ __forceinline__ long long Stride(int groups) const { return static_cast<long long>(kSplit ? gridDim.x / ranks : gridDim.x) * groups; }
+  // Before the first Sum: the blocks of a group are there.
+  __device__ __forceinline__ void Meet() const {
+    if constexpr (kSplit) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
   // The sum over the group, in all its threads. Two calls that follow each other take different `part`s (a V for each warp
-  // of the block): between two uses of the same one lies the other's barrier.
-  template <class V> __device__ __forceinline__ V Sum(V v, V* part) const {
+  // of the block) and `across` (a float2 for each block): between two uses of the same one lies the other's barrier.
+  template <class V> __device__ __forceinline__ V Sum(V v, V* part, float2* across) const {
 #pragma unroll
     for (int o = kLanes / 2; o; o >>= 1) v = Plus(v, Shuffle(v, o));
     if (kLanes == 32 && warps > 1) {
-      if (lane == 0) part[number * warps + warp] = v;
+      const int first = number * warps;
+      if (lane == 0) part[threadIdx.x >> 5] = v;
       __syncwarp();  // (bar.sync wants the warp's threads together)
       asm volatile("bar.sync %0, %1;" ::"r"(number + 1), "r"(warps * 32) : "memory");
-      v = lane < warps ? part[number * warps + lane] : V{};
+      v = lane < warps ? part[first + lane] : V{};
       for (int o = warps > 16 ? 16 : warps > 8 ? 8 : warps > 4 ? 4 : warps > 2 ? 2 : 1; o; o >>= 1) v = Plus(v, Shuffle(v, o));
       v = Broadcast(v);
+      if constexpr (kSplit) {
+        if (threadIdx.x < ranks) {  // thread r tells block r
+          const uint32_t mine = SharedAddress(across + Rank());
+          const float2 both = Both(v);
+          uint32_t to;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(mine), "r"(threadIdx.x));
+          asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(both.x), "f"(both.y) : "memory");
+        }
+        __syncwarp();
+        Meet();
+        float2 all = make_float2(0.f, 0.f);
+        for (int r = 0; r < ranks; r++) all = Plus(all, across[r]);
+        Set(all, &v);
+      }
     }
     return v;
   }
@@ -95,117 +130,141 @@ template <int kLanes> struct Group {
   __device__ __forceinline__ float2 Broadcast(float2 v) const { return make_float2(Broadcast(v.x), Broadcast(v.y)); }
   static __device__ __forceinline__ float Plus(float a, float b) { return a + b; }
   static __device__ __forceinline__ float2 Plus(float2 a, float2 b) { return make_float2(a.x + b.x, a.y + b.y); }
+  static __device__ __forceinline__ float2 Both(float v) { return make_float2(v, 0.f); }
+  static __device__ __forceinline__ float2 Both(float2 v) { return v; }
+  static __device__ __forceinline__ void Set(float2 from, float* to) { *to = from.x; }
+  static __device__ __forceinline__ void Set(float2 from, float2* to) { *to = from; }
 };
 
 // Values of 16 bytes: what a thread reads at once where addresses and the length of the rows allow it.
 template <class T> constexpr int kWide = 16 / sizeof(T);
 
-// What arithmetic takes at once of a vector's values: two of them, where there are two.
-template <int kVec> using Num = std::conditional_t<kVec == 1, float, Pair>;
-
-// kVec values of type T in registers, as kVec / 2 pairs or as the one that it is.
-template <class T, int kVec> struct Vector {
-  static constexpr int kWords = kVec * sizeof(T) / 4;  // 0: half a word
-  static constexpr int kNums = kVec == 1 ? 1 : kVec / 2;
-  unsigned w[kWords ? kWords : 1];
+// Pairs of values of type T in registers, as they lie in memory: kVec neighbours, or with kVec = 1 two values that are kLanes apart.
+// `left`: columns from the vector's first one to the end of the row.
+template <class T, int kVec, int kLanes> struct Vector {
+  static constexpr int kNums = kVec == 1 ? 1 : kVec / 2;        // pairs
+  static constexpr int kStep = kLanes * (kVec == 1 ? 2 : kVec);  // columns from one of a thread's vectors to the next
+  static constexpr int kWords = kNums * 2 * sizeof(T) / 4;
+  unsigned w[kWords];
   __device__ __forceinline__ void Load(const T* from) {
-    if constexpr (kWords) LoadWords(from, w);
-    else w[0] = *reinterpret_cast<const unsigned short*>(from);
+    if constexpr (kVec > 1) LoadWords(from, w);
+    else LoadSome(from, 2 * kLanes);
   }
-  __device__ __forceinline__ void Store(T* to) const {
-    if constexpr (kWords) StoreWords(to, w);
-    else *reinterpret_cast<unsigned short*>(to) = static_cast<unsigned short>(w[0]);
+  __device__ __forceinline__ void LoadSome(const T* from, int left) {  // zeros where nothing is there
+    if constexpr (kVec > 1) {
+      switchml::kernels::LoadWordsIf(left, from, w);
+    } else if constexpr (sizeof(T) == 4) {
+      unsigned x[1], y[1];
+      switchml::kernels::LoadWordsIf(left, from, x);
+      switchml::kernels::LoadWordsIf(left - kLanes, from + kLanes, y);
+      w[0] = x[0], w[1] = y[0];
+    } else {
+      asm volatile("{.reg .pred p, q; .reg .b16 x, y; mov.b16 x, 0; mov.b16 y, 0; setp.gt.s32 p, %2, 0; setp.gt.s32 q, %2, %3;"
+                   "@p ld.global.b16 x, [%1]; @q ld.global.b16 y, [%1 + %4]; mov.b32 %0, {x, y};}"
+                   : "=r"(w[0]) : "l"(from), "r"(left), "n"(kLanes), "n"(kLanes * 2));
+    }
+  }
+  template <bool kWhole> __device__ __forceinline__ void Store(T* to, int left) const {
+    if constexpr (kVec > 1) {
+      if (kWhole || left > 0) StoreWords(to, w);
+    } else {
+      if constexpr (sizeof(T) == 4) {
+        if (kWhole || left > 0) *reinterpret_cast<unsigned*>(to) = w[0];
+        if (kWhole || left > kLanes) *reinterpret_cast<unsigned*>(to + kLanes) = w[1];
+      } else {
+        if (kWhole || left > 0) *reinterpret_cast<unsigned short*>(to) = static_cast<unsigned short>(w[0]);
+        if (kWhole || left > kLanes) *reinterpret_cast<unsigned short*>(to + kLanes) = static_cast<unsigned short>(w[0] >> 16);
+      }
+    }
   }
   __device__ __forceinline__ void LoadShared(const uint4* from) {  // 16 bytes
     const uint4 v = *from;
     w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
   }
-  __device__ __forceinline__ void LoadIf(bool there, const T* from) {
-    if constexpr (kWords) switchml::kernels::LoadWordsIf(there, from, w);
-    else asm volatile("{.reg .pred p; .reg .b16 h; mov.b16 h, 0; setp.ne.b32 p, %2, 0; @p ld.global.b16 h, [%1]; cvt.u32.u16 %0, h;}"
-                      : "=r"(w[0]) : "l"(from), "r"(static_cast<int>(there)));
-  }
-  __device__ __forceinline__ Num<kVec> At(int i) const {
-    if constexpr (kVec == 1) return __uint_as_float(sizeof(T) == 4 ? w[0] : w[0] << 16);
-    else if constexpr (sizeof(T) == 4) return Pair(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+  __device__ __forceinline__ Pair At(int i) const {
+    if constexpr (sizeof(T) == 4) return Pair(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
     else return Pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
   }
-  __device__ __forceinline__ void Set(int i, Num<kVec> v) {
-    if constexpr (kVec == 1) {
-      w[0] = sizeof(T) == 4 ? __float_as_uint(v) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
+  __device__ __forceinline__ void Set(int i, Pair v) {
+    const float2 both = v.Both();
+    if constexpr (sizeof(T) == 4) {
+      w[2 * i] = __float_as_uint(both.x), w[2 * i + 1] = __float_as_uint(both.y);
     } else {
-      const float2 both = v.Both();
-      if constexpr (sizeof(T) == 4) {
-        w[2 * i] = __float_as_uint(both.x), w[2 * i + 1] = __float_as_uint(both.y);
-      } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(both.x, both.y);
-        w[i] = *reinterpret_cast<const unsigned*>(&h);
-      }
+      const __nv_bfloat162 h = __floats2bfloat162_rn(both.x, both.y);
+      w[i] = *reinterpret_cast<const unsigned*>(&h);
     }
+  }
+  // A pair of which what does not exist is 0.
+  template <bool kWhole> static __device__ __forceinline__ Pair There(Pair v, int left) {
+    if constexpr (kWhole || kVec > 1) return v;  // (vectors of neighbours exist or do not)
+    const float2 both = v.Both();
+    return Pair(both.x, left > kLanes ? both.y : 0.f);
   }
 };
 
-// kVec values of weight or bias. W: their type where that is known (and both are there), else void. (To find out for every
+// Weight or bias of a vector's columns. W: their type where that is known (and both are there), else void. (To find out for every
 // vector which of three values it is costs as much as the rest of the forward pass.)
-template <int kVec, class W>
-__device__ __forceinline__ void LoadParameter(const Parameter& p, int i, float none, Num<kVec> (&out)[Vector<float, kVec>::kNums]) {
-  constexpr int kNums = Vector<float, kVec>::kNums;
-  if constexpr (!std::is_void_v<W>) {
-    Vector<W, kVec> v;
-    v.Load(static_cast<const W*>(p.data) + i);
+template <int kVec, int kLanes, bool kWhole, class W>
+__device__ __forceinline__ void LoadParameter(const Parameter& p, int i, int left, float none, Pair (&out)[Vector<float, kVec, kLanes>::kNums]) {
+  constexpr int kNums = Vector<float, kVec, kLanes>::kNums;
+  const auto load = [&](auto type) {
+    Vector<decltype(type), kVec, kLanes> v;
+    const auto* from = static_cast<const decltype(type)*>(p.data) + i;
+    if constexpr (kWhole) v.Load(from);
+    else v.LoadSome(from, left);
 #pragma unroll
     for (int k = 0; k < kNums; k++) out[k] = v.At(k);
+  };
+  if constexpr (!std::is_void_v<W>) {
+    load(W{});
   } else if (!p.data) {
 #pragma unroll
-    for (int k = 0; k < kNums; k++) out[k] = Num<kVec>(none);
+    for (int k = 0; k < kNums; k++) out[k] = Pair(none);
   } else if (p.type == SML_NORM_F32) {
-    Vector<float, kVec> v;
-    v.Load(static_cast<const float*>(p.data) + i);
-#pragma unroll
-    for (int k = 0; k < kNums; k++) out[k] = v.At(k);
+    load(float{});
   } else {
-    Vector<__nv_bfloat16, kVec> v;
-    v.Load(static_cast<const __nv_bfloat16*>(p.data) + i);
-#pragma unroll
-    for (int k = 0; k < kNums; k++) out[k] = v.At(k);
+    load(__nv_bfloat16{});
   }
 }
 
 // One pass: a row is read once, statistics and result come out of registers. Bound by memory: 16384 x 8192 bf16 with a residual,
 // 1.07 GB, 162 us = 6.6 TB/s; 8192 x 1024, 67 MB, 13.3 us, where a copy of as many bytes takes 12.2 (most of the difference is
-// that 8192 rows make 1.7 times the warps that the GPU holds). Ragged rows pay for single loads: 4099 x 1021, 34 MB, 16 us.
+// that 8192 rows make 1.7 times the warps that the GPU holds). Rows at odd addresses take a load per value: 4099 x 1021, 34 MB,
+// 12 us, 16384 x 2047, 268 MB, 71 us. Rows of a cluster: 8192 x 12000 fp32 396 us (read three times by a block each: 588).
 // 32 bf16 values per lane instead of 16 save half the sums over lanes (8192 x 4096: 45 instead of 57 us); 16 fp32 values are
 // as many bytes.
 //
-// Values that a thread holds. kWhole: the row is exactly what its threads hold, nothing has to be asked.
+// Values that a thread holds. kWhole: the row is exactly what its threads hold.
 __host__ __device__ constexpr int ForwardHeld(int vec, int size) { return vec == 8 ? 32 : 16; }
 
-template <class T, int kVec, int kLanes, bool kWhole, class W>
-__global__ void __launch_bounds__(512, 2)
-ForwardKernel(const T* x, const T* residual, Parameter weight, Parameter bias, T* y, T* sum, float* mean_out, float* rstd_out,
-              long long rows, int n, float eps, int groups, int warps) {
-  using N = Num<kVec>;
-  constexpr int kHeld = ForwardHeld(kVec, sizeof(T)), kVectors = kHeld / kVec, kNums = Vector<T, kVec>::kNums, kStep = kLanes * kVec;
-  __shared__ float part[2][16];
-  const Group<kLanes> group(warps);
-  const int column = group.First(kHeld, kVec), left = n - column;  // vector j is there where j * kStep < left
-  WaitForEarlierKernels();
-  for (long long row = static_cast<long long>(blockIdx.x) * groups + group.number; row < rows;
-       row += static_cast<long long>(gridDim.x) * groups) {
+template <class T, int kVec, int kLanes, bool kWhole, bool kSplit, class W>
+__device__ __forceinline__ void ForwardRows(const T* x, const T* residual, const Parameter& weight, const Parameter& bias, T* y, T* sum,
+                                            float* mean_out, float* rstd_out, long long rows, int n, float eps, int groups,
+                                            const Group<kLanes, kSplit>& group, float (*part)[16], float2 (*across)[8]) {
+  using V = Vector<T, kVec, kLanes>;
+  constexpr int kHeld = ForwardHeld(kVec, sizeof(T)), kNums = V::kNums, kVectors = kHeld / (2 * kNums), kStep = V::kStep;
+  const int column = group.First(kHeld, kVec), left = n - column;
+  for (long long row = group.FirstRow(groups), stride = group.Stride(groups); row < rows; row += stride) {
     const long long at = row * n + column;
-    N s[kVectors][kNums];
+    Pair s[kVectors][kNums];
     {
-      Vector<T, kVec> raw[kVectors], more[kVectors];
+      V raw[kVectors], more[kVectors];
 #pragma unroll
-      for (int j = 0; j < kVectors; j++) raw[j].LoadIf(kWhole || j * kStep < left, x + at + j * kStep);
+      for (int j = 0; j < kVectors; j++) {
+        if constexpr (kWhole) raw[j].Load(x + at + j * kStep);
+        else raw[j].LoadSome(x + at + j * kStep, left - j * kStep);
+      }
       if (residual) {
 #pragma unroll
-        for (int j = 0; j < kVectors; j++) more[j].LoadIf(kWhole || j * kStep < left, residual + at + j * kStep);
+        for (int j = 0; j < kVectors; j++) {
+          if constexpr (kWhole) more[j].Load(residual + at + j * kStep);
+          else more[j].LoadSome(residual + at + j * kStep, left - j * kStep);
+        }
 #pragma unroll
         for (int j = 0; j < kVectors; j++) {
 #pragma unroll
           for (int i = 0; i < kNums; i++) raw[j].Set(i, raw[j].At(i) + more[j].At(i));
-          if (kWhole || j * kStep < left) raw[j].Store(sum + at + j * kStep);
+          raw[j].template Store<kWhole>(sum + at + j * kStep, left - j * kStep);
         }
       }
 #pragma unroll
@@ -214,43 +273,60 @@ ForwardKernel(const T* x, const T* residual, Parameter weight, Parameter bias, T
         for (int i = 0; i < kNums; i++) s[j][i] = raw[j].At(i);
       }
     }
-    N total(0.f);
+    Pair total(0.f);
 #pragma unroll
     for (int j = 0; j < kVectors; j++) {
 #pragma unroll
       for (int i = 0; i < kNums; i++) total = total + s[j][i];
     }
-    const float mean = group.Sum(Sum(total), part[0]) / n;
-    N squares(0.f);
+    const float mean = group.Sum(Sum(total), part[0], across[0]) / n;
+    Pair squares(0.f);
 #pragma unroll
     for (int j = 0; j < kVectors; j++) {
+      if (!kWhole && j * kStep >= left) continue;
 #pragma unroll
       for (int i = 0; i < kNums; i++) {
-        s[j][i] = s[j][i] + N(-mean);
-        if (kWhole || j * kStep < left) squares = Fma(s[j][i], s[j][i], squares);
+        s[j][i] = V::template There<kWhole>(s[j][i] + Pair(-mean), left - j * kStep);
+        squares = Fma(s[j][i], s[j][i], squares);
       }
     }
-    const float rstd = 1.f / sqrtf(group.Sum(Sum(squares), part[1]) / n + eps);
+    const float rstd = 1.f / sqrtf(group.Sum(Sum(squares), part[1], across[1]) / n + eps);
 #pragma unroll
     for (int j = 0; j < kVectors; j++) {
-      if (kWhole || j * kStep < left) {
-        N w[kNums], b[kNums];
-        LoadParameter<kVec, W>(weight, column + j * kStep, 1.f, w);
-        LoadParameter<kVec, W>(bias, column + j * kStep, 0.f, b);
-        Vector<T, kVec> out;
+      if (!kWhole && j * kStep >= left) continue;
+      Pair w[kNums], b[kNums];
+      LoadParameter<kVec, kLanes, kWhole, W>(weight, column + j * kStep, left - j * kStep, 1.f, w);
+      LoadParameter<kVec, kLanes, kWhole, W>(bias, column + j * kStep, left - j * kStep, 0.f, b);
+      V out;
 #pragma unroll
-        for (int i = 0; i < kNums; i++) out.Set(i, Fma(s[j][i] * N(rstd), w[i], b[i]));
-        out.Store(y + at + j * kStep);
-      }
+      for (int i = 0; i < kNums; i++) out.Set(i, Fma(s[j][i] * Pair(rstd), w[i], b[i]));
+      out.template Store<kWhole>(y + at + j * kStep, left - j * kStep);
     }
     if (column == 0 && mean_out) mean_out[row] = mean, rstd_out[row] = rstd;
   }
 }
 
+template <class T, int kVec, int kLanes, bool kWhole, bool kSplit, class W>
+__global__ void __launch_bounds__(512, 2)
+ForwardKernel(const T* x, const T* residual, Parameter weight, Parameter bias, T* y, T* sum, float* mean_out, float* rstd_out,
+              long long rows, int n, float eps, int groups, int warps, int ranks) {
+  __shared__ float part[2][16];
+  __shared__ float2 across[2][8];
+  const Group<kLanes, kSplit> group(warps, ranks);
+  WaitForEarlierKernels();
+  group.Meet();
+  if (kWhole || (WarpAsks(kVec, kSplit) && group.Whole(ForwardHeld(kVec, sizeof(T)), n)))
+    ForwardRows<T, kVec, kLanes, true, kSplit, W>(x, residual, weight, bias, y, sum, mean_out, rstd_out, rows, n, eps, groups, group, part, across);
+  else
+    ForwardRows<T, kVec, kLanes, false, kSplit, W>(x, residual, weight, bias, y, sum, mean_out, rstd_out, rows, n, eps, groups, group, part, across);
+}
+
 // The backward pass of rows that a group holds, and the sums over the rows that each block saw, in the order of the groups.
 // A block per SM goes through the rows; a group reads its next rows while it deals with one, so that the sums of weight and
 // bias stay in registers and only 148 partial ones meet. Bound by memory: 16384 x 8192 bf16 with the sum's gradient, 1.07 GB,
-// 165 us = 6.5 TB/s with the closing sums; on short inputs by its ends (8192 x 1024, 50 MB, 13.8 us: 7 rounds of rows, then 16 groups' sums).
+// 165 us = 6.5 TB/s with the closing sums; on short inputs by its ends (8192 x 1024, 50 MB, 13.8 us: 7 rounds of rows, then 16
+// groups' sums). Single values: 16384 x 2047 99 us. Rows of a cluster: 8192 x 12000 255 us (one pass for the input's gradient and one for
+// the columns: 539).
 // Sums, normalised values, gradients and what is read ahead take 6 to 8 registers per value: 16 bf16 values in vectors fit
 // the 128 registers of 16 warps, of the others 8 fit the 85 of 24 warps. (16 of those, for rows that need them, spill.)
 __host__ __device__ constexpr int BackwardThreads(int held) { return held == 16 ? 512 : 768; }
@@ -264,44 +340,45 @@ __host__ __device__ constexpr int BackwardStages(int vec, int held, int size) {
 }
 
 __device__ __forceinline__ void CopyAsync(uint4* to, const void* from, bool there) {  // zeros where nothing is there
-  const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(to));
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from), "r"(there ? 16 : 0) : "memory");
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(SharedAddress(to)), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void CommitCopies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kLeft> __device__ __forceinline__ void WaitForCopies() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
 
-template <class T, int kVec, int kLanes, bool kWhole, int kHeld, class W>
-__global__ void __launch_bounds__(BackwardThreads(kHeld), 1)
-BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const float* mean_in, const float* rstd_in, T* dx,
-               float* workspace, long long rows, int n, int groups, int warps) {
-  using N = Num<kVec>;
-  constexpr int kVectors = kHeld / kVec, kNums = Vector<T, kVec>::kNums, kStep = kLanes * kVec;
-  extern __shared__ __align__(16) unsigned char shared[];
-  __shared__ float2 part[2][BackwardThreads(kHeld) / 32];
-  const Group<kLanes> group(warps);
+// The sums over rows that a thread keeps, of its columns.
+template <int kPairs> struct ColumnSums {
+  Pair dw[kPairs], db[kPairs];
+};
+
+template <class T, int kVec, int kLanes, bool kWhole, bool kSplit, int kHeld, class W>
+__device__ __forceinline__ void BackwardRows(const T* dy, const T* dsum, const T* s, const Parameter& weight, const float* mean_in,
+                                             const float* rstd_in, T* dx, long long rows, int n, int groups, const Group<kLanes, kSplit>& group,
+                                             float2 (*part)[BackwardThreads(kHeld) / 32], float2 (*across)[8], uint4* ring,
+                                             ColumnSums<kHeld / 2>* sums) {
+  using V = Vector<T, kVec, kLanes>;
+  constexpr int kNums = V::kNums, kVectors = kHeld / (2 * kNums), kStep = V::kStep;
   const int column = group.First(kHeld, kVec), left = n - column;
-  const long long stride = static_cast<long long>(gridDim.x) * groups;  // (of rows)
+  const long long stride = group.Stride(groups);
   // The weight stays in registers where these suffice, else it comes from L1 for every row.
   constexpr bool kKeepWeight = sizeof(T) == 2 && kVec > 1;
-  N w[kVectors][kNums], dw[kVectors][kNums], db[kVectors][kNums];
-#pragma unroll
-  for (int j = 0; j < kVectors; j++) {
-#pragma unroll
-    for (int i = 0; i < kNums; i++) w[j][i] = dw[j][i] = db[j][i] = N(0.f);
-  }
-  Vector<T, kVec> d[kVectors], v[kVectors], more[kVectors];
-  float mean = 0.f, rstd = 0.f;
-  const auto load = [&](long long row) {
-    const long long at = row * n + column;
+  Pair w[kVectors][kNums];
+  if constexpr (kKeepWeight) {
 #pragma unroll
     for (int j = 0; j < kVectors; j++) {
-      d[j].LoadIf(kWhole || j * kStep < left, dy + at + j * kStep);
-      v[j].LoadIf(kWhole || j * kStep < left, s + at + j * kStep);
+      if (kWhole || j * kStep < left) LoadParameter<kVec, kLanes, kWhole, W>(weight, column + j * kStep, left - j * kStep, 1.f, w[j]);
+    }
+  }
+  V d[kVectors], v[kVectors], more[kVectors];
+  float mean = 0.f, rstd = 0.f;
+  const auto load = [&](const T* from, V(&to)[kVectors]) {
+#pragma unroll
+    for (int j = 0; j < kVectors; j++) {
+      if constexpr (kWhole) to[j].Load(from + j * kStep);
+      else to[j].LoadSome(from + j * kStep, left - j * kStep);
     }
   };
   // The ring: kStages rows of kVectors vectors of dy, s and, if there is one, dsum for every thread.
   constexpr int kStages = BackwardStages(kVec, kHeld, sizeof(T)), kThreads = BackwardThreads(kHeld);
-  uint4* const ring = reinterpret_cast<uint4*>(shared) + threadIdx.x;
   const auto copy = [&](long long row, int stage) {
     if (row < rows) {
       const long long at = row * n + column;
@@ -317,20 +394,14 @@ BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const f
     }
     CommitCopies();
   };
-  WaitForEarlierKernels();
-  if constexpr (kKeepWeight) {
-#pragma unroll
-    for (int j = 0; j < kVectors; j++) {
-      if (kWhole || j * kStep < left) LoadParameter<kVec, W>(weight, column + j * kStep, 1.f, w[j]);
-    }
-  }
   // (Groups that do not fit into the block any more have no row.)
-  long long row = group.number < groups ? static_cast<long long>(blockIdx.x) * groups + group.number : rows;
+  long long row = group.number < groups ? group.FirstRow(groups) : rows;
   if constexpr (kStages > 0) {
 #pragma unroll
     for (int i = 0; i < kStages - 1; i++) copy(row + i * stride, i);
   } else if (row < rows) {
-    load(row);
+    load(dy + row * n + column, d);
+    load(s + row * n + column, v);
   }
   if (row < rows) mean = mean_in[row], rstd = rstd_in[row];
   int turn = 0, stage = 0;
@@ -347,41 +418,41 @@ BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const f
         v[j].LoadShared(from + (kVectors + j) * kThreads);
       }
     }
-    N c1(0.f), c2(0.f), xhat[kVectors][kNums], g[kVectors][kNums];
+    Pair c1(0.f), c2(0.f), xhat[kVectors][kNums], g[kVectors][kNums];
 #pragma unroll
     for (int j = 0; j < kVectors; j++) {
       if (!kWhole && j * kStep >= left) continue;  // (what is not there has gradients of 0, but 0 times infinity is NaN)
-      if constexpr (!kKeepWeight) LoadParameter<kVec, W>(weight, column + j * kStep, 1.f, w[j]);
+      if constexpr (!kKeepWeight) LoadParameter<kVec, kLanes, kWhole, W>(weight, column + j * kStep, left - j * kStep, 1.f, w[j]);
 #pragma unroll
       for (int i = 0; i < kNums; i++) {
-        const N dyi = d[j].At(i);
-        xhat[j][i] = (v[j].At(i) + N(-mean)) * N(r);
+        const Pair dyi = d[j].At(i);
+        xhat[j][i] = V::template There<kWhole>((v[j].At(i) + Pair(-mean)) * Pair(r), left - j * kStep);
         g[j][i] = dyi * w[j][i];
         c1 = c1 + g[j][i];
         c2 = Fma(g[j][i], xhat[j][i], c2);
-        dw[j][i] = Fma(dyi, xhat[j][i], dw[j][i]);
-        db[j][i] = db[j][i] + dyi;
+        sums->dw[j * kNums + i] = Fma(dyi, xhat[j][i], sums->dw[j * kNums + i]);
+        sums->db[j * kNums + i] = sums->db[j * kNums + i] + dyi;
       }
     }
     if constexpr (kStages == 0) {
-      if (dsum) {
-#pragma unroll
-        for (int j = 0; j < kVectors; j++) more[j].LoadIf(kWhole || j * kStep < left, dsum + at + j * kStep);
+      if (dsum) load(dsum + at, more);
+      if (row + stride < rows) {
+        load(dy + at + stride * n, d);
+        load(s + at + stride * n, v);
       }
-      if (row + stride < rows) load(row + stride);
     }
     if (row + stride < rows) mean = mean_in[row + stride], rstd = rstd_in[row + stride];
-    const float2 c12 = group.Sum(make_float2(Sum(c1), Sum(c2)), part[turn]);
+    const float2 c12 = group.Sum(make_float2(Sum(c1), Sum(c2)), part[turn], across[turn]);
     turn ^= 1;
-    const N minus_c1(-c12.x / n), minus_c2(-c12.y / n);
+    const Pair minus_c1(-c12.x / n), minus_c2(-c12.y / n);
     const auto store = [&](auto plus) {
 #pragma unroll
       for (int j = 0; j < kVectors; j++) {
         if (!kWhole && j * kStep >= left) continue;
-        Vector<T, kVec> out;
+        V out;
 #pragma unroll
-        for (int i = 0; i < kNums; i++) out.Set(i, plus(Fma(xhat[j][i], minus_c2, g[j][i] + minus_c1) * N(r), j, i));
-        out.Store(dx + at + j * kStep);
+        for (int i = 0; i < kNums; i++) out.Set(i, plus(Fma(xhat[j][i], minus_c2, g[j][i] + minus_c1) * Pair(r), j, i));
+        out.template Store<kWhole>(dx + at + j * kStep, left - j * kStep);
       }
     };
     if (dsum) {
@@ -389,46 +460,72 @@ BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const f
 #pragma unroll
         for (int j = 0; j < kVectors; j++) more[j].LoadShared(ring + (stage * 3 * kVectors + 2 * kVectors + j) * kThreads);
       }
-      store([&](N e, int j, int i) { return e + more[j].At(i); });
+      store([&](Pair e, int j, int i) { return e + more[j].At(i); });
     } else {
-      store([](N e, int, int) { return e; });
+      store([](Pair e, int, int) { return e; });
     }
     stage = stage + 1 < kStages ? stage + 1 : 0;
   }
+}
+
+template <class T, int kVec, int kLanes, bool kWhole, bool kSplit, int kHeld, class W>
+__global__ void __launch_bounds__(BackwardThreads(kHeld), 1)
+BackwardKernel(const T* dy, const T* dsum, const T* s, Parameter weight, const float* mean, const float* rstd, T* dx,
+               float* workspace, long long rows, int n, int groups, int warps, int ranks) {
+  using V = Vector<T, kVec, kLanes>;
+  extern __shared__ __align__(16) unsigned char shared[];
+  __shared__ float2 part[2][BackwardThreads(kHeld) / 32];
+  __shared__ float2 across[2][8];
+  const Group<kLanes, kSplit> group(warps, ranks);
+  uint4* const ring = reinterpret_cast<uint4*>(shared) + threadIdx.x;
+  ColumnSums<kHeld / 2> sums;
+#pragma unroll
+  for (int i = 0; i < kHeld / 2; i++) sums.dw[i] = sums.db[i] = Pair(0.f);
+  WaitForEarlierKernels();
+  group.Meet();
+  if (kWhole || (WarpAsks(kVec, kSplit) && group.Whole(kHeld, n)))
+    BackwardRows<T, kVec, kLanes, true, kSplit, kHeld, W>(dy, dsum, s, weight, mean, rstd, dx, rows, n, groups, group, part, across, ring, &sums);
+  else
+    BackwardRows<T, kVec, kLanes, false, kSplit, kHeld, W>(dy, dsum, s, weight, mean, rstd, dx, rows, n, groups, group, part, across, ring, &sums);
   if (!workspace) return;
   LetNextKernelStart();  // (what finishes the sums)
   // The upper half of the groups gives its sums to the lower one until one has all. (In the ring's place, after a barrier: no
   // thread has copies under way that are for rows, and what it has of empty ones counts for nothing.)
-  N* const sums = reinterpret_cast<N*>(shared);
-  const int width = kLanes == 32 ? warps * 32 : kLanes, t = kLanes == 32 ? group.warp * 32 + group.lane : group.lane;
+  Pair* const given = reinterpret_cast<Pair*>(shared);
+  const int width = kLanes == 32 ? warps * 32 : kLanes;
+  const int t = kLanes == 32 ? static_cast<int>(threadIdx.x) - group.number * width : group.lane;
   for (int there = groups; there > 1;) {
     const int half = (there + 1) / 2;
     __syncthreads();
     if (group.number >= half && group.number < there) {
 #pragma unroll
-      for (int i = 0; i < kVectors * kNums; i++) {
-        sums[(2 * i * half + group.number - half) * width + t] = dw[i / kNums][i % kNums];
-        sums[((2 * i + 1) * half + group.number - half) * width + t] = db[i / kNums][i % kNums];
+      for (int i = 0; i < kHeld / 2; i++) {
+        given[(2 * i * half + group.number - half) * width + t] = sums.dw[i];
+        given[((2 * i + 1) * half + group.number - half) * width + t] = sums.db[i];
       }
     }
     __syncthreads();
     if (group.number < there - half) {
 #pragma unroll
-      for (int i = 0; i < kVectors * kNums; i++) {
-        dw[i / kNums][i % kNums] = dw[i / kNums][i % kNums] + sums[(2 * i * half + group.number) * width + t];
-        db[i / kNums][i % kNums] = db[i / kNums][i % kNums] + sums[((2 * i + 1) * half + group.number) * width + t];
+      for (int i = 0; i < kHeld / 2; i++) {
+        sums.dw[i] = sums.dw[i] + given[(2 * i * half + group.number) * width + t];
+        sums.db[i] = sums.db[i] + given[((2 * i + 1) * half + group.number) * width + t];
       }
     }
     there = half;
   }
   if (group.number) return;
-  float* const out = workspace + static_cast<long long>(blockIdx.x) * 2 * n + column;
+  const int column = group.First(kHeld, kVec);
+  float* const out = workspace + static_cast<long long>(kSplit ? blockIdx.x / ranks : blockIdx.x) * 2 * n;
 #pragma unroll
-  for (int i = 0; i < kVectors * kNums; i++) {
-    const int c = i / kNums * kStep + i % kNums * 2;
-    if (kWhole || i / kNums * kStep < left) {
-      *reinterpret_cast<N*>(out + c) = dw[i / kNums][i % kNums];
-      *reinterpret_cast<N*>(out + n + c) = db[i / kNums][i % kNums];  // (pairs: n is even)
+  for (int i = 0; i < kHeld / 2; i++) {
+    const int c = column + i / V::kNums * V::kStep + i % V::kNums * 2;
+    if constexpr (kVec > 1) {  // (n is even)
+      if (c < n) *reinterpret_cast<Pair*>(out + c) = sums.dw[i], *reinterpret_cast<Pair*>(out + n + c) = sums.db[i];
+    } else {
+      const float2 dw = sums.dw[i].Both(), db = sums.db[i].Both();
+      if (c < n) out[c] = dw.x, out[n + c] = db.x;
+      if (c + kLanes < n) out[c + kLanes] = dw.y, out[n + c + kLanes] = db.y;
     }
   }
 }
@@ -597,18 +694,23 @@ struct Alignment {
 
 // How rows of n values are held by groups of a block of up to `warps` warps, with `held` values per lane.
 struct Geometry {
-  int lanes = 0, warps = 0, groups = 0, blocks = 0;  // warps: of a group; lanes = 0: the rows are too long
+  // lanes = 0: the rows are too long; warps: of a group in a block; groups: of a block; ranks: blocks of a group; parts: blocks / ranks
+  int lanes = 0, warps = 0, groups = 0, ranks = 1, parts = 0;
   bool whole = false;
   Geometry(long long rows, int n, int held, int block_warps, int most_warps, int most_blocks) {
-    if (n > most_warps * 32 * held) return;
+    while (n > ranks * most_warps * 32 * held) {
+      if (ranks == 8) return;
+      ranks *= 2;
+    }
     lanes = n <= 8 * held ? 8 : 32;
-    warps = lanes == 8 ? 1 : (n - 1) / (32 * held) + 1;
+    warps = lanes == 8 ? 1 : ranks > 1 ? most_warps : (n - 1) / (32 * held) + 1;
     if (block_warps % warps && block_warps < 16) block_warps = 16;  // (a block reserves all barriers: 4 of them to an SM)
     groups = lanes == 8 ? block_warps * 4 : block_warps / warps > 0 ? block_warps / warps : 1;
-    whole = lanes == 32 && n == warps * 32 * held;
+    whole = n == ranks * warps * 32 * held && lanes == 32;
     const long long wanted = (rows + groups - 1) / groups;
-    blocks = static_cast<int>(wanted < most_blocks ? wanted : most_blocks);
+    parts = static_cast<int>(wanted < most_blocks / ranks ? wanted : most_blocks / ranks);
   }
+  unsigned Blocks() const { return static_cast<unsigned>(parts) * ranks; }
   int Threads() const { return lanes == 8 ? groups * 8 : groups * warps * 32; }
 };
 
@@ -626,30 +728,39 @@ template <class T> Kind TypeOf(const Parameter& a, const Parameter& b) {
   return a.type == SML_NORM_F32 ? Kind::kF32 : Kind::kBf16;
 }
 
-template <class T, int kVec, int kLanes, int kHeld> auto BackwardKernelOf(Kind type) {
-  return type == Kind::kF32 ? BackwardKernel<T, kVec, kLanes, false, kHeld, float> : BackwardKernel<T, kVec, kLanes, false, kHeld, void>;
+template <class T, int kVec, int kLanes, bool kSplit, int kHeld> auto BackwardKernelOf(Kind type) {
+  return type == Kind::kF32 ? BackwardKernel<T, kVec, kLanes, false, kSplit, kHeld, float>
+                            : BackwardKernel<T, kVec, kLanes, false, kSplit, kHeld, void>;
 }
 template <class T, int kHeld> auto BackwardKernelOf(const Geometry& g, int vec, Kind type) {
   if constexpr (kHeld == 8) {  // (the others are for longer rows)
     if (g.lanes == 8)
-      return vec == 1 ? BackwardKernelOf<T, 1, 8, kHeld>(type) : vec == 2 ? BackwardKernelOf<T, 2, 8, kHeld>(type)
-             : BackwardKernelOf<T, kWide<T>, 8, kHeld>(type);
+      return vec == 1 ? BackwardKernelOf<T, 1, 8, false, kHeld>(type) : vec == 2 ? BackwardKernelOf<T, 2, 8, false, kHeld>(type)
+             : BackwardKernelOf<T, kWide<T>, 8, false, kHeld>(type);
+  } else {
+    if (g.ranks > 1)
+      return vec == 1 ? BackwardKernelOf<T, 1, 32, true, kHeld>(type) : vec == 2 ? BackwardKernelOf<T, 2, 32, true, kHeld>(type)
+             : BackwardKernelOf<T, kWide<T>, 32, true, kHeld>(type);
   }
-  if (vec <= 2) return vec == 1 ? BackwardKernelOf<T, 1, 32, kHeld>(type) : BackwardKernelOf<T, 2, 32, kHeld>(type);
-  if (!g.whole) return BackwardKernelOf<T, kWide<T>, 32, kHeld>(type);
-  return type == Kind::kF32 ? BackwardKernel<T, kWide<T>, 32, true, kHeld, float>
-         : type == Kind::kBf16 ? BackwardKernel<T, kWide<T>, 32, true, kHeld, T> : BackwardKernel<T, kWide<T>, 32, true, kHeld, void>;
+  if (vec <= 2) return vec == 1 ? BackwardKernelOf<T, 1, 32, false, kHeld>(type) : BackwardKernelOf<T, 2, 32, false, kHeld>(type);
+  if (!g.whole) return BackwardKernelOf<T, kWide<T>, 32, false, kHeld>(type);
+  return type == Kind::kF32 ? BackwardKernel<T, kWide<T>, 32, true, false, kHeld, float>
+         : type == Kind::kBf16 ? BackwardKernel<T, kWide<T>, 32, true, false, kHeld, T> : BackwardKernel<T, kWide<T>, 32, true, false, kHeld, void>;
 }
-template <class T, int kVec, int kLanes> auto ForwardKernelOf(Kind type) {
-  return type == Kind::kF32 ? ForwardKernel<T, kVec, kLanes, false, float> : ForwardKernel<T, kVec, kLanes, false, void>;
+template <class T, int kVec, int kLanes, bool kSplit> auto ForwardKernelOf(Kind type) {
+  return type == Kind::kF32 ? ForwardKernel<T, kVec, kLanes, false, kSplit, float> : ForwardKernel<T, kVec, kLanes, false, kSplit, void>;
 }
 template <class T> auto ForwardKernelOf(const Geometry& g, int vec, Kind type) {
   if (g.lanes == 8)
-    return vec == 1 ? ForwardKernelOf<T, 1, 8>(type) : vec == 2 ? ForwardKernelOf<T, 2, 8>(type) : ForwardKernelOf<T, kWide<T>, 8>(type);
-  if (vec <= 2) return vec == 1 ? ForwardKernelOf<T, 1, 32>(type) : ForwardKernelOf<T, 2, 32>(type);
-  if (!g.whole) return ForwardKernelOf<T, kWide<T>, 32>(type);
-  return type == Kind::kF32 ? ForwardKernel<T, kWide<T>, 32, true, float>
-         : type == Kind::kBf16 ? ForwardKernel<T, kWide<T>, 32, true, T> : ForwardKernel<T, kWide<T>, 32, true, void>;
+    return vec == 1 ? ForwardKernelOf<T, 1, 8, false>(type) : vec == 2 ? ForwardKernelOf<T, 2, 8, false>(type)
+           : ForwardKernelOf<T, kWide<T>, 8, false>(type);
+  if (g.ranks > 1)
+    return vec == 1 ? ForwardKernelOf<T, 1, 32, true>(type) : vec == 2 ? ForwardKernelOf<T, 2, 32, true>(type)
+           : ForwardKernelOf<T, kWide<T>, 32, true>(type);
+  if (vec <= 2) return vec == 1 ? ForwardKernelOf<T, 1, 32, false>(type) : ForwardKernelOf<T, 2, 32, false>(type);
+  if (!g.whole) return ForwardKernelOf<T, kWide<T>, 32, false>(type);
+  return type == Kind::kF32 ? ForwardKernel<T, kWide<T>, 32, true, false, float>
+         : type == Kind::kBf16 ? ForwardKernel<T, kWide<T>, 32, true, false, T> : ForwardKernel<T, kWide<T>, 32, true, false, void>;
 }
 
 template <class T>
@@ -664,8 +775,8 @@ int Forward(const void* x_in, const void* residual_in, Parameter weight, Paramet
   if (!g.lanes)
     return Launched(LaunchOverlapped(ForwardAnyKernel<T>, RowBlocks(rows), kAnyThreads, 0, 1, stream, x, residual, weight, bias, y, sum,
                                      mean, rstd, rows, n, eps));
-  return Launched(LaunchOverlapped(ForwardKernelOf<T>(g, vec, TypeOf<T>(weight, bias)), g.blocks, g.Threads(), 0, 1, stream, x, residual, weight, bias, y, sum, mean, rstd, rows, n,
-                                   eps, g.groups, g.warps));
+  return Launched(LaunchOverlapped(ForwardKernelOf<T>(g, vec, TypeOf<T>(weight, bias)), g.Blocks(), g.Threads(), 0, g.ranks, stream, x, residual, weight, bias, y, sum, mean, rstd, rows, n,
+                                   eps, g.groups, g.warps, g.ranks));
 }
 
 template <class T>
@@ -690,9 +801,9 @@ int Backward(const void* dy_in, const void* dsum_in, const void* s_in, Parameter
       e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
       if (e != cudaSuccess) return Launched(e);
     }
-    parts = g.blocks;
-    e = LaunchOverlapped(kernel, parts, BackwardThreads(held), shared, 1, stream, dy, dsum, s, weight, mean, rstd, dx, workspace, rows, n,
-                         g.groups, g.warps);
+    parts = g.parts;
+    e = LaunchOverlapped(kernel, g.Blocks(), BackwardThreads(held), shared, g.ranks, stream, dy, dsum, s, weight, mean, rstd, dx, workspace, rows, n,
+                         g.groups, g.warps, g.ranks);
   } else {
     e = LaunchOverlapped(BackwardAnyKernel<T>, RowBlocks(rows), kAnyThreads, 0, 1, stream, dy, dsum, s, weight, mean, rstd, dx, rows, n);
     if (e == cudaSuccess && workspace) {
@@ -722,7 +833,7 @@ extern "C" long long switchml_layer_norm_workspace(long long rows, int features,
   if (rows <= 0 || features <= 0 || !Known(type)) return 0;
   // (Which it will be depends on the addresses too.)
   const Geometry g = BackwardGeometry(rows, features, 8), h = BackwardGeometry(rows, features, 16);
-  const int held = g.blocks > h.blocks ? g.blocks : h.blocks;
+  const int held = g.parts > h.parts ? g.parts : h.parts;
   return 2ll * features * (h.lanes ? held : RowShares(rows, features));
 }
 

@@ -35,9 +35,6 @@ __device__ __forceinline__ Pair Fma(Pair a, Pair b, Pair c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.w) : "l"(a.w), "l"(b.w), "l"(c.w));
   return r;
 }
-// The same for single numbers, for code that takes either.
-__device__ __forceinline__ float Fma(float a, float b, float c) { return fmaf(a, b, c); }
-__device__ __forceinline__ float Sum(float v) { return v; }
 __device__ __forceinline__ float Sum(Pair p) {
   const float2 v = p.Both();
   return v.x + v.y;
@@ -65,22 +62,22 @@ template <int kWords> __device__ __forceinline__ void LoadWords(const void* from
     asm volatile("ld.global.b32 %0, [%1];" : "=r"(w[0]) : "l"(from));
   }
 }
-// Only where `there`, else zeros: without a branch.
-template <int kWords> __device__ __forceinline__ void LoadWordsIf(bool there, const void* from, unsigned (&w)[kWords]) {
+// Only where left > 0, else zeros: without a branch.
+template <int kWords> __device__ __forceinline__ void LoadWordsIf(int left, const void* from, unsigned (&w)[kWords]) {
 #pragma unroll
   for (int i = 0; i < kWords; i++) w[i] = 0;
   if constexpr (kWords == 8) {
-    asm volatile("{.reg .pred p; setp.ne.b32 p, %9, 0; @p ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];}"
+    asm volatile("{.reg .pred p; setp.gt.s32 p, %9, 0; @p ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];}"
                  : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3]), "+r"(w[4]), "+r"(w[5]), "+r"(w[6]), "+r"(w[7])
-                 : "l"(from), "r"(static_cast<int>(there)));
+                 : "l"(from), "r"(left));
   } else if constexpr (kWords == 4) {
-    asm volatile("{.reg .pred p; setp.ne.b32 p, %5, 0; @p ld.global.v4.b32 {%0,%1,%2,%3}, [%4];}"
-                 : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3]) : "l"(from), "r"(static_cast<int>(there)));
+    asm volatile("{.reg .pred p; setp.gt.s32 p, %5, 0; @p ld.global.v4.b32 {%0,%1,%2,%3}, [%4];}"
+                 : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3]) : "l"(from), "r"(left));
   } else if constexpr (kWords == 2) {
-    asm volatile("{.reg .pred p; setp.ne.b32 p, %3, 0; @p ld.global.v2.b32 {%0,%1}, [%2];}"
-                 : "+r"(w[0]), "+r"(w[1]) : "l"(from), "r"(static_cast<int>(there)));
+    asm volatile("{.reg .pred p; setp.gt.s32 p, %3, 0; @p ld.global.v2.b32 {%0,%1}, [%2];}"
+                 : "+r"(w[0]), "+r"(w[1]) : "l"(from), "r"(left));
   } else {
-    asm volatile("{.reg .pred p; setp.ne.b32 p, %2, 0; @p ld.global.b32 %0, [%1];}" : "+r"(w[0]) : "l"(from), "r"(static_cast<int>(there)));
+    asm volatile("{.reg .pred p; setp.gt.s32 p, %2, 0; @p ld.global.b32 %0, [%1];}" : "+r"(w[0]) : "l"(from), "r"(left));
   }
 }
 template <int kWords> __device__ __forceinline__ void StoreWords(void* to, const unsigned (&w)[kWords]) {

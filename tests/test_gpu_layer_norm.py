@@ -65,6 +65,56 @@ def test_rows(rows, residual, dtype):
     run_and_check(*make((rows, 264), dtype, F32, residual, True, seed=rows), 1e-5, True)
 
 
+@pytest.mark.parametrize("dtype,wtype", [(F32, F32), (BF16, F32), (BF16, BF16)])
+@pytest.mark.parametrize("rows,features", [(300, 12000), (301, 12002), (299, 8193), (150, 16385), (160, 20001), (80, 33000), (75, 65535)])
+def test_many_rows_that_several_blocks_share(rows, features, dtype, wtype):
+    run_and_check(*make((rows, features), dtype, wtype, rows % 2 == 0, True, seed=rows), 1e-5, True)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [1, 2, 36, 37, 38, 73, 75])
+def test_rows_around_the_number_of_clusters(rows, dtype):
+    run_and_check(*make((rows, 20002), dtype, F32, True, rows % 2 == 0, seed=rows), 1e-5, False)
+
+
+@pytest.mark.parametrize("features", [8200, 12000, 20001, 40001])
+def test_long_rows_on_two_streams_and_replayed(features):
+    """Every run adds in the same order."""
+    _, dev = make((301, features), BF16, F32, True, True)
+    leaves = [dev[k].requires_grad_() for k in ("x", "weight", "bias")]
+
+    def once():
+        y, s = layer_norm(dev["x"], dev["weight"], dev["bias"], residual=dev["residual"])
+        return (y, s) + torch.autograd.grad((y, s), leaves, (dev["dy"], dev["ds"]))
+
+    streams, results = [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for stream in streams:
+        with torch.cuda.stream(stream):
+            results.append(once())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = once()
+    for _ in range(2):
+        for o in out:
+            o.detach().zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(out, *results))
+
+
+@pytest.mark.parametrize("features", [12000, 20001])
+def test_values_that_are_not_finite_in_a_long_row(features):
+    data, dev = make((40, features), BF16, F32, False, True)
+    dev["x"][2, 5], dev["x"][4, features - 1] = float("nan"), float("inf")
+    y = layer_norm(dev["x"], dev["weight"], dev["bias"])
+    assert y[2].isnan().all() and y[4].isnan().all()
+    values, bounds = layer_norm64(data["x"], None, data["weight"], data["bias"], 1e-5)
+    keep = [r for r in range(40) if r not in (2, 4)]
+    check("y", y[keep], values["y"][keep], bounds["y"][keep])
+
+
 @pytest.mark.parametrize("offset", [1, 2, 4, 8])
 @pytest.mark.parametrize("features", [96, 1000, 1024, 4096, 6000])
 def test_addresses_behind_an_aligned_one(features, offset):
