@@ -324,11 +324,11 @@ ForwardKernel(const T* x, const T* residual, Parameter weight, Parameter bias, T
 // The backward pass of rows that a group holds, and the sums over the rows that each block saw, in the order of the groups.
 // A block per SM goes through the rows; a group reads its next rows while it deals with one, so that the sums of weight and
 // bias stay in registers and only 148 partial ones meet. Bound by memory: 16384 x 8192 bf16 with the sum's gradient, 1.07 GB,
-// 165 us = 6.5 TB/s with the closing sums; on short inputs by its ends (8192 x 1024, 50 MB, 13.8 us: 7 rounds of rows, then 16
-// groups' sums). Single values: 16384 x 2047 99 us. Rows of a cluster: 8192 x 12000 255 us (one pass for the input's gradient and one for
-// the columns: 539).
+// 165 us = 6.5 TB/s with the closing sums; on short inputs by its ends (8192 x 1024, 50 MB, 14.8 us: 7 rounds of rows, then 16
+// groups' sums). Single values: 16384 x 2047 99 us. Rows of a cluster: 8192 x 12000 255 us (one pass for the input's gradient and
+// one for the columns: 539).
 // Sums, normalised values, gradients and what is read ahead take 6 to 8 registers per value: 16 bf16 values in vectors fit
-// the 128 registers of 16 warps, of the others 8 fit the 85 of 24 warps. (16 of those, for rows that need them, spill.)
+// the 128 registers of 16 warps, of the others 8 fit the 85 of 24 warps. (Of 16 of those, for rows that need them, most spill.)
 __host__ __device__ constexpr int BackwardThreads(int held) { return held == 16 ? 512 : 768; }
 int BackwardHeld(int n, int vec) { return (vec == 8 && n > 256) || n > BackwardThreads(8) * 8 ? 16 : 8; }
 
