@@ -72,7 +72,8 @@ __host__ __device__ constexpr bool WarpAsks(int vec, bool split) { return vec ==
 __device__ __forceinline__ uint32_t SharedAddress(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
 template <int kLanes, bool kSplit> struct Group {  // kSplit: over the blocks of a cluster
-  int number, warps, ranks, lane, warp;  // number: in the block; warps: of a group in a block; ranks: blocks of a group; lane, warp: in the group
+  // number: in the block; warps: of a group in a block; ranks: blocks of a group; lane, warp: in the group
+  int number, warps, ranks, lane, warp;
   unsigned mask;
   __device__ __forceinline__ Group(int warps_of_group, int blocks_of_group) : warps(warps_of_group), ranks(kSplit ? blocks_of_group : 1) {
     const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
@@ -88,8 +89,12 @@ template <int kLanes, bool kSplit> struct Group {  // kSplit: over the blocks of
   // Whether all values of this warp's exist in a row of n.
   __device__ __forceinline__ bool Whole(int held, int n) const { return kLanes == 32 && (warp + 1) * 32 * held <= n; }
   // Row of the first turn, and the distance to the next.
-  __device__ __forceinline__ long long FirstRow(int groups) const { return static_cast<long long>(kSplit ? blockIdx.x / ranks : blockIdx.x) * groups + number; }
-  __device__ __forceinline__ long long Stride(int groups) const { return static_cast<long long>(kSplit ? gridDim.x / ranks : gridDim.x) * groups; }
+  __device__ __forceinline__ long long FirstRow(int groups) const {
+    return static_cast<long long>(kSplit ? blockIdx.x / ranks : blockIdx.x) * groups + number;
+  }
+  __device__ __forceinline__ long long Stride(int groups) const {
+    return static_cast<long long>(kSplit ? gridDim.x / ranks : gridDim.x) * groups;
+  }
   // Before the first Sum: the blocks of a group are there.
   __device__ __forceinline__ void Meet() const {
     if constexpr (kSplit) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -682,6 +687,9 @@ int RowShares(long long rows, int n) {
   return static_cast<int>(shares);
 }
 
+// Columns are counted in 32 bits, beyond a row's end too.
+bool Fits(int features) { return features > 0 && features <= 1 << 30; }
+
 bool Known(int type) { return type == SML_NORM_F32 || type == SML_NORM_BF16; }
 
 // Values that are read and written at once: what the length of the rows and all addresses allow.
@@ -775,8 +783,8 @@ int Forward(const void* x_in, const void* residual_in, Parameter weight, Paramet
   if (!g.lanes)
     return Launched(LaunchOverlapped(ForwardAnyKernel<T>, RowBlocks(rows), kAnyThreads, 0, 1, stream, x, residual, weight, bias, y, sum,
                                      mean, rstd, rows, n, eps));
-  return Launched(LaunchOverlapped(ForwardKernelOf<T>(g, vec, TypeOf<T>(weight, bias)), g.Blocks(), g.Threads(), 0, g.ranks, stream, x, residual, weight, bias, y, sum, mean, rstd, rows, n,
-                                   eps, g.groups, g.warps, g.ranks));
+  return Launched(LaunchOverlapped(ForwardKernelOf<T>(g, vec, TypeOf<T>(weight, bias)), g.Blocks(), g.Threads(), 0, g.ranks, stream,
+                                   x, residual, weight, bias, y, sum, mean, rstd, rows, n, eps, g.groups, g.warps, g.ranks));
 }
 
 template <class T>
@@ -786,14 +794,15 @@ int Backward(const void* dy_in, const void* dsum_in, const void* s_in, Parameter
   T* dx = static_cast<T*>(dx_in);
   if (!dweight && !dbias) workspace = nullptr;
   Alignment at;
-  at.Of(dy), at.Of(dsum), at.Of(s), at.Of(weight), at.Of(dx);
+  at.Of(dy), at.Of(dsum), at.Of(s), at.Of(weight), at.Of(dx), at.Of(workspace);  // (vectors' sums go there in pairs)
   const int vec = at.Vec(n, kWide<T>);
   const int held = BackwardHeld(n, vec);
   const Geometry g = BackwardGeometry(rows, n, held);
   int parts = 0;
   cudaError_t e;
   if (g.lanes) {
-    const auto kernel = held == 16 ? BackwardKernelOf<T, 16>(g, vec, TypeOf<T>(weight, weight)) : BackwardKernelOf<T, 8>(g, vec, TypeOf<T>(weight, weight));
+    const Kind type = TypeOf<T>(weight, weight);
+    const auto kernel = held == 16 ? BackwardKernelOf<T, 16>(g, vec, type) : BackwardKernelOf<T, 8>(g, vec, type);
     const int ring = BackwardStages(vec, held, sizeof(T)) * BackwardRowBytes(held, sizeof(T));
     const int ends = workspace && g.groups > 1 ? (g.groups + 1) / 2 * (g.Threads() / g.groups) * 2 * held * static_cast<int>(sizeof(float)) : 0;
     const int shared = ring > ends ? ring : ends;
@@ -802,8 +811,8 @@ int Backward(const void* dy_in, const void* dsum_in, const void* s_in, Parameter
       if (e != cudaSuccess) return Launched(e);
     }
     parts = g.parts;
-    e = LaunchOverlapped(kernel, g.Blocks(), BackwardThreads(held), shared, g.ranks, stream, dy, dsum, s, weight, mean, rstd, dx, workspace, rows, n,
-                         g.groups, g.warps, g.ranks);
+    e = LaunchOverlapped(kernel, g.Blocks(), BackwardThreads(held), shared, g.ranks, stream, dy, dsum, s, weight, mean, rstd, dx,
+                         workspace, rows, n, g.groups, g.warps, g.ranks);
   } else {
     e = LaunchOverlapped(BackwardAnyKernel<T>, RowBlocks(rows), kAnyThreads, 0, 1, stream, dy, dsum, s, weight, mean, rstd, dx, rows, n);
     if (e == cudaSuccess && workspace) {
@@ -823,14 +832,14 @@ int Backward(const void* dy_in, const void* dsum_in, const void* s_in, Parameter
 extern "C" int switchml_layer_norm_forward(const void* x, const void* residual, const void* weight, const void* bias, void* y,
                                            void* sum, float* mean, float* rstd, long long rows, int features, float eps, int type,
                                            int wtype, void* stream) {
-  if (!x || !y || (residual && !sum) || !mean != !rstd || rows <= 0 || features <= 0 || !Known(type) || !Known(wtype)) return -1;
+  if (!x || !y || (residual && !sum) || !mean != !rstd || rows <= 0 || !Fits(features) || !Known(type) || !Known(wtype)) return -1;
   return (type == SML_NORM_F32 ? Forward<float> : Forward<__nv_bfloat16>)(x, residual, Parameter{weight, wtype},
                                                                           Parameter{bias, wtype}, y, sum, mean, rstd, rows, features,
                                                                           eps, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" long long switchml_layer_norm_workspace(long long rows, int features, int type) {
-  if (rows <= 0 || features <= 0 || !Known(type)) return 0;
+  if (rows <= 0 || !Fits(features) || !Known(type)) return 0;
   // (Which it will be depends on the addresses too.)
   const Geometry g = BackwardGeometry(rows, features, 8), h = BackwardGeometry(rows, features, 16);
   const int held = g.parts > h.parts ? g.parts : h.parts;
@@ -840,7 +849,7 @@ extern "C" long long switchml_layer_norm_workspace(long long rows, int features,
 extern "C" int switchml_layer_norm_backward(const void* dy, const void* dsum, const void* s, const void* weight, const float* mean,
                                             const float* rstd, void* dx, void* dweight, void* dbias, float* workspace, long long rows,
                                             int features, int type, int wtype, void* stream) {
-  if (!dy || !s || !mean || !rstd || !dx || ((dweight || dbias) && !workspace) || rows <= 0 || features <= 0 || !Known(type) ||
+  if (!dy || !s || !mean || !rstd || !dx || ((dweight || dbias) && !workspace) || rows <= 0 || !Fits(features) || !Known(type) ||
       !Known(wtype))
     return -1;
   return (type == SML_NORM_F32 ? Backward<float> : Backward<__nv_bfloat16>)(dy, dsum, s, Parameter{weight, wtype}, mean, rstd, dx,

@@ -1,8 +1,11 @@
 """ops/layer_norm.py against its formulas in 64 bits."""
+import ctypes
+
 import pytest
 import torch
 
 from _train_reference import check, layer_norm64
+from switchml_b200._native import library_path
 from switchml_b200.ops.layer_norm import FusedLayerNorm, layer_norm
 
 pytestmark = pytest.mark.gpu
@@ -102,6 +105,31 @@ def test_long_rows_on_two_streams_and_replayed(features):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(out, *results))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("features", [512, 4096, 12000])
+def test_in_c_with_a_workspace_at_an_odd_address(features, dtype):
+    lib = ctypes.CDLL(library_path("libswitchml_train.so"))
+    lib.switchml_layer_norm_workspace.restype = ctypes.c_longlong
+    data, dev = make((50, features), dtype, F32, False, True)
+    x, dy, w, size = dev["x"], dev["dy"], dev["weight"], ctypes.c_longlong(50)
+    kind = 0 if dtype == F32 else 1
+    space = torch.empty(lib.switchml_layer_norm_workspace(size, features, kind) + 1, device="cuda")
+    mean, rstd, dx, dw, db = (torch.empty_like(t) for t in (x[:, 0].float(), x[:, 0].float(), x, w, w))
+    y = torch.empty_like(x)
+
+    def at(t):
+        return None if t is None else ctypes.c_void_p(t.data_ptr())
+
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert lib.switchml_layer_norm_forward(at(x), None, at(w), at(dev["bias"]), at(y), None, at(mean), at(rstd), size, features,
+                                           ctypes.c_float(1e-5), kind, 0, stream) == 0
+    assert lib.switchml_layer_norm_backward(at(dy), None, at(x), at(w), at(mean), at(rstd), at(dx), at(dw), at(db), at(space[1:]), size,
+                                            features, kind, 0, stream) == 0
+    values, bounds = layer_norm64(data["x"], None, data["weight"], data["bias"], 1e-5, data["dy"])
+    for name, got in (("y", y), ("dx", dx), ("dweight", dw), ("dbias", db)):
+        check(name, got, values[name], bounds[name])
 
 
 @pytest.mark.parametrize("features", [12000, 20001])

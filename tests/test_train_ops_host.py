@@ -1,11 +1,13 @@
 """Host side of ops/layer_norm.py and ops/adamw.py: what is refused before a kernel is launched, and the arithmetic of
 moments in 8 bits, in its plain form."""
+import ctypes
 import math
 
 import pytest
 import torch
 
 from _train_reference import decode, encode, random_bits
+from switchml_b200._native import library_path
 from switchml_b200.ops.adamw import FusedAdamW, dequantized, grad_norm
 from switchml_b200.ops.layer_norm import FusedLayerNorm, layer_norm
 
@@ -18,6 +20,25 @@ def test_layer_norm_refuses():
         layer_norm(x.half())
     with pytest.raises(ValueError):
         FusedLayerNorm((2, 8))
+
+
+def test_layer_norm_in_c_refuses():
+    """Before a pointer is followed."""
+    lib = ctypes.CDLL(library_path("libswitchml_train.so"))
+    lib.switchml_layer_norm_workspace.restype = ctypes.c_longlong
+    p, rows, eps = ctypes.c_void_p(64), ctypes.c_longlong(1), ctypes.c_float(1e-5)
+
+    def forward(features, x=p, y=p, type=0):
+        return lib.switchml_layer_norm_forward(x, None, None, None, y, None, None, None, rows, features, eps, type, 0, None)
+
+    def backward(features, dweight=None):
+        return lib.switchml_layer_norm_backward(p, None, p, None, p, p, p, dweight, None, None, rows, features, 0, 0, None)
+
+    for features in (-1, 0, 2 ** 30 + 1, 2 ** 31 - 1):
+        assert forward(features) == -1 and backward(features) == -1
+        assert lib.switchml_layer_norm_workspace(rows, features, 0) == 0
+    assert forward(8, x=None) == -1 and forward(8, y=None) == -1 and forward(8, type=2) == -1
+    assert backward(8, dweight=p) == -1  # (no workspace)
 
 
 def test_grad_norm_refuses():
