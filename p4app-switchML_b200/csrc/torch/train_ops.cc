@@ -133,6 +133,9 @@ struct LayerNormBackward : public torch::autograd::Node {
 };
 
 variable_list LayerNormForward(Tensor x, OptTensor residual, const OptTensor& weight, const OptTensor& bias, double eps) {
+  // (A dual tensor need not require a gradient: this is asked whether a backward pass comes or not.)
+  for (const Tensor& t : {x, residual.value_or(Tensor()), weight.value_or(Tensor()), bias.value_or(Tensor())})
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "layer_norm has no forward-mode gradient");
   const bool autocast = x.is_cuda() && at::autocast::is_autocast_enabled(at::kCUDA);
   c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::DispatchKey::AutocastCUDA);
   if (autocast) {
@@ -158,8 +161,6 @@ variable_list LayerNormForward(Tensor x, OptTensor residual, const OptTensor& we
     const Normed r = Normalize(x, residual, weight, bias, eps, false);
     return residual ? variable_list{r.y, r.sum} : variable_list{r.y};
   }
-  for (const Tensor& t : {x, residual.value_or(Tensor()), weight.value_or(Tensor()), bias.value_or(Tensor())})
-    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "layer_norm has no forward-mode gradient");
   const Normed r = Normalize(x, residual, weight, bias, eps, true);
   const std::shared_ptr<LayerNormBackward> node(new LayerNormBackward(), torch::autograd::deleteNode);
   node->set_next_edges(torch::autograd::collect_next_edges(x, residual.value_or(Tensor()), weight.value_or(Tensor()), bias.value_or(Tensor())));

@@ -22,6 +22,17 @@ def test_layer_norm_refuses():
         FusedLayerNorm((2, 8))
 
 
+@pytest.mark.parametrize("where", ["x", "residual", "weight", "bias"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_layer_norm_refuses_forward_mode(where, grad):
+    """Whether anything requires a gradient or not: the result would have no tangent."""
+    with torch.autograd.forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        args = {"x": torch.ones(2, 8), "residual": torch.ones(2, 8), "weight": torch.ones(8), "bias": torch.ones(8)}
+        args[where] = torch.autograd.forward_ad.make_dual(args[where], torch.ones_like(args[where]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            layer_norm(**args)
+
+
 def test_layer_norm_in_c_refuses():
     """Before a pointer is followed."""
     lib = ctypes.CDLL(library_path("libswitchml_train.so"))
