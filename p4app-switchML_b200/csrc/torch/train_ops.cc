@@ -3,9 +3,11 @@
 // parameters to ask for their gradients, and layer norm's backward pass runs on the engine's thread.
 #include <ATen/autocast_mode.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -33,6 +35,18 @@ bool Known(const Tensor& t) { return t.scalar_type() == at::kFloat || t.scalar_t
 int NormType(const Tensor& t) { return t.scalar_type() == at::kFloat ? SML_NORM_F32 : SML_NORM_BF16; }
 
 void* Data(const Tensor& t) { return t.defined() ? const_cast<void*>(t.const_data_ptr()) : nullptr; }
+
+// What records operations to run them again (torch.jit.trace, make_fx, export) sees the allocation of a result here, but not the
+// kernel that writes it: the recording would return memory that nothing has written.
+void RefuseTracing(const char* what) {
+  using c10::impl::TorchDispatchModeKey;
+  using c10::impl::TorchDispatchModeTLS;
+  const bool modes = c10::impl::dispatch_mode_enabled();
+  TORCH_CHECK(!torch::jit::tracer::isTracing() && !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) &&
+                  !(modes && (TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY).has_value() ||
+                              TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FAKE).has_value())),
+              what, " cannot be traced");
+}
 
 // ---- layer norm ----
 
@@ -96,6 +110,7 @@ struct LayerNormBackward : public torch::autograd::Node {
 
   // Edges: x, residual, weight, bias; those of tensors that are not there lead nowhere.
   variable_list apply(variable_list&& grads) override {
+    RefuseTracing("layer_norm");
     TORCH_CHECK(!at::GradMode::is_enabled(), "layer_norm has no gradient of its gradient (create_graph)");
     std::lock_guard<std::mutex> lock(mutex_);
     const Tensor s_ = s.unpack(add ? shared_from_this() : nullptr), weight_ = weight.unpack(), stats_ = stats.unpack();
@@ -133,6 +148,7 @@ struct LayerNormBackward : public torch::autograd::Node {
 };
 
 variable_list LayerNormForward(Tensor x, OptTensor residual, const OptTensor& weight, const OptTensor& bias, double eps) {
+  RefuseTracing("layer_norm");
   // (A dual tensor need not require a gradient: this is asked whether a backward pass comes or not.)
   for (const Tensor& t : {x, residual.value_or(Tensor()), weight.value_or(Tensor()), bias.value_or(Tensor())})
     TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "layer_norm has no forward-mode gradient");
@@ -193,6 +209,7 @@ void NormOf(const std::vector<SmlNormTensor>& list, const Tensor& workspace, int
 
 // Takes a list as it is: a vector of tensors would count every one of them up and down.
 Tensor GradNorm(const py::list& tensors) {
+  RefuseTracing("grad_norm");
   const Py_ssize_t count = PyList_GET_SIZE(tensors.ptr());
   TORCH_CHECK_VALUE(count > 0, "grad_norm: no tensors");
   std::vector<SmlNormTensor> list;
@@ -255,6 +272,7 @@ class Adamw {
 
   // settings: (lr, beta1, beta2, eps, weight decay) of every group; lr_tensors: lr in device memory, or None.
   void Step(const std::vector<std::array<double, 5>>& settings, const std::vector<OptTensor>& lr_tensors, std::optional<double> max_norm) {
+    RefuseTracing("FusedAdamW");
     TORCH_CHECK(settings.size() == groups_.size() && lr_tensors.size() == groups_.size(), "FusedAdamW: groups have come or gone");
     const c10::cuda::OptionalCUDAGuard device(ticket_.device());
     at::NoGradGuard no_grad;
@@ -304,6 +322,7 @@ class Adamw {
 
   // The fp32 values of a group's parameters, in the layout of its state.
   Tensor Masters(size_t k) {
+    RefuseTracing("FusedAdamW");
     const c10::cuda::OptionalCUDAGuard device(ticket_.device());
     const Group& g = groups_.at(k);
     Tensor out = at::empty({g.exp_avg.numel()}, g.exp_avg.options().dtype(at::kFloat));

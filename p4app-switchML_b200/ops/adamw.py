@@ -9,7 +9,8 @@ state, which make the parameter a float32 value. The moments are float32, or wit
 which 32, neighbours in memory, share a scale that is a power of two (e8m0). Those are rounded up or down at
 random, with the distance as the chance: a second moment moves by a thousandth per step while its codes lie 6 to 12 %
 apart, so rounding to the nearest would hold it where it is. The random bits are a function of ``seed``, the step and
-the place of the value: the same run gives the same bits.
+the place of the value: the same run gives the same bits. A tracer (``torch.jit.trace``, ``make_fx``, ``torch.export``) would
+not see the kernels: calls under one are refused.
 """
 import torch
 

@@ -3,6 +3,7 @@ import copy
 
 import pytest
 import torch
+from torch.fx.experimental.proxy_tensor import make_fx
 
 import _train_reference as ref
 from switchml_b200.ops.adamw import FusedAdamW, dequantized, grad_norm
@@ -579,3 +580,13 @@ def test_training_command():
     out = json.loads([line for line in r.stdout.splitlines() if line.startswith("{")][-1])
     assert out["config"]["optimizer"] == "AdamW fused, 8-bit moments" and out["config"]["fused_norm"]
     assert 0 < out["final_loss"] < 100
+
+
+def test_tracers_are_refused():
+    p = torch.zeros(8, device="cuda", requires_grad=True)
+    p.grad = torch.ones(8, device="cuda")
+    opt = FusedAdamW([p], lr=0.1, weight_decay=0.0)
+    for call in (lambda g: opt.step(), lambda g: opt.master_buffers()[0], lambda g: grad_norm([g])):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            make_fx(call)(p.grad)
+    assert int(opt.state[p]["step"]) == 0 and not p.any()

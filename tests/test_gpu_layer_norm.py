@@ -3,6 +3,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from _train_reference import check, layer_norm64
 from switchml_b200._native import library_path
@@ -402,3 +403,14 @@ def test_module_in_the_place_of_torch_s():
         FusedLayerNorm((4, 320))
     with pytest.raises(ValueError):
         fused(x[:, :319])
+
+
+def test_tracers_of_a_backward_pass_are_refused():
+    x = torch.randn(4, 64, device="cuda", requires_grad=True)
+    dy = torch.randn(4, 64, device="cuda")
+    y = layer_norm(x)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(lambda dy: torch.autograd.grad(y, x, dy, retain_graph=True)[0])(dy)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(FusedLayerNorm(64).cuda(), (x,))
+    assert torch.autograd.grad(y, x, dy)[0].isfinite().all()

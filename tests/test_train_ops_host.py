@@ -5,6 +5,8 @@ import math
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from _train_reference import decode, encode, random_bits
 from switchml_b200._native import library_path
@@ -31,6 +33,21 @@ def test_layer_norm_refuses_forward_mode(where, grad):
         args[where] = torch.autograd.forward_ad.make_dual(args[where], torch.ones_like(args[where]))
         with pytest.raises(RuntimeError, match="forward-mode"):
             layer_norm(**args)
+
+
+@pytest.mark.parametrize("call", [lambda x: layer_norm(x), lambda x: grad_norm([x])], ids=["layer_norm", "grad_norm"])
+def test_tracers_are_refused(call):
+    """They would record the allocation of the result without the kernel that writes it."""
+    x = torch.ones(2, 8)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(call, (x,), check_trace=False)
+    for options in ({}, {"pre_dispatch": True}, {"tracing_mode": "fake"}):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            make_fx(call, **options)(x)
+    with FakeTensorMode(), pytest.raises(RuntimeError, match="cannot be traced"):
+        call(torch.ones(2, 8))
+    with pytest.raises(ValueError, match="CUDA"):  # (and not for good)
+        call(x)
 
 
 def test_layer_norm_in_c_refuses():
