@@ -414,3 +414,18 @@ def test_tracers_of_a_backward_pass_are_refused():
     with pytest.raises(RuntimeError, match="cannot be traced"):
         torch.jit.trace(FusedLayerNorm(64).cuda(), (x,))
     assert torch.autograd.grad(y, x, dy)[0].isfinite().all()
+
+
+def test_gradients_with_a_tangent_are_refused():
+    """Forward mode over reverse mode: the gradient would come without its tangent."""
+    x, r = (torch.randn(4, 64, device="cuda", requires_grad=True) for _ in range(2))
+    dy = torch.randn(4, 64, device="cuda")
+    y, s = layer_norm(x, residual=r)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(dy, dy.clone())
+        for out in (y, s):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(out, x, dual, retain_graph=True)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            layer_norm(torch.autograd.forward_ad.make_dual(x.detach(), dy))
+        torch.autograd.grad(y, x, dy)
