@@ -101,6 +101,10 @@ void RefuseDual(const Tensor& t) {
 struct LayerNormBackward : public torch::autograd::Node {
   torch::autograd::SavedVariable s, weight, stats;
   bool add = false;  // there was a residual
+  bool has_weight = false;
+  at::ScalarType type = at::kFloat;  // of s
+  std::vector<int64_t> sizes;
+  at::Device where = at::kCPU;
   at::ScalarType parameter_type = at::kFloat;
 
   std::string name() const override { return "LayerNormBackward"; }
@@ -112,14 +116,30 @@ struct LayerNormBackward : public torch::autograd::Node {
     stats.reset_data();
   }
 
+  // What the forward pass has saved, as the kernels take it. It may come back as another tensor: from hooks on saved tensors, and
+  // because a leaf is saved as itself, of which .data may have been exchanged.
+  Tensor Unpacked(const torch::autograd::SavedVariable& saved, const char* name, at::ScalarType its_type, at::IntArrayRef its_sizes,
+                  std::shared_ptr<torch::autograd::Node> node = nullptr) const {
+    const Tensor t = saved.unpack(std::move(node));
+    TORCH_CHECK(t.defined() && t.layout() == at::kStrided && t.scalar_type() == its_type && t.sizes() == its_sizes && t.device() == where,
+                "layer_norm: the ", name, " that the backward pass finds is not what the forward pass saved: ", its_type, " ", its_sizes, " on ", where);
+    return t.contiguous();
+  }
+
   // Edges: x, residual, weight, bias; those of tensors that are not there lead nowhere.
   variable_list apply(variable_list&& grads) override {
     RefuseTracing("layer_norm");
     TORCH_CHECK(!at::GradMode::is_enabled(), "layer_norm has no gradient of its gradient (create_graph)");
     for (const Tensor& t : grads) RefuseDual(t);
     std::lock_guard<std::mutex> lock(mutex_);
-    const Tensor s_ = s.unpack(add ? shared_from_this() : nullptr), weight_ = weight.unpack(), stats_ = stats.unpack();
-    const c10::cuda::OptionalCUDAGuard device(s_.device());
+    const c10::cuda::OptionalCUDAGuard device(where);
+    const int64_t n = sizes.back(), rows = c10::multiply_integers(sizes) / n;
+    const Tensor s_ = Unpacked(s, "input", type, sizes, add ? shared_from_this() : nullptr);
+    const Tensor stats_ = Unpacked(stats, "statistics", at::kFloat, {2, rows});
+    const Tensor weight_ = has_weight ? Unpacked(weight, "weight", parameter_type, {n}) : Tensor();
+    for (const Tensor& t : grads)
+      TORCH_CHECK(!t.defined() || (t.layout() == at::kStrided && t.scalar_type() == type && t.sizes() == sizes && t.device() == where),
+                  "layer_norm: a gradient is ", t.scalar_type(), " ", t.sizes(), " on ", t.device(), ", the input ", type, " ", sizes, " on ", where);
     const bool want_weight = task_should_compute_output(2), want_bias = task_should_compute_output(3);
     const Tensor dsum = grads.size() > 1 && grads[1].defined() ? grads[1].contiguous() : Tensor();
     variable_list out(4);
@@ -128,7 +148,6 @@ struct LayerNormBackward : public torch::autograd::Node {
       dx = dsum;
     } else {
       const Tensor dy = grads[0].contiguous();
-      const int64_t n = s_.size(-1), rows = s_.numel() / n;
       dx = at::empty_like(s_);
       if (want_weight) out[2] = at::empty({n}, s_.options().dtype(parameter_type));
       if (want_bias) out[3] = at::empty({n}, s_.options().dtype(parameter_type));
@@ -185,6 +204,8 @@ variable_list LayerNormForward(Tensor x, OptTensor residual, const OptTensor& we
   const std::shared_ptr<LayerNormBackward> node(new LayerNormBackward(), torch::autograd::deleteNode);
   node->set_next_edges(torch::autograd::collect_next_edges(x, residual.value_or(Tensor()), weight.value_or(Tensor()), bias.value_or(Tensor())));
   node->add = residual.has_value();
+  node->has_weight = r.weight.defined();
+  node->type = r.x.scalar_type(), node->sizes = r.x.sizes().vec(), node->where = r.x.device();
   if (r.weight.defined()) node->parameter_type = r.weight.scalar_type();
   else if (r.bias.defined()) node->parameter_type = r.bias.scalar_type();
   variable_list out = residual ? variable_list{r.y, r.sum} : variable_list{r.y};

@@ -3,6 +3,7 @@ import ctypes
 
 import pytest
 import torch
+import torch.utils.checkpoint
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from _train_reference import check, layer_norm64
@@ -429,3 +430,57 @@ def test_gradients_with_a_tangent_are_refused():
         with pytest.raises(RuntimeError, match="forward-mode"):
             layer_norm(torch.autograd.forward_ad.make_dual(x.detach(), dy))
         torch.autograd.grad(y, x, dy)
+
+
+def backward_through_hooks(change, residual=False):
+    """Gradients of x, weight and bias where hooks give back `change` of every saved tensor."""
+    _, dev = make((6, 64), BF16, F32, residual, True)
+    leaves = [dev[k].requires_grad_() for k in ("x", "weight", "bias")]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+        out = layer_norm(dev["x"], dev["weight"], dev["bias"], residual=dev["residual"])
+    return torch.autograd.grad(out[0] if residual else out, leaves, dev["dy"])
+
+
+@pytest.mark.parametrize("residual", [False, True])
+def test_saved_tensors_that_come_back_in_another_layout(residual):
+    def apart(t):
+        return torch.stack([t, t + 1], -1)[..., 0]
+
+    assert all(torch.equal(a, b) for a, b in zip(backward_through_hooks(apart, residual), backward_through_hooks(lambda t: t, residual)))
+
+
+# (Only what is as large as the saved tensor or larger, and of no narrower type than it says: the refusal is what is tested.)
+@pytest.mark.parametrize("change", [lambda t: t.double(), lambda t: t.cpu(), lambda t: torch.cat([t, t]), lambda t: t.unsqueeze(0), lambda t: t.int()])
+def test_saved_tensors_that_come_back_as_others_are_refused(change):
+    for dims, dtype in ((1, F32), (2, F32), (2, BF16)):  # weight, statistics, x
+        # (Whole numbers in the place of what requires a gradient are refused by autograd before the node sees them.)
+        with pytest.raises(RuntimeError, match="not what the forward pass saved|can require gradients"):
+            backward_through_hooks(lambda t: change(t) if (t.dim(), t.dtype) == (dims, dtype) else t)
+
+
+def test_data_exchanged_between_the_passes_is_refused():
+    x, w = torch.randn(4, 64, device="cuda", requires_grad=True), torch.ones(64, device="cuda", requires_grad=True)
+    for leaf, other_leaf in ((x, w), (w, x)):  # (another type takes the exchanged one itself out of the graph)
+        y, keep = layer_norm(x, w), leaf.data
+        for other in (keep.bfloat16(), torch.cat([keep, keep])):
+            leaf.data = other
+            with pytest.raises(RuntimeError, match="not what the forward pass saved"):
+                torch.autograd.grad(y, other_leaf, torch.ones_like(y), retain_graph=True)
+        leaf.data = keep
+        torch.autograd.grad(y, other_leaf, torch.ones_like(y))
+
+
+def test_saved_tensors_on_the_cpu_and_recomputed():
+    _, dev = make((6, 64), BF16, F32, True, True)
+    leaves = [dev[k].requires_grad_() for k in ("x", "residual", "weight", "bias")]
+
+    def grads(f=lambda f, *a: f(*a)):
+        def norm(x, r, w, b):
+            return layer_norm(x, w, b, residual=r)
+        return torch.autograd.grad(f(norm, *leaves), leaves, (dev["dy"], dev["ds"]))
+
+    want = grads()
+    with torch.autograd.graph.save_on_cpu():
+        got = grads()
+    again = grads(lambda f, *a: torch.utils.checkpoint.checkpoint(f, *a, use_reentrant=False))
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, got, again))
