@@ -579,6 +579,10 @@ int GradNorm(const SmlNormTensor* tensors, int count, double* workspace, int* ti
   return Launched(LaunchOverlapped(FinishNormKernel, 1, kNormThreads, 0, 1, stream, a.all, a.parts, out));
 }
 
+bool At(const void* p, unsigned multiple) { return reinterpret_cast<uintptr_t>(p) % multiple == 0; }
+
+unsigned SizeOf(int type) { return type == SML_ADAMW_F32 ? 4 : 2; }
+
 }  // namespace
 
 extern "C" int switchml_adamw_step(const SmlAdamwTensor* tensors, int count, const SmlAdamwState* state, const SmlAdamwStep* step,
@@ -587,8 +591,14 @@ extern "C" int switchml_adamw_step(const SmlAdamwTensor* tensors, int count, con
       !state->steps || !state->ticket || (state->bits == 8 && (!state->exp_avg_scale || !state->exp_avg_sq_scale)) ||
       (type != SML_ADAMW_F32 && (type != SML_ADAMW_BF16 || !state->remainder)))
     return -1;
+  const unsigned vector = state->bits == 32 ? 32 : 8;
+  if (!At(state->exp_avg, vector) || !At(state->exp_avg_sq, vector) || !At(state->remainder, 16) || !At(state->steps, 4) ||
+      !At(state->ticket, 4) || !At(step->lr_tensor, 4) || !At(step->norm, 4))
+    return -1;
   for (int i = 0; i < count; i++)
-    if (tensors[i].numel < 0 || tensors[i].numel > kMaxNumel || (tensors[i].numel && (!tensors[i].param || !tensors[i].grad))) return -1;
+    if (tensors[i].numel < 0 || tensors[i].numel > kMaxNumel || (tensors[i].numel && (!tensors[i].param || !tensors[i].grad)) ||
+        !At(tensors[i].param, SizeOf(type)) || !At(tensors[i].grad, SizeOf(type)))
+      return -1;
   StepFactors a;
   a.state = *state;
   a.lr = static_cast<float>(step->lr);
@@ -604,9 +614,11 @@ extern "C" int switchml_adamw_step(const SmlAdamwTensor* tensors, int count, con
 }
 
 extern "C" int switchml_adamw_masters(const SmlAdamwTensor* tensors, int count, const short* remainder, float* out, int type, void* stream) {
-  if (!tensors || count < 0 || !out || (type != SML_ADAMW_F32 && (type != SML_ADAMW_BF16 || !remainder))) return -1;
+  if (!tensors || count < 0 || !out || (type != SML_ADAMW_F32 && (type != SML_ADAMW_BF16 || !remainder)) || !At(out, 32) || !At(remainder, 16))
+    return -1;
   for (int i = 0; i < count; i++)
-    if (tensors[i].numel < 0 || tensors[i].numel > kMaxNumel || (tensors[i].numel && !tensors[i].param)) return -1;
+    if (tensors[i].numel < 0 || tensors[i].numel > kMaxNumel || (tensors[i].numel && !tensors[i].param) || !At(tensors[i].param, SizeOf(type)))
+      return -1;
   if (count <= kFewTensors) return Masters<kFewTensors>(tensors, count, remainder, out, type, static_cast<cudaStream_t>(stream));
   return Masters<kMaxTensors>(tensors, count, remainder, out, type, static_cast<cudaStream_t>(stream));
 }
@@ -616,10 +628,10 @@ extern "C" long long switchml_grad_norm_workspace(int count) {
 }
 
 extern "C" int switchml_grad_norm(const SmlNormTensor* tensors, int count, double* workspace, int* ticket, float* out, void* stream) {
-  if (count < 0 || !out || !workspace || (count && !tensors)) return -1;
+  if (count < 0 || !out || !workspace || (count && !tensors) || !At(out, 4) || !At(workspace, 8) || !At(ticket, 4)) return -1;
   for (int i = 0; i < count; i++)
     if (tensors[i].numel < 0 || tensors[i].numel > kMaxNumel || (tensors[i].numel && !tensors[i].data) ||
-        (tensors[i].type != SML_ADAMW_F32 && tensors[i].type != SML_ADAMW_BF16))
+        (tensors[i].type != SML_ADAMW_F32 && tensors[i].type != SML_ADAMW_BF16) || !At(tensors[i].data, SizeOf(tensors[i].type)))
       return -1;
   if (count <= kFewTensors) return GradNorm<kFewTensors>(tensors, count, workspace, ticket, out, static_cast<cudaStream_t>(stream));
   return GradNorm<kMaxTensors>(tensors, count, workspace, ticket, out, static_cast<cudaStream_t>(stream));

@@ -19,6 +19,9 @@
  * remainder taken as signed. What else writes to the parameter is off by half of a bf16 step at most; nothing
  * takes the parameter back to what it was.
  *
+ * Parameters and gradients lie at any multiple of their element. Flat buffers are read in whole vectors: fp32 ones (moments with
+ * bits = 32, what switchml_adamw_masters writes) begin at a multiple of 32 bytes, remainders of 16, moments with bits = 8 of 8.
+ *
  * Return 0, or < 0: -1 bad argument, -4 launch.
  */
 #ifndef SWITCHML_ADAMW_H_

@@ -69,6 +69,60 @@ def test_layer_norm_in_c_refuses():
     assert backward(8, dweight=p) == -1  # (no workspace)
 
 
+class _Tensor(ctypes.Structure):
+    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("numel", ctypes.c_longlong), ("place", ctypes.c_uint),
+                ("step", ctypes.c_int)]
+
+
+class _State(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "remainder", "steps", "ticket")] + \
+               [("bits", ctypes.c_int), ("seed", ctypes.c_uint), ("first", ctypes.c_ulonglong)]
+
+
+class _Step(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "decay")] + \
+               [("lr_tensor", ctypes.c_void_p), ("norm", ctypes.c_void_p), ("max_norm", ctypes.c_float)]
+
+
+class _NormTensor(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("numel", ctypes.c_longlong), ("type", ctypes.c_int)]
+
+
+def test_adamw_in_c_refuses_addresses():
+    """Flat buffers that whole vectors cannot be read from. (Calls that are in order have no tensors: they launch nothing.)"""
+    lib = ctypes.CDLL(library_path("libswitchml_train.so"))
+    good = {"exp_avg": 4096, "exp_avg_sq": 8192, "exp_avg_scale": 1, "exp_avg_sq_scale": 3, "remainder": 16, "steps": 4, "ticket": 8}
+
+    def step(bits, type, tensors=(), lr_tensor=None, norm=None, **state):
+        array = (_Tensor * 2)(*tensors)
+        return lib.switchml_adamw_step(array, len(tensors), ctypes.byref(_State(**{**good, **state}, bits=bits)),
+                                       ctypes.byref(_Step(lr_tensor=lr_tensor, norm=norm)), type, None)
+
+    for bits, multiple in ((32, 32), (8, 8)):
+        for type, size in ((0, 4), (1, 2)):
+            assert step(bits, type) == 0 and step(bits, type, exp_avg=64 + multiple, lr_tensor=4, norm=8) == 0
+            for name in ("exp_avg", "exp_avg_sq"):
+                for off in {1, 4, multiple // 2}:
+                    assert step(bits, type, **{name: 4096 + off}) == -1
+            assert step(bits, type, remainder=24) == -1
+            for name in ("steps", "ticket", "lr_tensor", "norm"):
+                assert step(bits, type, **{name: 6}) == -1
+            for param, grad in ((64 + size // 2, 64), (64, 64 + size // 2)):
+                assert step(bits, type, [(param, grad, 8, 0, 0)]) == -1
+
+    def masters(out, remainder, type, tensors=()):
+        return lib.switchml_adamw_masters((_Tensor * 2)(*tensors), len(tensors), ctypes.c_void_p(remainder), ctypes.c_void_p(out), type, None)
+
+    assert masters(32, 16, 1) == 0 and masters(32, None, 0) == 0
+    assert masters(16, 16, 1) == -1 and masters(16, None, 0) == -1 and masters(32, 8, 1) == -1
+    assert masters(32, 16, 1, [(65, None, 8, 0, 0)]) == -1 and masters(32, 16, 0, [(66, None, 8, 0, 0)]) == -1
+
+    def norm(data, type, workspace=8, ticket=None, out=4):
+        return lib.switchml_grad_norm((_NormTensor * 1)((data, 8, type)), 1, ctypes.c_void_p(workspace), ctypes.c_void_p(ticket), ctypes.c_void_p(out), None)
+
+    assert norm(65, 1) == -1 and norm(66, 0) == -1 and norm(64, 0, workspace=4) == -1 and norm(64, 0, ticket=2) == -1 and norm(64, 0, out=2) == -1
+
+
 def test_grad_norm_refuses():
     with pytest.raises(ValueError):
         grad_norm([])
