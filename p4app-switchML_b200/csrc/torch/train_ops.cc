@@ -269,6 +269,7 @@ struct Group {
   std::vector<Tensor> params;
   std::vector<int64_t> numel, place;  // place: in units of SML_ADAMW_ALIGN values
   std::vector<at::ScalarType> type;
+  std::vector<std::vector<int64_t>> sizes, strides;  // as the state lies; empty for contiguous parameters
   Tensor exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, remainder, steps;
   int64_t first = 0;
 };
@@ -280,7 +281,11 @@ class Adamw {
   void AddGroup(std::vector<Tensor> params, std::vector<int64_t> place, Tensor exp_avg, Tensor exp_avg_sq, OptTensor exp_avg_scale,
                 OptTensor exp_avg_sq_scale, OptTensor remainder, Tensor steps, int64_t first) {
     Group g;
-    for (const Tensor& p : params) g.numel.push_back(p.numel()), g.type.push_back(p.scalar_type());
+    for (const Tensor& p : params) {
+      g.numel.push_back(p.numel()), g.type.push_back(p.scalar_type());
+      g.sizes.push_back(p.is_contiguous() ? std::vector<int64_t>() : p.sizes().vec());
+      g.strides.push_back(p.is_contiguous() ? std::vector<int64_t>() : p.strides().vec());
+    }
     g.params = std::move(params), g.place = std::move(place);
     g.exp_avg = std::move(exp_avg), g.exp_avg_sq = std::move(exp_avg_sq), g.steps = std::move(steps), g.first = first;
     g.exp_avg_scale = exp_avg_scale.value_or(Tensor()), g.exp_avg_sq_scale = exp_avg_sq_scale.value_or(Tensor());
@@ -375,6 +380,17 @@ class Adamw {
     const Tensor& p = g.params[i];
     TORCH_CHECK(p.numel() == g.numel[i] && Dense(p) && p.scalar_type() == g.type[i] && p.device() == ticket_.device(),
                 "FusedAdamW: a parameter has another size, type or device than when its state was made, or gaps in memory");
+    TORCH_CHECK(SameOrder(g, i), "FusedAdamW: a parameter's values lie in another order than when its state was made (sizes ", p.sizes(),
+                ", strides ", p.strides(), "): a memory format is chosen before the optimizer is made");
+  }
+  // Values and state meet by their places in memory.
+  static bool SameOrder(const Group& g, size_t i) {
+    const Tensor& p = g.params[i];
+    if (g.sizes[i].empty()) return p.is_contiguous();
+    if (p.sizes() != g.sizes[i]) return false;
+    for (int64_t d = 0; d < p.dim(); d++)
+      if (p.size(d) > 1 && p.stride(d) != g.strides[i][d]) return false;
+    return true;
   }
   static void CheckGrad(const Tensor& p, const Tensor& grad) {
     TORCH_CHECK(grad.layout() == at::kStrided, "FusedAdamW: a gradient is ", grad.layout(), ": strided is wanted");

@@ -40,7 +40,8 @@ class FusedAdamW(torch.optim.Optimizer):
     that share their scale with them. The ``.grad`` of the parameters stays as it is.
 
     State is allocated when a group is added, and ``load_state_dict`` copies into it, so that captured steps
-    stay valid. Counts of steps are kept on the device, one per parameter: a parameter without a gradient
+    stay valid. It lies as the parameters do then: a memory format is chosen before the optimizer is made, and a
+    parameter that has changed its own is refused. Counts of steps are kept on the device, one per parameter: a parameter without a gradient
     takes no step. One step at a time: steps of one optimizer on several streams have to be ordered by the caller.
     """
 
@@ -237,7 +238,7 @@ class FusedAdamW(torch.optim.Optimizer):
             copies[0].append(new)
             copies[1].append(old)
             return
-        flat = torch.empty_strided(p.shape, p.stride(), dtype=torch.float32, device=p.device).copy_(old).as_strided((p.numel(),), (1,))
+        flat = torch.empty_strided(new.shape, new.stride(), dtype=torch.float32, device=p.device).copy_(old).as_strided((p.numel(),), (1,))
         blocks = torch.nn.functional.pad(flat, (0, -p.numel() % _SCALED)).view(-1, _SCALED)
         exponent = (blocks.abs().amax(1).view(torch.int32) >> 23).clamp_(min=8)
         codes = (blocks * ((261 - exponent).clamp_(min=1) << 23).view(torch.float32).unsqueeze(1)).to(torch.float8_e4m3fn).view(torch.uint8)

@@ -590,3 +590,37 @@ def test_tracers_are_refused():
         with pytest.raises(RuntimeError, match="cannot be traced"):
             make_fx(call)(p.grad)
     assert int(opt.state[p]["step"]) == 0 and not p.any()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_another_memory_format_than_the_state_has(bits):
+    """Refused: moments would meet other values' gradients. A format chosen before goes on as it is."""
+    torch.manual_seed(0)
+    for before, after in ((torch.contiguous_format, torch.channels_last), (torch.channels_last, torch.contiguous_format)):
+        layer = torch.nn.Conv2d(4, 5, 3).cuda().to(memory_format=before)
+        opt = FusedAdamW(layer.parameters(), state_bits=bits)
+        checker = Checker(opt, bits)
+        for p in layer.parameters():
+            p.grad = torch.randn_like(p)
+        checker.step()
+        layer.to(memory_format=after)
+        for call in (opt.step, opt.master_buffers):
+            with pytest.raises(RuntimeError, match="another order"):
+                call()
+        assert all(int(opt.state[p]["step"]) == 1 for p in layer.parameters())
+        layer.to(memory_format=before)
+        checker.step()
+    # Formats that are the same order of values, and contiguous tensors of other sizes, are no change.
+    p = torch.randn(6, 4, 1, 1, device="cuda", requires_grad=True)
+    opt = FusedAdamW([p], state_bits=bits)
+    for data in (p.data.to(memory_format=torch.channels_last), p.data.as_strided(p.shape, (4, 1, 7, 9)), p.data.view(4, 6)):
+        p.grad = None
+        p.data = data
+        p.grad = torch.randn_like(p)
+        opt.step()
+        opt.master_buffers()
+    p.grad = None
+    p.data = p.data.t()
+    p.grad = torch.randn_like(p)
+    with pytest.raises(RuntimeError, match="another order"):
+        opt.step()
