@@ -177,6 +177,8 @@ __device__ __forceinline__ unsigned VCode(float y, float v, unsigned hash) {
   return v > 0.f ? max(code, 1u << 24) : code;
 }
 constexpr unsigned kNanCode = 0x7f;
+// A mask of the first n of four bytes (all of them from 4 on, none up to 0).
+__device__ __forceinline__ unsigned BytesBelow(int n) { return n >= 4 ? ~0u : n <= 0 ? 0u : (1u << 8 * n) - 1; }
 
 // 8 numbers in e4m3.
 struct Packed8 {
@@ -218,7 +220,8 @@ template <bool kWhole, class T> __device__ __forceinline__ void StoreTensor(T* t
 }
 
 // kBlock values of a tensor from k on: 8 neighbours per lane, a scale for 4 lanes. State is there for whole blocks, and what
-// lies behind a tensor's end in it stays 0 (with the smallest scale).
+// lies behind a tensor's end in it stays 0, also where a block of moments becomes NaN: a good state that is loaded into the
+// tensor's part of the block would be lost to what shares its scale.
 template <class T, int kBits, bool kWhole>
 __device__ __forceinline__ void StepBlock(const StepFactors& a, const SmlAdamwTensor& x, long long k, long long state, const Factors& f,
                                           float clip, int lane) {
@@ -267,7 +270,13 @@ __device__ __forceinline__ void StepBlock(const StepFactors& a, const SmlAdamwTe
     }
   }
   StoreTensor<kWhole>(param, valid, p);
-  if constexpr (sizeof(T) == 2) StoreWords(a.state.remainder + state, r.w);
+  if constexpr (sizeof(T) == 2) {
+    if constexpr (!kWhole) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) r.w[i] = valid > 2 * i + 1 ? r.w[i] : valid > 2 * i ? r.w[i] & 0xffffu : 0;
+    }
+    StoreWords(a.state.remainder + state, r.w);
+  }
   if constexpr (kBits == 8) {
     float largest_m = 0.f, largest_v = 0.f;
 #pragma unroll
@@ -298,6 +307,11 @@ __device__ __forceinline__ void StepBlock(const StepFactors& a, const SmlAdamwTe
     }
     if (em == 255) m.w[0] = m.w[1] = kNanCode * 0x01010101u;
     if (ev == 255) v.w[0] = v.w[1] = kNanCode * 0x01010101u;
+    if constexpr (!kWhole) {
+      const unsigned low = BytesBelow(valid), high = BytesBelow(valid - 4);
+      m.w[0] &= low, m.w[1] &= high;
+      v.w[0] &= low, v.w[1] &= high;
+    }
     if (lane % (kScaled / 8) == 0) {
       a.state.exp_avg_scale[state / kScaled] = ScaleByte(em);
       a.state.exp_avg_sq_scale[state / kScaled] = ScaleByte(ev);

@@ -624,3 +624,54 @@ def test_another_memory_format_than_the_state_has(bits):
     p.grad = torch.randn_like(p)
     with pytest.raises(RuntimeError, match="another order"):
         opt.step()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("path", ["as it is", "from 32 bits", "anew"])
+def test_a_good_state_loaded_behind_values_that_were_not_finite(path, dtype):
+    """Sizes that leave a block of moments with a few of the tensor's values: nothing of the bad ones is left in the others."""
+    sizes = [7, 33, 1000, 256, 1]
+    start = make(sizes, dtype)
+    source = FusedAdamW(start, lr=1e-2, state_bits=32 if path == "from 32 bits" else 8, seed=5)
+    source.step()
+    good = copy.deepcopy(source.state_dict())
+    if path == "anew":
+        good["state"] = {}
+    results = []
+    for bad in (False, True):
+        params = [p.detach().clone().requires_grad_() for p in start]
+        opt = FusedAdamW(params, lr=1e-2, state_bits=8, seed=5)
+        if bad:
+            for p in params:
+                p.grad = torch.full_like(p, float("nan"))
+            opt.step()
+            opt.step()
+            assert all(p.isnan().all() for p in params)
+            for p, q in zip(params, start):
+                p.data.copy_(q)
+        opt.load_state_dict(good)
+        for i in range(3):
+            for p, q in zip(params, start):
+                p.grad = q.grad * (1 - 0.4 * i)
+            opt.step()
+        assert all(p.isfinite().all() for p in params)
+        (masters,), (state,) = opt.master_buffers(), opt.state_buffers()
+        at = 0
+        for n in sizes:
+            end = at + -(-n // 256) * 256
+            for flat in [masters, state["exp_avg"].view(torch.uint8), state["exp_avg_sq"].view(torch.uint8)] + \
+                    ([state["remainder"]] if dtype == BF16 else []):
+                assert not flat[at + n:end].any()
+            at = end
+        results.append(params + [masters] + [state[k].view(torch.uint8) for k in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_remainders_behind_the_end_where_the_learning_rate_is_not_finite():
+    params = make([5, 300], BF16)
+    opt = FusedAdamW(params, lr=torch.tensor(float("nan"), device="cuda"))
+    opt.step()
+    (masters,), (state,) = opt.master_buffers(), opt.state_buffers()
+    assert masters[:5].isnan().all() and masters[256:556].isnan().all()
+    for flat in (masters, state["remainder"]):
+        assert not flat[5:256].any() and not flat[556:].any()
