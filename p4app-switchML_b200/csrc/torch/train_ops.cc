@@ -48,6 +48,10 @@ void RefuseTracing(const char* what) {
               what, " cannot be traced");
 }
 
+void RefuseDual(const Tensor& t, const char* what) {
+  TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), what, " has no forward-mode gradient");
+}
+
 // ---- layer norm ----
 
 constexpr int64_t kMaxFeatures = 1 << 30;
@@ -92,10 +96,6 @@ Normed Normalize(const Tensor& x_in, const OptTensor& residual_in, const OptTens
   return r;
 }
 
-void RefuseDual(const Tensor& t) {
-  TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "layer_norm has no forward-mode gradient");
-}
-
 // A node of its own: with torch::autograd::Function forward and backward of a small input took 73 us of host time, where the
 // engine alone takes 35.
 struct LayerNormBackward : public torch::autograd::Node {
@@ -130,7 +130,7 @@ struct LayerNormBackward : public torch::autograd::Node {
   variable_list apply(variable_list&& grads) override {
     RefuseTracing("layer_norm");
     TORCH_CHECK(!at::GradMode::is_enabled(), "layer_norm has no gradient of its gradient (create_graph)");
-    for (const Tensor& t : grads) RefuseDual(t);
+    for (const Tensor& t : grads) RefuseDual(t, "layer_norm");
     std::lock_guard<std::mutex> lock(mutex_);
     const c10::cuda::OptionalCUDAGuard device(where);
     const int64_t n = sizes.back(), rows = c10::multiply_integers(sizes) / n;
@@ -174,7 +174,7 @@ struct LayerNormBackward : public torch::autograd::Node {
 variable_list LayerNormForward(Tensor x, OptTensor residual, const OptTensor& weight, const OptTensor& bias, double eps) {
   RefuseTracing("layer_norm");
   // (A dual tensor need not require a gradient: this is asked whether a backward pass comes or not.)
-  for (const Tensor& t : {x, residual.value_or(Tensor()), weight.value_or(Tensor()), bias.value_or(Tensor())}) RefuseDual(t);
+  for (const Tensor& t : {x, residual.value_or(Tensor()), weight.value_or(Tensor()), bias.value_or(Tensor())}) RefuseDual(t, "layer_norm");
   const bool autocast = x.is_cuda() && at::autocast::is_autocast_enabled(at::kCUDA);
   c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::DispatchKey::AutocastCUDA);
   if (autocast) {
@@ -241,6 +241,7 @@ Tensor GradNorm(const py::list& tensors) {
   std::vector<Tensor> keep;
   list.reserve(count);
   at::Device where(at::kCPU);
+  const bool grad_mode = at::GradMode::is_enabled();
   at::NoGradGuard no_grad;
   std::optional<c10::cuda::CUDAGuard> device;
   for (Py_ssize_t i = 0; i < count; i++) {
@@ -249,6 +250,9 @@ Tensor GradNorm(const py::list& tensors) {
     const Tensor* t = &THPVariable_Unpack(item);
     TORCH_CHECK_TYPE(t->layout() == at::kStrided && Known(*t), "grad_norm: a tensor is ", t->layout(), " ", t->scalar_type(),
                      ": strided float32 or bfloat16 is wanted");
+    RefuseDual(*t, "grad_norm");
+    TORCH_CHECK(!grad_mode || !t->requires_grad(),
+                "grad_norm has no gradient: a tensor that requires one is wanted detached, or the call under no_grad");
     if (i == 0) where = t->device();
     TORCH_CHECK_VALUE(t->is_cuda() && t->device() == where, "grad_norm: tensors on ", where, " and ", t->device(), ": one CUDA device is wanted");
     if (i == 0) device.emplace(where);

@@ -26,7 +26,8 @@ def _ops():
 
 def grad_norm(tensors):
     """The 2-norm over all values of `tensors` (float32, bfloat16; of one CUDA device) as a float32 tensor without
-    dimensions on that device: summed in float64 and in a fixed order."""
+    dimensions on that device: summed in float64 and in a fixed order. It has no gradient: tensors that require one are
+    refused while gradients are recorded, so that none is lost (a penalty on gradients that were made with ``create_graph``)."""
     return _ops().grad_norm(list(tensors))
 
 

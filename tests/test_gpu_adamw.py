@@ -675,3 +675,13 @@ def test_remainders_behind_the_end_where_the_learning_rate_is_not_finite():
     assert masters[:5].isnan().all() and masters[256:556].isnan().all()
     for flat in (masters, state["remainder"]):
         assert not flat[5:256].any() and not flat[556:].any()
+
+
+def test_grad_norm_of_what_requires_a_gradient():
+    w = torch.randn(1000, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad((w ** 3).sum(), w, create_graph=True)
+    with pytest.raises(RuntimeError, match="has no gradient"):
+        grad_norm([g])
+    with torch.no_grad():
+        got = grad_norm([g])
+    assert torch.equal(got, grad_norm([g.detach()])) and not got.requires_grad

@@ -134,6 +134,20 @@ def test_grad_norm_refuses():
         grad_norm([torch.eye(3).to_sparse()])
 
 
+def test_grad_norm_refuses_what_would_want_a_gradient():
+    w = torch.ones(3, requires_grad=True)
+    g, = torch.autograd.grad((w ** 3).sum(), w, create_graph=True)
+    for bad in (w, g):
+        with pytest.raises(RuntimeError, match="has no gradient"):
+            grad_norm([bad])
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+            grad_norm([bad])
+        with pytest.raises(ValueError, match="CUDA"):
+            grad_norm([bad.detach()])
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        grad_norm([torch.autograd.forward_ad.make_dual(w.detach(), torch.ones(3))])
+
+
 @pytest.mark.parametrize("options", [{"state_bits": 16}, {"max_norm": 0.0}, {"max_norm": float("nan")}, {"seed": -1}, {"seed": 1 << 32},
                                      {}, {"lr": -1.0}])
 def test_adamw_refuses(options):
