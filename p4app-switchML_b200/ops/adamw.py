@@ -175,11 +175,21 @@ class FusedAdamW(torch.optim.Optimizer):
         self._native.step(settings, tensors, self._max_norm)
         return loss
 
-    @torch.no_grad()
     def load_state_dict(self, state_dict):
         """Copies `state_dict` into the state. Moments may come in the other form (those of
         ``torch.optim.AdamW`` among them): they are converted, to 8 bits by rounding to the nearest. A parameter
         that it says nothing about starts anew."""
+        state_dict = dict(state_dict)  # hooks may change it, not the caller's
+        for hook in list(self._optimizer_load_state_dict_pre_hooks.values()):
+            changed = hook(self, state_dict)
+            if changed is not None:
+                state_dict = changed
+        self._load_all(state_dict)
+        for hook in list(self._optimizer_load_state_dict_post_hooks.values()):
+            hook(self)
+
+    @torch.no_grad()
+    def _load_all(self, state_dict):
         groups = state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("the state is that of other groups of parameters")

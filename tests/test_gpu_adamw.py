@@ -685,3 +685,32 @@ def test_grad_norm_of_what_requires_a_gradient():
     with torch.no_grad():
         got = grad_norm([g])
     assert torch.equal(got, grad_norm([g.detach()])) and not got.requires_grad
+
+
+def test_hooks_around_loading_a_state():
+    """As around torch.optim.AdamW's: in their order, what the first ones return is loaded, the caller's dict stays."""
+    p = make([300], F32)[0]
+    for kind in (torch.optim.AdamW, FusedAdamW):
+        opt, ran = kind([p], lr=1e-3), []
+        opt.step()
+        state = opt.state_dict()
+
+        def other_rate(o, d):
+            assert o is opt and d["param_groups"][0]["lr"] == 1e-3
+            ran.append("pre")
+            return {"state": d["state"], "param_groups": [{**d["param_groups"][0], "lr": 0.5}]}
+
+        def without_state(o, d):
+            assert d["param_groups"][0]["lr"] == 0.5
+            ran.append("pre 2")
+            d["state"] = {}
+
+        opt.register_load_state_dict_pre_hook(other_rate)
+        removed = opt.register_load_state_dict_pre_hook(lambda o, d: ran.append("removed"))
+        opt.register_load_state_dict_pre_hook(without_state)
+        opt.register_load_state_dict_post_hook(lambda o: ran.append(("post", o.param_groups[0]["lr"])))
+        removed.remove()
+        opt.load_state_dict(state)
+        assert ran == ["pre", "pre 2", ("post", 0.5)]
+        assert not opt.state[p] or int(opt.state[p]["step"]) == 0
+        assert state["state"] and state["param_groups"][0]["lr"] == 1e-3
