@@ -18,6 +18,9 @@ from .._native import native_extension
 
 _MOMENTS = ("exp_avg", "exp_avg_sq")
 _SCALED = 32  # values that share a scale
+# Options of torch.optim.AdamW that would make another step: a group that has one, from a checkpoint say, is refused. (The others say
+# how it computes, or, as decoupled_weight_decay, are set aside by torch.optim.AdamW too.)
+_OTHER_STEPS = ("amsgrad", "maximize", "differentiable")
 
 
 def _ops():
@@ -79,6 +82,12 @@ class FusedAdamW(torch.optim.Optimizer):
     def __getstate__(self):
         raise TypeError("FusedAdamW is neither copied nor pickled: take its state_dict()")
 
+    @staticmethod
+    def _check_options(group):
+        for name in _OTHER_STEPS:
+            if group.get(name):
+                raise ValueError("FusedAdamW has no %s" % name)
+
     def _check(self, group, device):
         lr, betas = group["lr"], group["betas"]
         if isinstance(lr, torch.Tensor):
@@ -96,6 +105,7 @@ class FusedAdamW(torch.optim.Optimizer):
         device = self._device
         if not params:
             raise ValueError("a group has no parameters")
+        self._check_options(group)
         for p in params:
             if p.dtype not in (torch.float32, torch.bfloat16):
                 raise TypeError("a parameter is %s: float32 or bfloat16 is wanted" % p.dtype)
@@ -164,6 +174,7 @@ class FusedAdamW(torch.optim.Optimizer):
                 loss = closure()
         settings, tensors = [], []
         for group in self.param_groups:
+            self._check_options(group)
             lr, (beta1, beta2), eps, decay = group["lr"], group["betas"], group["eps"], group["weight_decay"]
             tensor = isinstance(lr, torch.Tensor)
             now = (0.0 if tensor else lr, beta1, beta2, eps, decay)
@@ -193,6 +204,8 @@ class FusedAdamW(torch.optim.Optimizer):
         groups = state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("the state is that of other groups of parameters")
+        for group in groups:
+            self._check_options(group)
         plans = []
         for saved, group in zip(groups, self.param_groups):
             for key, p in zip(saved["params"], group["params"]):

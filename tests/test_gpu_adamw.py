@@ -714,3 +714,30 @@ def test_hooks_around_loading_a_state():
         assert ran == ["pre", "pre 2", ("post", 0.5)]
         assert not opt.state[p] or int(opt.state[p]["step"]) == 0
         assert state["state"] and state["param_groups"][0]["lr"] == 1e-3
+
+
+@pytest.mark.parametrize("option", ["amsgrad", "maximize", "differentiable"])
+def test_options_that_make_another_step_are_refused(option):
+    """From a checkpoint too, before anything of it is loaded; where they are off it is."""
+    p, q = make([300, 5], F32)
+    other = torch.optim.AdamW([q], lr=0.5)
+    other.step()
+    state = other.state_dict()
+    opt = FusedAdamW([q], lr=1e-3)
+    state["param_groups"][0][option] = True
+    with pytest.raises(ValueError, match=option):
+        opt.load_state_dict(state)
+    assert opt.param_groups[0]["lr"] == 1e-3 and int(opt.state[q]["step"]) == 0
+    state["param_groups"][0][option] = False
+    opt.load_state_dict(state)
+    assert opt.param_groups[0]["lr"] == 0.5 and int(opt.state[q]["step"]) == 1
+    with pytest.raises(ValueError, match=option):
+        opt.add_param_group({"params": [p], option: True})
+    assert len(opt.param_groups) == 1
+    opt.param_groups[0][option] = True
+    with pytest.raises(ValueError, match=option):
+        opt.step()
+    assert int(opt.state[q]["step"]) == 1
+    opt.param_groups[0][option] = False
+    opt.step()
+    assert int(opt.state[q]["step"]) == 2

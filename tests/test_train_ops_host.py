@@ -155,6 +155,14 @@ def test_adamw_refuses(options):
         FusedAdamW([torch.nn.Parameter(torch.zeros(4))], **options)
 
 
+@pytest.mark.parametrize("option", ["amsgrad", "maximize", "differentiable"])
+def test_adamw_refuses_options_of_torch_s(option):
+    with pytest.raises(ValueError, match=option):
+        FusedAdamW([{"params": [torch.nn.Parameter(torch.zeros(4))], option: True}])
+    with pytest.raises(ValueError, match="CUDA"):
+        FusedAdamW([{"params": [torch.nn.Parameter(torch.zeros(4))], option: False}])
+
+
 def test_adamw_refuses_types():
     with pytest.raises(TypeError):
         FusedAdamW([torch.nn.Parameter(torch.zeros(4, dtype=torch.float16))])
