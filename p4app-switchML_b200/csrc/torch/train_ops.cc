@@ -179,8 +179,9 @@ variable_list LayerNormForward(Tensor x, OptTensor residual, const OptTensor& we
   c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::DispatchKey::AutocastCUDA);
   if (autocast) {
     const auto type = at::autocast::get_autocast_dtype(at::kCUDA);
-    if (x.is_floating_point()) x = x.to(type);
-    if (residual && residual->is_floating_point()) residual = residual->to(type);
+    const auto cast = [&](const Tensor& t) { return t.is_floating_point() && t.scalar_type() != at::kDouble ? t.to(type) : t; };
+    x = cast(x);
+    if (residual) residual = cast(*residual);
   }
   TORCH_CHECK_TYPE(Known(x), "layer_norm: x is ", x.scalar_type(), ": float32 or bfloat16 is wanted");
   TORCH_CHECK_VALUE(x.is_cuda(), "layer_norm: x is on ", x.device(), ": a CUDA device is wanted");

@@ -5,9 +5,9 @@
 
 float32 and bfloat16; weight and bias (each may be None) are float32 or of the type of x. Statistics and
 gradients are summed in float32, the gradients of weight and bias in a fixed order: the same bits in every
-run. Under autocast x and the residual are cast to its type, as a linear layer casts its input. Inputs that are not
-contiguous are copied first. Gradients of gradients, forward-mode gradients
-and calls under a tracer (``torch.jit.trace``, ``make_fx``, ``torch.export``) are refused.
+run. Under autocast x and the residual are cast to its type, as a linear layer casts its input (which leaves float64
+alone: that type is refused). Inputs that are not contiguous are copied first. Gradients of gradients, forward-mode
+gradients and calls under a tracer (``torch.jit.trace``, ``make_fx``, ``torch.export``) are refused.
 """
 import torch
 

@@ -484,3 +484,14 @@ def test_saved_tensors_on_the_cpu_and_recomputed():
         got = grads()
     again = grads(lambda f, *a: torch.utils.checkpoint.checkpoint(f, *a, use_reentrant=False))
     assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, got, again))
+
+
+def test_autocast_leaves_float64_alone():
+    """As for a linear layer; the type is refused then, as without autocast."""
+    x = torch.randn(4, 64, device="cuda")
+    with torch.autocast("cuda", torch.bfloat16):
+        assert torch.nn.functional.linear(x.double(), x.double()).dtype == torch.float64
+        for args, kw in (((x.double(),), {}), ((x,), {"residual": x.double()}), ((x.double(),), {"residual": x})):
+            with pytest.raises((TypeError, ValueError)):
+                layer_norm(*args, **kw)
+        assert layer_norm(x.half(), residual=x)[1].dtype == BF16
