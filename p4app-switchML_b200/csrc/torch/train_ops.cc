@@ -36,6 +36,15 @@ int NormType(const Tensor& t) { return t.scalar_type() == at::kFloat ? SML_NORM_
 
 void* Data(const Tensor& t) { return t.defined() ? const_cast<void*>(t.const_data_ptr()) : nullptr; }
 
+// Whether the memory of a tensor does not hold its values: a view that says they are to be negated (imag() of a conjugate), or
+// zeros that autograd has not written out.
+bool Implied(const Tensor& t) { return t.is_neg() || t._is_zerotensor(); }
+
+Tensor Written(const Tensor& t) { return at::zeros(t.sizes(), t.options()).copy_(t); }
+
+// As the kernels read it.
+Tensor Contiguous(const Tensor& t) { return Implied(t) ? Written(t) : t.contiguous(); }
+
 // What records operations to run them again (torch.jit.trace, make_fx, export) sees the allocation of a result here, but not the
 // kernel that writes it: the recording would return memory that nothing has written.
 void RefuseTracing(const char* what) {
@@ -77,10 +86,10 @@ Normed Normalize(const Tensor& x_in, const OptTensor& residual_in, const OptTens
   const c10::cuda::OptionalCUDAGuard device(x_in.device());
   const bool add = residual_in.has_value();
   Normed r;
-  r.x = x_in.contiguous();
-  const Tensor residual = add ? residual_in->contiguous() : Tensor();
-  if (weight_in) r.weight = weight_in->contiguous();
-  if (bias_in) r.bias = bias_in->contiguous();
+  r.x = Contiguous(x_in);
+  const Tensor residual = add ? Contiguous(*residual_in) : Tensor();
+  if (weight_in) r.weight = Contiguous(*weight_in);
+  if (bias_in) r.bias = Contiguous(*bias_in);
   const int64_t n = r.x.size(-1), rows = r.x.numel() / n;
   r.y = at::empty_like(r.x);
   if (add) r.sum = at::empty_like(r.x);
@@ -123,7 +132,7 @@ struct LayerNormBackward : public torch::autograd::Node {
     const Tensor t = saved.unpack(std::move(node));
     TORCH_CHECK(t.defined() && t.layout() == at::kStrided && t.scalar_type() == its_type && t.sizes() == its_sizes && t.device() == where,
                 "layer_norm: the ", name, " that the backward pass finds is not what the forward pass saved: ", its_type, " ", its_sizes, " on ", where);
-    return t.contiguous();
+    return Contiguous(t);
   }
 
   // Edges: x, residual, weight, bias; those of tensors that are not there lead nowhere.
@@ -141,13 +150,13 @@ struct LayerNormBackward : public torch::autograd::Node {
       TORCH_CHECK(!t.defined() || (t.layout() == at::kStrided && t.scalar_type() == type && t.sizes() == sizes && t.device() == where),
                   "layer_norm: a gradient is ", t.scalar_type(), " ", t.sizes(), " on ", t.device(), ", the input ", type, " ", sizes, " on ", where);
     const bool want_weight = task_should_compute_output(2), want_bias = task_should_compute_output(3);
-    const Tensor dsum = grads.size() > 1 && grads[1].defined() ? grads[1].contiguous() : Tensor();
+    const Tensor dsum = grads.size() > 1 && grads[1].defined() ? Contiguous(grads[1]) : Tensor();
     variable_list out(4);
     Tensor dx;
     if (!grads[0].defined()) {  // only the sum was used
       dx = dsum;
     } else {
-      const Tensor dy = grads[0].contiguous();
+      const Tensor dy = Contiguous(grads[0]);
       dx = at::empty_like(s_);
       if (want_weight) out[2] = at::empty({n}, s_.options().dtype(parameter_type));
       if (want_bias) out[3] = at::empty({n}, s_.options().dtype(parameter_type));
@@ -257,8 +266,8 @@ Tensor GradNorm(const py::list& tensors) {
     if (i == 0) where = t->device();
     TORCH_CHECK_VALUE(t->is_cuda() && t->device() == where, "grad_norm: tensors on ", where, " and ", t->device(), ": one CUDA device is wanted");
     if (i == 0) device.emplace(where);
-    if (!Dense(*t)) {
-      keep.push_back(t->contiguous());
+    if (!Dense(*t) || Implied(*t)) {
+      keep.push_back(Contiguous(*t));
       t = &keep.back();
     }
     list.push_back({Data(*t), t->numel(), AdamwType(*t)});
@@ -326,7 +335,7 @@ class Adamw {
           if (!grad.defined()) continue;
           CheckParam(g, i);
           CheckGrad(p, grad);
-          if (!(p.is_contiguous() && grad.is_contiguous()) && p.strides() != grad.strides()) {
+          if ((!(p.is_contiguous() && grad.is_contiguous()) && p.strides() != grad.strides()) || Implied(grad)) {
             grad = at::empty_strided(p.sizes(), p.strides(), grad.options()).copy_(grad);
             keep.push_back(grad);
           }
@@ -383,7 +392,7 @@ class Adamw {
   // What a parameter's storage has become: p.data may have been exchanged.
   void CheckParam(const Group& g, size_t i) const {
     const Tensor& p = g.params[i];
-    TORCH_CHECK(p.numel() == g.numel[i] && Dense(p) && p.scalar_type() == g.type[i] && p.device() == ticket_.device(),
+    TORCH_CHECK(p.numel() == g.numel[i] && Dense(p) && !Implied(p) && p.scalar_type() == g.type[i] && p.device() == ticket_.device(),
                 "FusedAdamW: a parameter has another size, type or device than when its state was made, or gaps in memory");
     TORCH_CHECK(SameOrder(g, i), "FusedAdamW: a parameter's values lie in another order than when its state was made (sizes ", p.sizes(),
                 ", strides ", p.strides(), "): a memory format is chosen before the optimizer is made");

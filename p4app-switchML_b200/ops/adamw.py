@@ -111,8 +111,8 @@ class FusedAdamW(torch.optim.Optimizer):
                 raise TypeError("a parameter is %s: float32 or bfloat16 is wanted" % p.dtype)
             if p.layout != torch.strided or not p.is_cuda or (device or p.device) != p.device:
                 raise ValueError("a parameter is %s on %s: strided on one CUDA device is wanted" % (p.layout, p.device))
-            if not torch.ops.aten.is_non_overlapping_and_dense(p):
-                raise ValueError("a parameter of the shape %s has gaps or overlaps in memory" % (tuple(p.shape),))
+            if not torch.ops.aten.is_non_overlapping_and_dense(p) or p.is_neg():
+                raise ValueError("a parameter of the shape %s has gaps or overlaps in memory, or is a negated view" % (tuple(p.shape),))
             device = p.device
         # Tensors are taken side by side: two that share memory would be written by both.
         ends = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size())

@@ -741,3 +741,23 @@ def test_options_that_make_another_step_are_refused(option):
     opt.param_groups[0][option] = False
     opt.step()
     assert int(opt.state[q]["step"]) == 2
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_gradients_that_are_to_be_negated(bits):
+    """A single value is contiguous as imag() of a conjugate: its memory holds the opposite of it."""
+    params = [torch.zeros(n, device="cuda", requires_grad=True) for n in (1, 300)]
+    params[0].grad = torch.complex(torch.zeros(1), torch.full((1,), 2.0)).cuda().conj().imag
+    params[1].grad = torch._neg_view(torch.full((300,), 2.0, device="cuda"))
+    assert params[0].grad.is_neg() and params[0].grad.is_contiguous() and params[1].grad.is_neg()
+    opt = FusedAdamW(params, lr=1e-2, state_bits=bits, max_norm=1e6)
+    opt.step()
+    assert (params[0] > 0).all() and (params[1] > 0).all()
+    assert float(grad_norm([p.grad for p in params])) == pytest.approx(2 * 301 ** 0.5, rel=1e-6) == float(opt.grad_norm)
+    with pytest.raises(ValueError, match="negated"):
+        FusedAdamW([torch._neg_view(torch.zeros(8, device="cuda")).requires_grad_()])
+    params[1].grad = None
+    params[1].data = torch._neg_view(torch.zeros(300, device="cuda"))
+    params[1].grad = torch.ones(300, device="cuda")
+    with pytest.raises(RuntimeError):
+        opt.step()

@@ -495,3 +495,27 @@ def test_autocast_leaves_float64_alone():
             with pytest.raises((TypeError, ValueError)):
                 layer_norm(*args, **kw)
         assert layer_norm(x.half(), residual=x)[1].dtype == BF16
+
+
+def test_views_that_are_to_be_negated():
+    """Tensors whose memory holds the opposite of their values (as imag() of a conjugate gives them)."""
+    _, dev = make((6, 64), BF16, F32, True, True)
+
+    def grads(change):
+        data = {k: change(v) for k, v in dev.items()}
+        leaves = [data[k].requires_grad_() for k in ("x", "residual", "weight", "bias")]
+        out = layer_norm(data["x"], data["weight"], data["bias"], residual=data["residual"])
+        return out + torch.autograd.grad(out, leaves, (data["dy"], data["ds"]))
+
+    want = grads(lambda t: t.detach().clone())
+    got = grads(lambda t: torch._neg_view(-t.detach()))
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_gradients_of_zeros_that_are_not_written_out():
+    x, r = (torch.randn(4, 64, device="cuda", requires_grad=True) for _ in range(2))
+    out = layer_norm(x, residual=r)
+    for zeros in (torch._efficientzerotensor((4, 64), device="cuda"), torch.zeros(4, 64, device="cuda")):
+        for grads in ((zeros, None), (None, zeros), (zeros, zeros)):
+            got = torch.autograd.grad([o for o, g in zip(out, grads) if g is not None], (x, r), [g for g in grads if g is not None], retain_graph=True)
+            assert all(g.shape == x.shape and not g.any() for g in got)
