@@ -34,7 +34,13 @@ bool Known(const Tensor& t) { return t.scalar_type() == at::kFloat || t.scalar_t
 
 int NormType(const Tensor& t) { return t.scalar_type() == at::kFloat ? SML_NORM_F32 : SML_NORM_BF16; }
 
-void* Data(const Tensor& t) { return t.defined() ? const_cast<void*>(t.const_data_ptr()) : nullptr; }
+// (Null says that a tensor is not there: one that is, but has no memory, must not look like that.)
+void* Data(const Tensor& t) {
+  if (!t.defined()) return nullptr;
+  void* const data = const_cast<void*>(t.const_data_ptr());
+  TORCH_CHECK(data || !t.numel(), "a tensor of the shape ", t.sizes(), " has no memory");
+  return data;
+}
 
 // Whether the memory of a tensor does not hold its values: a view that says they are to be negated (imag() of a conjugate), or
 // zeros that autograd has not written out.

@@ -519,3 +519,11 @@ def test_gradients_of_zeros_that_are_not_written_out():
         for grads in ((zeros, None), (None, zeros), (zeros, zeros)):
             got = torch.autograd.grad([o for o, g in zip(out, grads) if g is not None], (x, r), [g for g in grads if g is not None], retain_graph=True)
             assert all(g.shape == x.shape and not g.any() for g in got)
+
+
+def test_weight_without_memory_is_refused():
+    """It must not count as one that is not there."""
+    x, weight = torch.randn(4, 64, device="cuda"), torch.randn(64, device="cuda")
+    weight.untyped_storage().resize_(0)
+    with pytest.raises(RuntimeError, match="no memory"):
+        layer_norm(x, weight)
