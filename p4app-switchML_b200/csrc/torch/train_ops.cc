@@ -375,7 +375,10 @@ class Adamw {
     RefuseTracing("FusedAdamW");
     const c10::cuda::OptionalCUDAGuard device(ticket_.device());
     const Group& g = groups_.at(k);
-    Tensor out = at::empty({g.exp_avg.numel()}, g.exp_avg.options().dtype(at::kFloat));
+    const auto options = g.exp_avg.options().dtype(at::kFloat);
+    // (A group of empty tensors has a block of state too, which belongs to none of them.)
+    const bool any = std::any_of(g.numel.begin(), g.numel.end(), [](int64_t n) { return n > 0; });
+    Tensor out = any ? at::empty({g.exp_avg.numel()}, options) : at::zeros({g.exp_avg.numel()}, options);
     for (const int type : {SML_ADAMW_F32, SML_ADAMW_BF16}) {
       tensors_.clear();
       for (size_t i = 0; i < g.params.size(); i++) {

@@ -761,3 +761,10 @@ def test_gradients_that_are_to_be_negated(bits):
     params[1].grad = torch.ones(300, device="cuda")
     with pytest.raises(RuntimeError):
         opt.step()
+
+
+def test_masters_of_empty_tensors():
+    opt = FusedAdamW([torch.empty(0, 3, device="cuda", requires_grad=True)])
+    junk = torch.full((256,), 5.0, device="cuda")
+    del junk  # (its memory is what comes next)
+    assert not opt.master_buffers()[0].any()
