@@ -313,7 +313,7 @@ class Adamw {
     // Steps may have been captured with the workspace that there was: it stays.
     count_ += g.params.size();
     workspaces_.push_back(NormWorkspace(count_, g.exp_avg.options()));
-    if (!ticket_.defined()) {
+    if (!norm_.defined()) {  // (the last one that is made)
       ticket_ = at::zeros({1}, g.exp_avg.options().dtype(at::kInt));
       norm_ = at::zeros({}, g.exp_avg.options().dtype(at::kFloat));
     }

@@ -139,10 +139,10 @@ class FusedAdamW(torch.optim.Optimizer):
             if any(p.dtype == torch.bfloat16 for p in params):
                 flat["remainder"] = torch.zeros(values, dtype=torch.int16, device=device)
             steps = torch.zeros(len(params), dtype=torch.int32, device=device)
+            states = {}
             for i, (p, place) in enumerate(zip(params, places)):
                 at, n = place * align, p.numel()
-                state = self.state[p]
-                state["step"] = steps[i]
+                state = states[p] = {"step": steps[i]}
                 for name in _MOMENTS:
                     state[name] = flat[name][at:at + n].as_strided(p.shape, p.stride())
                     if self._bits == 8:
@@ -151,6 +151,7 @@ class FusedAdamW(torch.optim.Optimizer):
                     state["remainder"] = flat["remainder"][at:at + n].as_strided(p.shape, p.stride())
         self._native.add_group(params, places, flat["exp_avg"], flat["exp_avg_sq"], flat.get("exp_avg_scale"),
                                flat.get("exp_avg_sq_scale"), flat.get("remainder"), steps, self._values)
+        self.state.update(states)
         self._device = device
         self._values += values
         self._buffers.append(flat)

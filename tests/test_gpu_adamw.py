@@ -768,3 +768,23 @@ def test_masters_of_empty_tensors():
     junk = torch.full((256,), 5.0, device="cuda")
     del junk  # (its memory is what comes next)
     assert not opt.master_buffers()[0].any()
+
+
+def test_a_group_that_could_not_be_added_leaves_nothing():
+    params = make([10, 300], F32)
+    opt = FusedAdamW(params[:1])
+    native = opt._native
+
+    class Full:
+        def add_group(self, *args):
+            raise torch.OutOfMemoryError("no room")
+
+    opt._native = Full()
+    with pytest.raises(torch.OutOfMemoryError):
+        opt.add_param_group({"params": params[1:]})
+    opt._native = native
+    assert len(opt.param_groups) == 1 and list(opt.state_dict()["state"]) == [0]
+    opt.step()
+    opt.add_param_group({"params": params[1:]})
+    opt.step()
+    assert [int(s["step"]) for s in opt.state_dict()["state"].values()] == [2, 1]
