@@ -45,6 +45,7 @@ constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr int kBlock = SML_ADAMW_ALIGN;  // values that a warp takes at once: 8 per lane
 constexpr int kScaled = 32;              // values that share a scale
 constexpr long long kMaxNumel = 1ll << 38;  // of a tensor: the number of its tiles fits 31 bits
+constexpr long long kMaxTiles = 0x7fffffff;  // of a launch
 constexpr int kMaxTensors = SML_ADAMW_TENSORS;
 constexpr int kFewTensors = 32;          // a launch of so few takes kernel parameters of 1 instead of 12 KB
 
@@ -517,7 +518,7 @@ unsigned TakeTensors(const Tensor* tensors, int count, long long tile, int* at, 
   *taken = 0;
   for (; *at < count && *taken < kMax; ++*at) {
     const unsigned long long more = static_cast<unsigned long long>((tensors[*at].numel + tile - 1) / tile);
-    if (tiles + more > 0x7fffffffull && *taken > 0) break;
+    if (tiles + more > kMaxTiles && *taken > 0) break;
     a->tensor[*taken] = tensors[*at];
     a->first_tile[(*taken)++] = static_cast<unsigned>(tiles);
     tiles += more;
@@ -643,10 +644,14 @@ extern "C" long long switchml_grad_norm_workspace(int count) {
 
 extern "C" int switchml_grad_norm(const SmlNormTensor* tensors, int count, double* workspace, int* ticket, float* out, void* stream) {
   if (count < 0 || !out || !workspace || (count && !tensors) || !At(out, 4) || !At(workspace, 8) || !At(ticket, 4)) return -1;
-  for (int i = 0; i < count; i++)
+  long long tiles = 0;  // (as many as a launch takes: the workspace is for launches that end with their table of tensors)
+  for (int i = 0; i < count; i++) {
     if (tensors[i].numel < 0 || tensors[i].numel > kMaxNumel || (tensors[i].numel && !tensors[i].data) ||
         (tensors[i].type != SML_ADAMW_F32 && tensors[i].type != SML_ADAMW_BF16) || !At(tensors[i].data, SizeOf(tensors[i].type)))
       return -1;
+    tiles += (tensors[i].numel + kNormTile - 1) / kNormTile;
+    if (tiles > kMaxTiles) return -1;
+  }
   if (count <= kFewTensors) return GradNorm<kFewTensors>(tensors, count, workspace, ticket, out, static_cast<cudaStream_t>(stream));
   return GradNorm<kMaxTensors>(tensors, count, workspace, ticket, out, static_cast<cudaStream_t>(stream));
 }

@@ -81,8 +81,8 @@ typedef struct SmlNormTensor {
 
 /* Doubles of workspace for `count` tensors. */
 long long switchml_grad_norm_workspace(int count);
-/* out = sqrt of the sum of squares of all tensors, summed in fp64; the same bits in every run. `workspace` need not be
- * initialised. `ticket`: one int, zero between launches, saves a launch; or NULL. */
+/* out = sqrt of the sum of squares of all tensors, summed in fp64; the same bits in every run. At most 2^43 values in all.
+ * `workspace` need not be initialised. `ticket`: one int, zero between launches, saves a launch; or NULL. */
 int switchml_grad_norm(const SmlNormTensor* tensors, int count, double* workspace, int* ticket, float* out, void* stream);
 
 #ifdef __cplusplus

@@ -123,6 +123,14 @@ def test_adamw_in_c_refuses_addresses():
     assert norm(65, 1) == -1 and norm(66, 0) == -1 and norm(64, 0, workspace=4) == -1 and norm(64, 0, ticket=2) == -1 and norm(64, 0, out=2) == -1
 
 
+def test_grad_norm_in_c_refuses_what_its_workspace_is_not_for():
+    """More tiles of 8192 values than one launch counts: tensors that share memory, which no GPU could hold side by side."""
+    lib = ctypes.CDLL(library_path("libswitchml_train.so"))
+    tensors = (_NormTensor * 384)(*[(64, 1 << 38, 1)] * 384)
+    for count in (64, 65, 384):
+        assert lib.switchml_grad_norm(tensors, count, ctypes.c_void_p(64), None, ctypes.c_void_p(64), None) == -1
+
+
 def test_grad_norm_refuses():
     with pytest.raises(ValueError):
         grad_norm([])
