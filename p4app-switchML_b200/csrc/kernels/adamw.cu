@@ -364,6 +364,7 @@ __global__ void __launch_bounds__(kThreads, kBits == 8 ? 7 : 8) AdamwKernel(cons
   }
   __syncthreads();
   if (!last) return;
+  __threadfence();  // (every block's reads of the counts lie before its turn at the ticket)
   for (int i = threadIdx.x; i < all.count; i += kThreads) all.state.steps[a.tensor[i].step]++;
   if (threadIdx.x == 0) *all.state.ticket = 0;
 }
