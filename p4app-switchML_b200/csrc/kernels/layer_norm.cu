@@ -611,18 +611,18 @@ BackwardAnyKernel(const T* dy, const T* dsum, const T* s, Parameter weight, cons
   }
 }
 
-// Sums over rows: a block takes 32 columns and one of gridDim.y shares of the rows; its sums go to the workspace.
+// Sums over rows: a block takes 32 columns, a warp every 8th row of them. Rows that no cluster holds have more than 65536 values, so
+// there are more than 2048 blocks, and shares of the rows would find no SM free.
 template <class T>
 __global__ void __launch_bounds__(kAnyThreads)
 ColumnsAnyKernel(const T* dy, const T* s, const float* mean, const float* rstd, float* workspace, long long rows, int n) {
   __shared__ float2 part[kAnyThreads / 32][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, column = blockIdx.x * 32 + lane;
-  const long long first = rows * blockIdx.y / gridDim.y, last = rows * (blockIdx.y + 1) / gridDim.y;
   float dw = 0.f, db = 0.f;
   WaitForEarlierKernels();
   if (column < n) {
 #pragma unroll 4
-    for (long long row = first + warp; row < last; row += kAnyThreads / 32) {
+    for (long long row = warp; row < rows; row += kAnyThreads / 32) {
       const float g = ToFloat(dy[row * n + column]);
       dw += g * ((ToFloat(s[row * n + column]) - mean[row]) * rstd[row]);
       db += g;
@@ -634,9 +634,8 @@ ColumnsAnyKernel(const T* dy, const T* s, const float* mean, const float* rstd, 
     float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kAnyThreads / 32; w++) sum.x += part[w][lane].x, sum.y += part[w][lane].y;
-    float* out = workspace + static_cast<long long>(blockIdx.y) * 2 * n;
-    out[column] = sum.x;
-    out[n + column] = sum.y;
+    workspace[column] = sum.x;
+    workspace[n + column] = sum.y;
   }
 }
 
@@ -679,13 +678,6 @@ FinishColumnsKernel(const float* workspace, void* dweight, void* dbias, int part
 }
 
 unsigned RowBlocks(long long rows) { return static_cast<unsigned>(rows < (1 << 20) ? rows : (1 << 20)); }
-
-int RowShares(long long rows, int n) {
-  const long long columns = (static_cast<long long>(n) + 31) / 32;
-  long long shares = (148 * 8 + columns - 1) / columns;
-  if (shares > rows / 32 + 1) shares = rows / 32 + 1;
-  return static_cast<int>(shares);
-}
 
 // Columns are counted in 32 bits, beyond a row's end too.
 bool Fits(int features) { return features > 0 && features <= 1 << 30; }
@@ -816,9 +808,8 @@ int Backward(const void* dy_in, const void* dsum_in, const void* s_in, Parameter
   } else {
     e = LaunchOverlapped(BackwardAnyKernel<T>, RowBlocks(rows), kAnyThreads, 0, 1, stream, dy, dsum, s, weight, mean, rstd, dx, rows, n);
     if (e == cudaSuccess && workspace) {
-      parts = RowShares(rows, n);
-      const unsigned columns = static_cast<unsigned>((static_cast<long long>(n) + 31) / 32);
-      ColumnsAnyKernel<T><<<dim3(columns, parts), kAnyThreads, 0, stream>>>(dy, s, mean, rstd, workspace, rows, n);
+      parts = 1;
+      ColumnsAnyKernel<T><<<(n - 1) / 32 + 1, kAnyThreads, 0, stream>>>(dy, s, mean, rstd, workspace, rows, n);
       e = cudaGetLastError();
     }
   }
@@ -843,7 +834,7 @@ extern "C" long long switchml_layer_norm_workspace(long long rows, int features,
   // (Which it will be depends on the addresses too.)
   const Geometry g = BackwardGeometry(rows, features, 8), h = BackwardGeometry(rows, features, 16);
   const int held = g.parts > h.parts ? g.parts : h.parts;
-  return 2ll * features * (h.lanes ? held : RowShares(rows, features));
+  return 2ll * features * (h.lanes ? held : 1);
 }
 
 extern "C" int switchml_layer_norm_backward(const void* dy, const void* dsum, const void* s, const void* weight, const float* mean,

@@ -527,3 +527,10 @@ def test_weight_without_memory_is_refused():
     weight.untyped_storage().resize_(0)
     with pytest.raises(RuntimeError, match="no memory"):
         layer_norm(x, weight)
+
+
+@pytest.mark.parametrize("dtype,wtype", [(F32, F32), (BF16, F32), (BF16, BF16)])
+@pytest.mark.parametrize("rows,features", [(75, 65537), (300, 70001), (9, 65568), (8, 131072)])
+def test_many_rows_that_no_cluster_holds(rows, features, dtype, wtype):
+    """Warps that add several rows of a column, and a last block of columns that is not full."""
+    run_and_check(*make((rows, features), dtype, wtype, rows % 2 == 0, True, seed=rows), 1e-5, True)
