@@ -42,6 +42,9 @@ void* Data(const Tensor& t) {
   return data;
 }
 
+// For a kernel that writes: a lazy clone of the tensor gets its own memory first.
+void* Writable(const Tensor& t) { return Data(t) ? t.mutable_data_ptr() : nullptr; }
+
 // Whether the memory of a tensor does not hold its values: a view that says they are to be negated (imag() of a conjugate), or
 // zeros that autograd has not written out.
 bool Implied(const Tensor& t) { return t.is_neg() || t._is_zerotensor(); }
@@ -345,7 +348,7 @@ class Adamw {
             grad = at::empty_strided(p.sizes(), p.strides(), grad.options()).copy_(grad);
             keep.push_back(grad);
           }
-          tensors_.push_back({Data(p), Data(grad), g.numel[i], static_cast<unsigned>(g.place[i]), static_cast<int>(i)});
+          tensors_.push_back({Writable(p), Data(grad), g.numel[i], static_cast<unsigned>(g.place[i]), static_cast<int>(i)});
           if (max_norm) norms_.push_back({Data(grad), g.numel[i], type});
         }
         if (tensors_.size() > begin) runs.push_back({k, {begin, tensors_.size(), type}});
@@ -354,9 +357,8 @@ class Adamw {
     if (max_norm) NormOf(norms_, workspaces_.back(), ticket_.data_ptr<int>(), norm_);
     for (const auto& [k, run] : runs) {
       const Group& g = groups_[k];
-      const auto bytes = [](const Tensor& t) { return static_cast<unsigned char*>(Data(t)); };
-      const SmlAdamwState state{Data(g.exp_avg), Data(g.exp_avg_sq), bytes(g.exp_avg_scale), bytes(g.exp_avg_sq_scale),
-                                static_cast<short*>(Data(g.remainder)), g.steps.data_ptr<int>(), ticket_.data_ptr<int>(), bits_, seed_, static_cast<unsigned long long>(g.first)};
+      const SmlAdamwState state{Writable(g.exp_avg), Writable(g.exp_avg_sq), static_cast<unsigned char*>(Writable(g.exp_avg_scale)),
+                                static_cast<unsigned char*>(Writable(g.exp_avg_sq_scale)), static_cast<short*>(Writable(g.remainder)), g.steps.data_ptr<int>(), ticket_.data_ptr<int>(), bits_, seed_, static_cast<unsigned long long>(g.first)};
       const auto& s = settings[k];
       const SmlAdamwStep step{s[0], s[1], s[2], s[3], s[4], lr_tensors[k] ? lr_tensors[k]->const_data_ptr<float>() : nullptr,
                               max_norm ? norm_.data_ptr<float>() : nullptr, static_cast<float>(max_norm.value_or(0.0))};

@@ -788,3 +788,17 @@ def test_a_group_that_could_not_be_added_leaves_nothing():
     opt.add_param_group({"params": params[1:]})
     opt.step()
     assert [int(s["step"]) for s in opt.state_dict()["state"].values()] == [2, 1]
+
+
+def test_lazy_clones_of_a_parameter_stay_as_they_are():
+    p, q = make([300, 40], F32)
+    kept, before = torch._lazy_clone(p.detach()), p.detach().clone()
+    opt = FusedAdamW([p, q])
+    opt.step()
+    assert torch.equal(kept, before) and not torch.equal(p, before)
+    moments = opt.state[p]["exp_avg"]
+    for t in (p.detach(), moments):
+        kept = torch._lazy_clone(t)
+        before = kept.clone()
+        opt.step()
+        assert torch.equal(kept, before) and not torch.equal(t, before)
