@@ -682,6 +682,10 @@ unsigned RowBlocks(long long rows) { return static_cast<unsigned>(rows < (1 << 2
 // Columns are counted in 32 bits, beyond a row's end too.
 bool Fits(int features) { return features > 0 && features <= 1 << 30; }
 
+// Whether all of them lie at multiples of their element (null does).
+template <class... Pointers> bool Aligned(unsigned size, Pointers... p) { return ((reinterpret_cast<uintptr_t>(p) % size == 0) && ...); }
+unsigned SizeOf(int type) { return type == SML_NORM_F32 ? 4 : 2; }
+
 bool Known(int type) { return type == SML_NORM_F32 || type == SML_NORM_BF16; }
 
 // Values that are read and written at once: what the length of the rows and all addresses allow.
@@ -824,6 +828,7 @@ extern "C" int switchml_layer_norm_forward(const void* x, const void* residual, 
                                            void* sum, float* mean, float* rstd, long long rows, int features, float eps, int type,
                                            int wtype, void* stream) {
   if (!x || !y || (residual && !sum) || !mean != !rstd || rows <= 0 || !Fits(features) || !Known(type) || !Known(wtype)) return -1;
+  if (!Aligned(SizeOf(type), x, residual, y, sum) || !Aligned(SizeOf(wtype), weight, bias) || !Aligned(4, mean, rstd)) return -1;
   return (type == SML_NORM_F32 ? Forward<float> : Forward<__nv_bfloat16>)(x, residual, Parameter{weight, wtype},
                                                                           Parameter{bias, wtype}, y, sum, mean, rstd, rows, features,
                                                                           eps, static_cast<cudaStream_t>(stream));
@@ -843,6 +848,7 @@ extern "C" int switchml_layer_norm_backward(const void* dy, const void* dsum, co
   if (!dy || !s || !mean || !rstd || !dx || ((dweight || dbias) && !workspace) || rows <= 0 || !Fits(features) || !Known(type) ||
       !Known(wtype))
     return -1;
+  if (!Aligned(SizeOf(type), dy, dsum, s, dx) || !Aligned(SizeOf(wtype), weight, dweight, dbias) || !Aligned(4, mean, rstd, workspace)) return -1;
   return (type == SML_NORM_F32 ? Backward<float> : Backward<__nv_bfloat16>)(dy, dsum, s, Parameter{weight, wtype}, mean, rstd, dx,
                                                                             dweight, dbias, workspace, rows, features, wtype,
                                                                             static_cast<cudaStream_t>(stream));

@@ -5,7 +5,7 @@
  *
  * x, residual, y, sum, dy, dsum, dx: [rows, features], contiguous, all of `type`. weight and bias: [features] of `wtype`,
  * each may be NULL (ones and zeros). mean and rstd: one fp32 per row. Types: SML_NORM_F32, SML_NORM_BF16.
- * All pointers are aligned to their element; up to 2^30 features. Statistics and sums are fp32.
+ * All pointers are aligned to their element (others are refused); up to 2^30 features. Statistics and sums are fp32.
  * Return 0, or < 0: -1 bad argument, -4 launch.
  */
 #ifndef SWITCHML_LAYER_NORM_H_

@@ -69,6 +69,21 @@ def test_layer_norm_in_c_refuses():
     assert backward(8, dweight=p) == -1  # (no workspace)
 
 
+def test_layer_norm_in_c_refuses_addresses_between_elements():
+    lib = ctypes.CDLL(library_path("libswitchml_train.so"))
+    rows, eps = ctypes.c_longlong(1), ctypes.c_float(1e-5)
+    for type, wtype in ((0, 0), (1, 0), (1, 1)):
+        sizes = {"x": type, "residual": type, "weight": wtype, "bias": wtype, "y": type, "sum": type, "mean": 0, "rstd": 0}
+        for bad, kind in sizes.items():
+            at = {name: ctypes.c_void_p(64 + (name == bad) * (1 if kind else 2)) for name in sizes}
+            assert lib.switchml_layer_norm_forward(*at.values(), rows, 8, eps, type, wtype, None) == -1, bad
+        sizes = {"dy": type, "dsum": type, "s": type, "weight": wtype, "mean": 0, "rstd": 0, "dx": type, "dweight": wtype, "dbias": wtype,
+                 "workspace": 0}
+        for bad, kind in sizes.items():
+            at = {name: ctypes.c_void_p(64 + (name == bad) * (1 if kind else 2)) for name in sizes}
+            assert lib.switchml_layer_norm_backward(*at.values(), rows, 8, type, wtype, None) == -1, bad
+
+
 class _Tensor(ctypes.Structure):
     _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("numel", ctypes.c_longlong), ("place", ctypes.c_uint),
                 ("step", ctypes.c_int)]
