@@ -220,17 +220,21 @@ template <bool kWhole, class T> __device__ __forceinline__ void StoreTensor(T* t
   }
 }
 
+// What is known of a block of kBlock values: whole, at addresses that vectors can be read from or at any other; or a tensor's last.
+enum class Block { kVectors, kSingles, kEnd };
+
 // kBlock values of a tensor from k on: 8 neighbours per lane, a scale for 4 lanes. State is there for whole blocks, and what
 // lies behind a tensor's end in it stays 0, also where a block of moments becomes NaN: a good state that is loaded into the
 // tensor's part of the block would be lost to what shares its scale.
-template <class T, int kBits, bool kWhole>
+template <class T, int kBits, Block kIs>
 __device__ __forceinline__ void StepBlock(const StepFactors& a, const SmlAdamwTensor& x, long long k, long long state, const Factors& f,
                                           float clip, int lane) {
   using M = std::conditional_t<kBits == 32, Packed<float>, Packed8>;
   constexpr int kMoment = kBits / 8;
+  constexpr bool kWhole = kIs == Block::kVectors;
   k += lane * 8;
   state += k;
-  const int valid = static_cast<int>(max(min(x.numel - k, 8ll), 0ll));
+  const int valid = kIs == Block::kEnd ? static_cast<int>(max(min(x.numel - k, 8ll), 0ll)) : 8;
   T* const param = static_cast<T*>(x.param) + k;
   char* const m_at = static_cast<char*>(a.state.exp_avg) + state * kMoment;
   char* const v_at = static_cast<char*>(a.state.exp_avg_sq) + state * kMoment;
@@ -272,7 +276,7 @@ __device__ __forceinline__ void StepBlock(const StepFactors& a, const SmlAdamwTe
   }
   StoreTensor<kWhole>(param, valid, p);
   if constexpr (sizeof(T) == 2) {
-    if constexpr (!kWhole) {
+    if constexpr (kIs == Block::kEnd) {
 #pragma unroll
       for (int i = 0; i < 4; i++) r.w[i] = valid > 2 * i + 1 ? r.w[i] : valid > 2 * i ? r.w[i] & 0xffffu : 0;
     }
@@ -308,7 +312,7 @@ __device__ __forceinline__ void StepBlock(const StepFactors& a, const SmlAdamwTe
     }
     if (em == 255) m.w[0] = m.w[1] = kNanCode * 0x01010101u;
     if (ev == 255) v.w[0] = v.w[1] = kNanCode * 0x01010101u;
-    if constexpr (!kWhole) {
+    if constexpr (kIs == Block::kEnd) {
       const unsigned low = BytesBelow(valid), high = BytesBelow(valid - 4);
       m.w[0] &= low, m.w[1] &= high;
       v.w[0] &= low, v.w[1] &= high;
@@ -322,11 +326,11 @@ __device__ __forceinline__ void StepBlock(const StepFactors& a, const SmlAdamwTe
   StoreWords(v_at, v.w);
 }
 
-// For tensors at other addresses and for ends: out of the way of the other's registers and instructions.
-template <class T, int kBits, int kMax>  // (one for each kernel: ptxas 12.9 falls over one that two share)
+// For tensors at other addresses and for ends: out of the way of the first kind's registers and instructions.
+template <class T, int kBits, Block kIs, int kMax>  // (one for each kernel: ptxas 12.9 falls over one that two share)
 __device__ __noinline__ void StepAnyBlock(const StepFactors& a, const SmlAdamwTensor& x, long long k, long long state, Factors f,
                                           float clip, int lane) {
-  StepBlock<T, kBits, false>(a, x, k, state, f, clip, lane);
+  StepBlock<T, kBits, kIs>(a, x, k, state, f, clip, lane);
 }
 
 template <class T, int kBits, int kMax>
@@ -351,8 +355,9 @@ __global__ void __launch_bounds__(kThreads, kBits == 8 ? 7 : 8) AdamwKernel(cons
     const Factors f = FactorsOf(all, all.state.steps[x.step] + 1, lr);
     const bool vectors = ((reinterpret_cast<uintptr_t>(x.param) | reinterpret_cast<uintptr_t>(x.grad)) & (8 * sizeof(T) - 1)) == 0;
     for (long long k = start; k < end; k += kBlock) {
-      if (vectors && k + kBlock <= end) StepBlock<T, kBits, true>(all, x, k, state, f, clip, lane);
-      else StepAnyBlock<T, kBits, kMax>(all, x, k, state, f, clip, lane);
+      if (k + kBlock > end) StepAnyBlock<T, kBits, Block::kEnd, kMax>(all, x, k, state, f, clip, lane);
+      else if (vectors) StepBlock<T, kBits, Block::kVectors>(all, x, k, state, f, clip, lane);
+      else StepAnyBlock<T, kBits, Block::kSingles, kMax>(all, x, k, state, f, clip, lane);
     }
   }
   // The block that ends last counts the step: every block has read the counts by then.
