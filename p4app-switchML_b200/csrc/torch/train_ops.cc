@@ -43,7 +43,12 @@ void* Data(const Tensor& t) {
 }
 
 // For a kernel that writes: a lazy clone of the tensor gets its own memory first.
-void* Writable(const Tensor& t) { return Data(t) ? t.mutable_data_ptr() : nullptr; }
+void* Writable(const Tensor& t) {
+  if (!t.defined()) return nullptr;
+  void* const data = t.mutable_data_ptr();
+  TORCH_CHECK(data || !t.numel(), "a tensor of the shape ", t.sizes(), " has no memory");
+  return data;
+}
 
 // Whether the memory of a tensor does not hold its values: a view that says they are to be negated (imag() of a conjugate), or
 // zeros that autograd has not written out.
@@ -329,8 +334,8 @@ class Adamw {
     TORCH_CHECK(settings.size() == groups_.size() && lr_tensors.size() == groups_.size(), "FusedAdamW: groups have come or gone");
     const c10::cuda::OptionalCUDAGuard device(ticket_.device());
     at::NoGradGuard no_grad;
-    tensors_.clear(), norms_.clear();
-    std::vector<Tensor> keep, grads;
+    tensors_.clear(), norms_.clear(), stepped_.clear();
+    std::vector<Tensor> keep;
     struct Run { size_t begin, end; int type; };
     std::vector<std::pair<size_t, Run>> runs;  // of tensors whose gradients are of one type, by group
     for (size_t k = 0; k < groups_.size(); k++) {
@@ -340,16 +345,18 @@ class Adamw {
         for (size_t i = 0; i < g.params.size(); i++) {
           const Tensor& p = g.params[i];
           if (TypeOf(g, i) != type) continue;
-          Tensor grad = p.grad();
-          if (!grad.defined()) continue;
+          const Tensor* grad = &p.grad();
+          if (!grad->defined()) continue;
           CheckParam(g, i);
-          CheckGrad(p, grad);
-          if ((!(p.is_contiguous() && grad.is_contiguous()) && p.strides() != grad.strides()) || Implied(grad)) {
-            grad = at::empty_strided(p.sizes(), p.strides(), grad.options()).copy_(grad);
-            keep.push_back(grad);
+          CheckGrad(p, *grad);
+          if ((!(p.is_contiguous() && grad->is_contiguous()) && p.strides() != grad->strides()) || Implied(*grad)) {
+            keep.push_back(at::empty_strided(p.sizes(), p.strides(), grad->options()).copy_(*grad));
+            grad = &keep.back();
           }
-          tensors_.push_back({Writable(p), Data(grad), g.numel[i], static_cast<unsigned>(g.place[i]), static_cast<int>(i)});
-          if (max_norm) norms_.push_back({Data(grad), g.numel[i], type});
+          void* const grad_data = Data(*grad);
+          tensors_.push_back({Writable(p), grad_data, g.numel[i], static_cast<unsigned>(g.place[i]), static_cast<int>(i)});
+          stepped_.push_back(p.unsafeGetTensorImpl());
+          if (max_norm) norms_.push_back({grad_data, g.numel[i], type});
         }
         if (tensors_.size() > begin) runs.push_back({k, {begin, tensors_.size(), type}});
       }
@@ -365,11 +372,7 @@ class Adamw {
       Check(switchml_adamw_step(&tensors_[run.begin], static_cast<int>(run.end - run.begin), &state, &step, run.type, CurrentStream()),
             "FusedAdamW");
     }
-    for (const Group& g : groups_) {
-      for (const Tensor& p : g.params) {
-        if (p.grad().defined()) p.unsafeGetTensorImpl()->bump_version();
-      }
-    }
+    for (c10::TensorImpl* p : stepped_) p->bump_version();
   }
 
   // The fp32 values of a group's parameters, in the layout of its state.
@@ -432,6 +435,7 @@ class Adamw {
   size_t count_ = 0;                // of all parameters
   std::vector<SmlAdamwTensor> tensors_;
   std::vector<SmlNormTensor> norms_;
+  std::vector<c10::TensorImpl*> stepped_;  // parameters of this step
 };
 
 }  // namespace

@@ -175,7 +175,8 @@ class FusedAdamW(torch.optim.Optimizer):
                 loss = closure()
         settings, tensors = [], []
         for group in self.param_groups:
-            self._check_options(group)
+            if "amsgrad" in group or "maximize" in group or "differentiable" in group:
+                self._check_options(group)
             lr, (beta1, beta2), eps, decay = group["lr"], group["betas"], group["eps"], group["weight_decay"]
             tensor = isinstance(lr, torch.Tensor)
             now = (0.0 if tensor else lr, beta1, beta2, eps, decay)
