@@ -1,11 +1,11 @@
 // AdamW over many tensors in one launch, and the norm of all their gradients (adamw.h has the formulas).
 //
-// A launch takes its tensors' addresses and sizes as kernel parameters: nothing has to be copied to the device, a captured
-// launch keeps its own, and two of them share nothing. The parameters' memory is read through the constant cache; a warp
-// finds the tensor of its tile by halving.
+// A launch takes its tensors' addresses and sizes as kernel parameters: nothing has to be copied to the device, and a captured
+// launch keeps its own table. (Launches of one optimizer share its counts of steps, its ticket and the norm: they follow each
+// other.) The parameters' memory is read through the constant cache; a warp finds the tensor of its tile by halving.
 //
-// The step is one pass over memory: 28 bytes per value with fp32 parameters and moments, 16.06 with moments in 8 bits (bf16
-// parameters: 26 and 14.06). A lane takes 8 neighbours, whole sectors of every array; tiles go to the warps in the order of
+// The step is one pass over memory: 28 bytes per value with fp32 parameters and moments, 16.125 with moments in 8 bits (bf16
+// parameters: 26 and 14.125). A lane takes 8 neighbours, whole sectors of every array; tiles go to the warps in the order of
 // the addresses (blocks that stay and stride over the tiles: 1200 instead of 1096 us). 2^28 values:
 //   fp32, moments in 32 bits 1096 us = 6.86 TB/s, in 8 bits 669 us = 6.47 TB/s; bf16 1043 us = 6.69 and 655 us = 5.79 TB/s
 // (a plain copy: 6.55 TB/s). With 32 bits memory is the limit. With 8 bits it is nearly so: 51 instructions per value, of
@@ -41,6 +41,7 @@ int Launched(cudaError_t e) {
   return -4;
 }
 
+constexpr int kSms = 148;  // of a B200
 constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr int kBlock = SML_ADAMW_ALIGN;  // values that a warp takes at once: 8 per lane
 constexpr int kScaled = 32;              // values that share a scale
@@ -91,8 +92,8 @@ struct Factors {
 
 __device__ __forceinline__ Factors FactorsOf(const StepFactors& a, int t, float lr) {
   Factors f;
-  // 1 - beta^t = -expm1(t log beta): the logarithm comes from the host in more than fp32, and expm1 keeps what a
-  // difference from 1 would lose.
+  // 1 - beta^t = -expm1(t log beta): the host takes the logarithm in fp64 and rounds it to fp32 once (of a beta that was rounded
+  // first, 1 - beta would keep few of its bits), and expm1 keeps what a difference from 1 would lose.
   f.size = lr / -expm1f(t * a.log_beta1);
   f.rsqrt2 = 1.f / sqrtf(-expm1f(t * a.log_beta2));
   f.keep = 1.f - lr * a.decay;
@@ -326,7 +327,9 @@ __device__ __forceinline__ void StepBlock(const StepFactors& a, const SmlAdamwTe
   StoreWords(v_at, v.w);
 }
 
-// For tensors at other addresses and for ends: out of the way of the first kind's registers and instructions.
+// For tensors at other addresses and for ends: out of the way of the first kind's registers and instructions. (A value per load
+// and store: 2^25 values one element behind a multiple of 32 bytes take 172 us in fp32 with 32 bits and 132 with 8, where aligned
+// ones take 144 and 93, in bf16 166 and 126 for 139 and 89.)
 template <class T, int kBits, Block kIs, int kMax>  // (one for each kernel: ptxas 12.9 falls over one that two share)
 __device__ __noinline__ void StepAnyBlock(const StepFactors& a, const SmlAdamwTensor& x, long long k, long long state, Factors f,
                                           float clip, int lane) {
@@ -419,10 +422,12 @@ __global__ void __launch_bounds__(kThreads) MastersKernel(const __grid_constant_
 }
 
 constexpr int kNormThreads = 256;
-// Values that a block takes at once: 4 vectors per thread in flight. ResNet-50's 161 gradients, a bucket's 28 and 301 ragged
-// bf16 ones took 23.6, 7.9 and 11.8 us with 2048, 19.6, 6.6 and 9.1 with 4096, 19.4, 5.8 and 7.9 with 8192.
+// Values that a block takes at once: 4 vectors per thread in flight. Reading needs them, the more the shorter the type: with 2048,
+// 4096 and 8192 64 bf16 tensors of 2^20 values took 54, 37 and 30 us (fp32 56, 43 and 43), one of 2^22 4.9, 4.5 and 4.2, one of
+// 2^20 fp32 values 3.6, 3.3 and 3.1, 300 of 5000 5.2, 5.1 and 4.9. 2^28 values in one are best with 4096 (162, 150 and 158), tensors
+// far below a tile with the smallest (1000 of 1000: 8.6, 9.3 and 11.4).
 constexpr int kNormTile = 8192;
-constexpr int kNormBlocks = 148 * 5;  // partial sums of a launch, at most: the blocks that the GPU holds
+constexpr int kNormBlocks = kSms * 5;  // partial sums of a launch, at most: the blocks that the GPU holds
 
 template <int kMax> struct NormArgs {
   SmlNormTensor tensor[kMax];
@@ -539,7 +544,7 @@ unsigned TakeTensors(const Tensor* tensors, int count, long long tile, int* at, 
 // ones). Fewer values make smaller tiles: as many as the GPU holds warps, so that all run at once.
 int TileBlocks(const SmlAdamwTensor* tensors, int count, int bits) {
   const int most = bits == 8 ? 16 : 4;
-  const long long resident = 148ll * kWarps * (bits == 8 ? 7 : 8);
+  const long long resident = static_cast<long long>(kSms) * kWarps * (bits == 8 ? 7 : 8);
   long long blocks = 0;
   for (int i = 0; i < count; i++) blocks += (tensors[i].numel + kBlock - 1) / kBlock;
   for (long long tile = (blocks + resident - 1) / resident; tile < most; tile++) {

@@ -329,7 +329,7 @@ ForwardKernel(const T* x, const T* residual, Parameter weight, Parameter bias, T
 // The backward pass of rows that a group holds, and the sums over the rows that each block saw, in the order of the groups.
 // A block per SM goes through the rows; a group reads its next rows while it deals with one, so that the sums of weight and
 // bias stay in registers and only 148 partial ones meet. Bound by memory: 16384 x 8192 bf16 with the sum's gradient, 1.07 GB,
-// 165 us = 6.5 TB/s with the closing sums; on short inputs by its ends (8192 x 1024, 50 MB, 14.8 us: 7 rounds of rows, then 16
+// 165 us = 6.5 TB/s with the closing sums; on short inputs by its ends (8192 x 1024, 50 MB, 14.8 us: 7 rounds of rows, then 8
 // groups' sums). Single values: 16384 x 2047 99 us. Rows of a cluster: 8192 x 12000 255 us (one pass for the input's gradient and
 // one for the columns: 539).
 // Sums, normalised values, gradients and what is read ahead take 6 to 8 registers per value: 16 bf16 values in vectors fit
@@ -718,11 +718,12 @@ struct Geometry {
   int Threads() const { return lanes == 8 ? groups * 8 : groups * warps * 32; }
 };
 
+constexpr int kSms = 148;  // of a B200
 constexpr int kForwardWarps = 8;  // of a block, where a row does not need more
 
 Geometry BackwardGeometry(long long rows, int n, int held) {
   const int warps = BackwardThreads(held) / 32;
-  return Geometry(rows, n, held, warps, warps, 148);
+  return Geometry(rows, n, held, warps, warps, kSms);
 }
 
 // The type of weight and bias, for kernels that want to know it.

@@ -18,8 +18,8 @@ from .._native import native_extension
 
 _MOMENTS = ("exp_avg", "exp_avg_sq")
 _SCALED = 32  # values that share a scale
-# Options of torch.optim.AdamW that would make another step: a group that has one, from a checkpoint say, is refused. (The others say
-# how it computes, or, as decoupled_weight_decay, are set aside by torch.optim.AdamW too.)
+# Options of torch.optim.AdamW that would make another step: a group that has one, from a checkpoint say, is refused. (The others
+# choose between ways to the same result, or, as decoupled_weight_decay, are set right by torch.optim.AdamW too.)
 _OTHER_STEPS = ("amsgrad", "maximize", "differentiable")
 
 
@@ -67,7 +67,8 @@ class FusedAdamW(torch.optim.Optimizer):
 
     @property
     def grad_norm(self):
-        """The norm of the last step's gradients (a tensor on the device), None without `max_norm`."""
+        """The norm of the last step's gradients, None without `max_norm`: always the same tensor on the device, which every step
+        and every replay of a captured one writes anew. ``.clone()`` keeps a value."""
         return self._native.norm if self._max_norm is not None else None
 
     def add_param_group(self, group):
