@@ -682,8 +682,8 @@ unsigned RowBlocks(long long rows) { return static_cast<unsigned>(rows < (1 << 2
 // Columns are counted in 32 bits, beyond a row's end too.
 bool Fits(int features) { return features > 0 && features <= 1 << 30; }
 
-// Whether all of them lie at multiples of their element (null does).
-template <class... Pointers> bool Aligned(unsigned size, Pointers... p) { return ((reinterpret_cast<uintptr_t>(p) % size == 0) && ...); }
+// Whether all of them lie at multiples of their element, a power of two (null does).
+template <class... Pointers> bool Aligned(unsigned size, Pointers... p) { return ((reinterpret_cast<uintptr_t>(p) | ...) & (size - 1)) == 0; }
 unsigned SizeOf(int type) { return type == SML_NORM_F32 ? 4 : 2; }
 
 bool Known(int type) { return type == SML_NORM_F32 || type == SML_NORM_BF16; }

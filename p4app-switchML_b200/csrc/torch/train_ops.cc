@@ -5,6 +5,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
@@ -52,7 +53,9 @@ void* Writable(const Tensor& t) {
 
 // Whether the memory of a tensor does not hold its values: a view that says they are to be negated (imag() of a conjugate), or
 // zeros that autograd has not written out.
-bool Implied(const Tensor& t) { return t.is_neg() || t._is_zerotensor(); }
+bool Implied(const Tensor& t) {
+  return t.key_set().has_any(c10::DispatchKeySet{c10::DispatchKey::Negative, c10::DispatchKey::ZeroTensor});
+}
 
 Tensor Written(const Tensor& t) { return at::zeros(t.sizes(), t.options()).copy_(t); }
 
@@ -70,6 +73,9 @@ void RefuseTracing(const char* what) {
                               TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FAKE).has_value())),
               what, " cannot be traced");
 }
+
+// Dual tensors are such while a level of forward mode is open: asked once per call, since to ask a view looks at its base.
+bool DualsExist() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
 
 void RefuseDual(const Tensor& t, const char* what) {
   TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), what, " has no forward-mode gradient");
@@ -153,7 +159,9 @@ struct LayerNormBackward : public torch::autograd::Node {
   variable_list apply(variable_list&& grads) override {
     RefuseTracing("layer_norm");
     TORCH_CHECK(!at::GradMode::is_enabled(), "layer_norm has no gradient of its gradient (create_graph)");
-    for (const Tensor& t : grads) RefuseDual(t, "layer_norm");
+    if (DualsExist()) {
+      for (const Tensor& t : grads) RefuseDual(t, "layer_norm");
+    }
     std::lock_guard<std::mutex> lock(mutex_);
     const c10::cuda::OptionalCUDAGuard device(where);
     const int64_t n = sizes.back(), rows = c10::multiply_integers(sizes) / n;
@@ -197,7 +205,9 @@ struct LayerNormBackward : public torch::autograd::Node {
 variable_list LayerNormForward(Tensor x, OptTensor residual, const OptTensor& weight, const OptTensor& bias, double eps) {
   RefuseTracing("layer_norm");
   // (A dual tensor need not require a gradient: this is asked whether a backward pass comes or not.)
-  for (const Tensor& t : {x, residual.value_or(Tensor()), weight.value_or(Tensor()), bias.value_or(Tensor())}) RefuseDual(t, "layer_norm");
+  if (DualsExist()) {
+    for (const Tensor& t : {x, residual.value_or(Tensor()), weight.value_or(Tensor()), bias.value_or(Tensor())}) RefuseDual(t, "layer_norm");
+  }
   const bool autocast = x.is_cuda() && at::autocast::is_autocast_enabled(at::kCUDA);
   c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::DispatchKey::AutocastCUDA);
   if (autocast) {
@@ -265,7 +275,7 @@ Tensor GradNorm(const py::list& tensors) {
   std::vector<Tensor> keep;
   list.reserve(count);
   at::Device where(at::kCPU);
-  const bool grad_mode = at::GradMode::is_enabled();
+  const bool grad_mode = at::GradMode::is_enabled(), duals = DualsExist();
   at::NoGradGuard no_grad;
   std::optional<c10::cuda::CUDAGuard> device;
   for (Py_ssize_t i = 0; i < count; i++) {
@@ -274,7 +284,7 @@ Tensor GradNorm(const py::list& tensors) {
     const Tensor* t = &THPVariable_Unpack(item);
     TORCH_CHECK_TYPE(t->layout() == at::kStrided && Known(*t), "grad_norm: a tensor is ", t->layout(), " ", t->scalar_type(),
                      ": strided float32 or bfloat16 is wanted");
-    RefuseDual(*t, "grad_norm");
+    if (duals) RefuseDual(*t, "grad_norm");
     TORCH_CHECK(!grad_mode || !t->requires_grad(),
                 "grad_norm has no gradient: a tensor that requires one is wanted detached, or the call under no_grad");
     if (i == 0) where = t->device();
