@@ -612,7 +612,9 @@ BackwardAnyKernel(const T* dy, const T* dsum, const T* s, Parameter weight, cons
 }
 
 // Sums over rows: a block takes 32 columns, a warp every 8th row of them. Rows that no cluster holds have more than 65536 values, so
-// there are more than 2048 blocks, and shares of the rows would find no SM free.
+// there are more than 2048 blocks, and shares of the rows would find no SM free. A thread reads four rows before it adds one (4000 x
+// 70001, the whole backward pass: 1626 us in fp32 and 1350 in bf16; eight 1668 and 1439, a plain loop that the compiler unrolls 1706
+// to 1944 and 1458 to 1714).
 template <class T>
 __global__ void __launch_bounds__(kAnyThreads)
 ColumnsAnyKernel(const T* dy, const T* s, const float* mean, const float* rstd, float* workspace, long long rows, int n) {
@@ -621,12 +623,20 @@ ColumnsAnyKernel(const T* dy, const T* s, const float* mean, const float* rstd, 
   float dw = 0.f, db = 0.f;
   WaitForEarlierKernels();
   if (column < n) {
-#pragma unroll 4
-    for (long long row = warp; row < rows; row += kAnyThreads / 32) {
-      const float g = ToFloat(dy[row * n + column]);
-      dw += g * ((ToFloat(s[row * n + column]) - mean[row]) * rstd[row]);
-      db += g;
+    const auto add = [&](T g, T v, long long row) {
+      dw += ToFloat(g) * ((ToFloat(v) - mean[row]) * rstd[row]);
+      db += ToFloat(g);
+    };
+    constexpr int kRows = 4, kStep = kAnyThreads / 32;
+    long long row = warp;
+    for (; row + (kRows - 1) * kStep < rows; row += kRows * kStep) {
+      T g[kRows], v[kRows];
+#pragma unroll
+      for (int i = 0; i < kRows; i++) g[i] = dy[(row + i * kStep) * n + column], v[i] = s[(row + i * kStep) * n + column];
+#pragma unroll
+      for (int i = 0; i < kRows; i++) add(g[i], v[i], row + i * kStep);
     }
+    for (; row < rows; row += kStep) add(dy[row * n + column], s[row * n + column], row);
   }
   part[warp][lane] = make_float2(dw, db);
   __syncthreads();
