@@ -8,7 +8,7 @@
 // parameters: 26 and 14.125). A lane takes 8 neighbours, whole sectors of every array; tiles go to the warps in the order of
 // the addresses (blocks that stay and stride over the tiles: 1200 instead of 1096 us). 2^28 values:
 //   fp32, moments in 32 bits 1096 us = 6.86 TB/s, in 8 bits 669 us = 6.47 TB/s; bf16 1043 us = 6.69 and 655 us = 5.79 TB/s
-// (a plain copy: 6.55 TB/s). With 32 bits memory is the limit. With 8 bits it is nearly so: 51 instructions per value, of
+// (a plain copy: 6.55 TB/s). With 32 bits memory is the limit. With 8 bits it is nearly so: 53 instructions per value, of
 // which hashing takes 9 and each of the two codes 6; one value per lane took 4 times, scalar arithmetic 1.4 times as long. Reading
 // the next block ahead gained 1 % there (bf16: 5 %) and lost as much with 32 bits and on a few million values.
 #include <cuda_bf16.h>

@@ -4,6 +4,7 @@ import ctypes
 import pytest
 import torch
 import torch.utils.checkpoint
+from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from _train_reference import check, layer_norm64
@@ -522,8 +523,13 @@ def test_gradients_of_zeros_that_are_not_written_out():
 
 
 def test_weight_without_memory_is_refused():
-    """It must not count as one that is not there."""
+    """It must not count as one that is not there: storage given up, a fake tensor outside of its mode, a functionalised one."""
     x, weight = torch.randn(4, 64, device="cuda"), torch.randn(64, device="cuda")
+    fake = FakeTensorMode().from_tensor(weight)
+    with pytest.raises(RuntimeError, match="no memory"):
+        layer_norm(x, fake)
+    with pytest.raises(RuntimeError, match="no memory"):
+        torch.func.functionalize(lambda w: layer_norm(x, w))(weight)
     weight.untyped_storage().resize_(0)
     with pytest.raises(RuntimeError, match="no memory"):
         layer_norm(x, weight)
